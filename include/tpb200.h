@@ -61,8 +61,10 @@ const char *tpb_status_string(int status);
 
 /* Reads (and clears) the device status word that bounded waits inside the
  * kernels write when they give up.  Synchronises `stream` first.  Returns
- * TPB_OK or TPB_ERR_TIMEOUT; *detail (optional) receives the raw word:
- * (role << 24) | stage, role 1 = tile loader, 2 = MMA issuer, 3 = epilogue. */
+ * TPB_OK, TPB_ERR_TIMEOUT or TPB_ERR_STATE; *detail (optional) receives the raw word:
+ * (role << 24) | stage, role 1 = tile loader, 2 = MMA issuer, 3 = epilogue.  A role of 32 or
+ * more is no wait that ran out but a key / value cache whose contents do not fit the call
+ * (stage 1 = sequence id, 2 = page, 3 = length, 4 = rows that are not the last extension's): TPB_ERR_STATE. */
 int tpb_status_poll(tpb_handle_t h, tpb_stream_t stream, uint32_t *detail);
 
 /* Device facts the host side sizes its work with. */
@@ -435,6 +437,104 @@ int tpb_attn_prepare(tpb_handle_t h, tpb_stream_t stream, const void *q, const v
 int tpb_attention(tpb_handle_t h, tpb_stream_t stream, void *out, int out_dtype, const void *qb,
                   const void *kb, const void *vt, int64_t seq_q, int64_t seq_kv, int heads,
                   int kv_heads, int head_dim, float scale);
+
+/* ---- Causal attention over packed prompts --------------------------------------------
+ * Stands where the reference's text models attend over a whole prompt (src/models/qwen3_cuda.zig; CPU definition
+ * src/ops/attention.zig:46-150), for any number of prompts in one call:
+ *   out[i] = sum_{j <= i} softmax_j(scale * q[i] . k[j]) v[j]      j over the tokens of i's own sequence, kv head = head / (heads / kv_heads)
+ * q and out [tokens][heads * head_dim], k and v [tokens][kv_heads * head_dim], all of `dtype` (TPB_BF16 or TPB_F16), rows ld_* elements
+ * apart (so q, k and v may be parts of one fused projection's output).  Sequence s holds the tokens cu[s] .. cu[s+1] - 1; cu is a
+ * device array of n_seqs + 1 ascending offsets (values outside 0 .. tokens are clamped, an empty sequence is skipped).  Rows of `out` in
+ * no sequence are left as they were, and what k and v hold there, or at places that a row's mask hides, is never part of a result:
+ * NaN and infinities included.  A NaN or infinity at a visible place follows the formula.
+ * head_dim 64 or 128; heads a multiple of kv_heads and at most 128 times as many; pointers 16-byte aligned, ld_* multiples of 8
+ * elements, kv_heads below 65536, scale finite and not negative.  out must not overlap the inputs.  f32 scores and sums; probabilities are rounded to `dtype` for the
+ * second product. */
+int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t ld_out, const void *q, int64_t ld_q,
+                         const void *k, int64_t ld_k, const void *v, int64_t ld_v, int dtype, const int32_t *cu, int n_seqs,
+                         int64_t tokens, int heads, int kv_heads, int head_dim, float scale);
+
+/* ---- Key / value cache in 8 bits, in pages ---------------------------------------------
+ * The decode half of the same models: stands where the reference keeps its cache (src/core/kv_cache.zig) and attends over it
+ * (decode kernels of src/gpu/cuda/elt.zig), in 8 bits a value and with pages that sequences can share.
+ *
+ * A cache is memory that the caller owns, described by a tpb_kv_cache (a plain struct, read during each call; the calls below
+ * keep nothing of it).  All pointers are device memory:
+ *   k, v              [layers][n_pages][kv_heads][page_tokens][head_dim], one byte a value, 16-byte aligned
+ *   k_scale, v_scale  [layers][n_pages][kv_heads] f32: a value stands for q * scale.  A block -- the tokens of one page, one head -- has one scale
+ *   table             [max_seqs][max_pages] the pages of each sequence, in order; -1 behind them
+ *   lens              [max_seqs] tokens of each sequence (0 = the sequence is free)
+ *   tail              [max_seqs] tokens that the last tpb_kv_extend gave the sequence; 0 after a truncation or a fork
+ *   refs              [n_pages] how many sequences hold the page; 0 = free
+ *   result            [4] what the last page operation (extend, truncate, fork, compact) says, for the host to read when it likes:
+ *                     {tpb_status, free pages after it, pages taken from the free ones (compact: pages moved), pages it needed}
+ *   scratch           tpb_kv_scratch_bytes(...) bytes, 16-byte aligned
+ * An empty cache: table all -1, lens, tail and refs all 0.  A page that more than one sequence holds is always full (fork copies the
+ * part-filled page, truncate makes a private copy of a shared page that it cuts), so new tokens never touch another sequence.
+ *
+ * Everything is decided on the device: no call synchronises, and all of them can be captured into a graph and replayed as lengths grow.  Calls on
+ * one cache are ordered by the caller (one stream, or events), as for any memory; different caches are independent.
+ * A page operation either happens as a whole or, with result[0] != TPB_OK, changes nothing (but sets the listed sequences' tail to 0
+ * where it is an extension): TPB_ERR_OOM = not enough free pages, TPB_ERR_INVALID_ARG = a sequence id out of range or listed twice, a
+ * length that does not fit, a fork onto a sequence in use.  A kernel that meets an id, a page or a length out of range skips it and sets the
+ * status word: tpb_status_poll then returns TPB_ERR_STATE. */
+typedef enum tpb_kv_format { TPB_KV_S8 = 0, TPB_KV_E4M3 = 1 } tpb_kv_format;
+typedef struct tpb_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t *table, *lens, *tail, *refs, *result, *scratch;
+    int64_t n_pages;      /* 1 .. 2^24 */
+    int32_t layers;       /* layers * n_pages * kv_heads * page_tokens below 2^31 */
+    int32_t kv_heads;
+    int32_t page_tokens;  /* 16, 32 or 64 */
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t max_seqs, max_pages;  /* max_pages * page_tokens below 2^31, max_seqs * max_pages below 2^31 */
+    int32_t format;       /* tpb_kv_format */
+} tpb_kv_cache;
+
+/* 0 for sizes out of range. */
+size_t tpb_kv_scratch_bytes(int64_t n_pages, int max_seqs);
+
+/* Page operations.  seqs, n_new, new_lens, src, dst: device arrays of n ids / counts; a sequence is listed at most once per call (src of a
+ * fork: as often as wanted).  Pages are taken lowest index first, in the order of the list.
+ *   extend    gives sequence seqs[i] room for n_new[i] more tokens and sets its tail to n_new[i]: lens counts them from here on, and
+ *             tpb_kv_append then fills them in, layer by layer.
+ *   truncate  cuts sequence seqs[i] to new_lens[i] tokens (rejected drafts; not more than it has) or, with new_lens = NULL, frees it.  A cut
+ *             inside a page that other sequences hold as well takes a free page for the rest of it.
+ *   fork      makes the free sequence dst[i] a copy of src[i].  share != 0: it holds src's full pages too, and has a copy of the
+ *             part-filled one; share = 0: it gets a copy of every page.
+ *   compact   moves the pages in use to the lowest indices: with L pages in use, the i-th page in use at or above L moves into the
+ *             i-th free one below L.  Afterwards pages L .. n_pages - 1 are free. */
+int tpb_kv_extend(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, const int32_t *seqs, const int32_t *n_new, int n);
+int tpb_kv_truncate(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, const int32_t *seqs, const int32_t *new_lens, int n);
+int tpb_kv_fork(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, const int32_t *src, const int32_t *dst, int n, int share);
+int tpb_kv_compact(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c);
+
+/* A batch names sequences (seqs[i], each at most once) and rows of a packed tensor: sequence seqs[i] owns the rows cu[i] .. cu[i+1] - 1 (cu:
+ * n_seqs + 1 ascending offsets).  dtype: TPB_F32, TPB_BF16 or TPB_F16; rows ld elements apart, 16-byte aligned.
+ *
+ * append   quantises the rows of k and v into the last cu[i+1] - cu[i] places of the sequence, which must be as many as its tail.  A block's
+ *          scale is the smallest power of two, at least 2^-100, with amax <= limit * scale (limit: s8 127, e4m3 448) over the values that
+ *          are added; a block that holds earlier tokens keeps its scale or takes a larger one, and what it holds is rounded again,
+ *          rn(q * old / new).  (The largest f32 values, above limit * 2^(127 - p) with p = 6 for s8 and 8 for e4m3, saturate there.)
+ *          Powers of two make both quotients exact, so a value is rounded once for every doubling of its block's
+ *          scale and by nothing else (s8: at most one step in all; e4m3: only what falls below its normal range).
+ *          A block with a NaN or infinity among its values gets the scale NaN.
+ * read     the other way: the tokens start[i] .. start[i] + cu[i+1] - cu[i] - 1 of each sequence (start = NULL: from 0) as values; places
+ *          behind the sequence's end read as zero.
+ * attention  rows are the queries of the sequence's last cu[i+1] - cu[i] tokens, causal among themselves:
+ *          out[r] = sum_{j <= p(r)} softmax_j(scale * q[r] . k[j]) v[j],  p(r) = lens - (cu[i+1] - r); zero where p(r) < 0.
+ *          heads a multiple of kv_heads, scale finite and not negative.  f32 accuracy: q and the probabilities are split in two f16 terms, the cache's values are exact.
+ *          max_len: an upper bound of the lengths that the host knows (0 = none): a hint that saves a launch for short sequences.
+ *          workspace: tpb_kv_attention_workspace_bytes(h, head_dim) bytes, 16-byte aligned, of this call alone while it runs. */
+int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, const void *k, int64_t ld_k, const void *v,
+                  int64_t ld_v, int dtype, const int32_t *seqs, const int32_t *cu, int n_seqs, int64_t rows);
+int tpb_kv_read(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, void *k, int64_t ld_k, void *v, int64_t ld_v,
+                int dtype, const int32_t *seqs, const int32_t *start, const int32_t *cu, int n_seqs, int64_t rows);
+size_t tpb_kv_attention_workspace_bytes(tpb_handle_t h, int head_dim);
+int tpb_kv_attention(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, void *out, int64_t ld_out, const void *q,
+                     int64_t ld_q, int dtype, const int32_t *seqs, const int32_t *cu, int n_seqs, int64_t rows, int heads, float scale,
+                     int64_t max_len, void *workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libtpb200.so")
 # built for one interpreter: the suffix names its ABI, so that another one does not load it
 CALL_PATH = os.path.join(_HERE, "lib", "_tpbcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+ATTN_CALL_PATH = os.path.join(_HERE, "lib", "_tpbattncall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 TPB_OK = 0
 TPB_ERR_INVALID_ARG = -1
@@ -25,6 +26,7 @@ TPB_ERR_STATE = -5
 TPB_ERR_NO_DEVICE = -6
 
 TPB_F32, TPB_BF16, TPB_F16, TPB_S32 = 0, 1, 2, 3
+KV_FORMAT = {"s8": 0, "e4m3": 1}
 GGUF_FMT = {"q8_0": 0, "q4_0": 1, "q4_k": 2, "q5_k": 3, "q6_k": 4, "iq4_nl": 5}
 
 _vp, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
@@ -74,6 +76,16 @@ SIGNATURES = {
     "tpb_attn_vt_elems": (_sz, [_i64, _i]),
     "tpb_attn_prepare": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _f, _vp, _vp, _i64, _i, _i, _i, _vp, _vp, _vp]),
     "tpb_attention": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _i, _i, _i, _f]),
+    "tpb_attention_packed": (_i, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i, _i64, _i, _i, _i, _f]),
+    "tpb_kv_scratch_bytes": (_sz, [_i64, _i]),
+    "tpb_kv_extend": (_i, [_vp, _vp, _vp, _vp, _vp, _i]),
+    "tpb_kv_truncate": (_i, [_vp, _vp, _vp, _vp, _vp, _i]),
+    "tpb_kv_fork": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i]),
+    "tpb_kv_compact": (_i, [_vp, _vp, _vp]),
+    "tpb_kv_append": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _i64]),
+    "tpb_kv_read": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _i64]),
+    "tpb_kv_attention_workspace_bytes": (_sz, [_vp, _i]),
+    "tpb_kv_attention": (_i, [_vp, _vp, _vp, _i, _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _i64, _i, _f, _i64, _vp, _sz]),
     "tpb_peer_alloc": (_i, [_vp, _sz, C.POINTER(_vp), _vp]),
     "tpb_peer_open": (_i, [_vp, _vp, C.POINTER(_vp)]),
     "tpb_peer_close": (_i, [_vp, _vp]),
@@ -86,6 +98,13 @@ SIGNATURES = {
     "tpb_convrot_gemm_allgather": (_i, [_vp, _vp, C.POINTER(_vp), _i, _i, _i, _i64, _vp, _vp, _vp, _vp, _i, _vp,
                                         _i64, _i64, _i64]),
 }
+
+
+class KvCacheDesc(C.Structure):
+    """struct tpb_kv_cache."""
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "table", "lens", "tail", "refs", "result", "scratch")] + [
+        ("n_pages", _i64)] + [(n, C.c_int32) for n in ("layers", "kv_heads", "page_tokens", "head_dim", "max_seqs", "max_pages", "format")]
+
 
 _lib = None
 
@@ -134,6 +153,18 @@ class CtypesCalls:
         return rc
 
 
+def _load_extension(name: str, path: str):
+    """The CPython extension at ``path``; where it is not built for this interpreter, its calls through ctypes, with the same arguments
+    and results."""
+    lib = load()
+    if not os.path.exists(path):
+        return CtypesCalls(lib)
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    calls = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(calls)
+    return calls
+
+
 _calls = None
 
 
@@ -143,13 +174,16 @@ def load_calls():
     interpreter the calls are made through ctypes, with the same arguments and results."""
     global _calls
     if _calls is None:
-        lib = load()
-        if os.path.exists(CALL_PATH):
-            loader = importlib.machinery.ExtensionFileLoader("_tpbcall", CALL_PATH)
-            spec = importlib.util.spec_from_loader("_tpbcall", loader)
-            calls = importlib.util.module_from_spec(spec)
-            loader.exec_module(calls)
-        else:
-            calls = CtypesCalls(lib)
-        _calls = calls
+        _calls = _load_extension("_tpbcall", CALL_PATH)
     return _calls
+
+
+_attn_calls = None
+
+
+def load_attn_calls():
+    """The calls made once per layer: attention over prompts and over the key / value cache (csrc/pycall_attn.c)."""
+    global _attn_calls
+    if _attn_calls is None:
+        _attn_calls = _load_extension("_tpbattncall", ATTN_CALL_PATH)
+    return _attn_calls

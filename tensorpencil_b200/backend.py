@@ -56,6 +56,7 @@ class Backend:
         self.h = h
         # for the calls made once per weight: native argument passing, and the raw handle and device index it takes
         self._calls = _lib.load_calls()
+        self._attn_calls = _lib.load_attn_calls()
         self._hv = h.value
         self._index = device
         # prep -> GEMM state (backend.zig:336-341)
@@ -292,6 +293,40 @@ class Backend:
                                            seq, seq, heads, kv_heads, head_dim,
                                            float(scale if scale is not None else head_dim ** -0.5)))
         self.launches += 2
+        return out
+
+    def attentionPacked(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, heads: int, kv_heads: int,
+                        head_dim: int = 128, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of whole prompts, packed one behind another: sequence s is the rows cu[s] .. cu[s + 1] - 1 (cu: int32, on the
+        device).  q [tokens][heads*hd], k / v [tokens][kv_heads*hd], all bf16 or all f16, contiguous within a row (parts of a fused
+        projection's output may be passed as they are); head_dim 64 or 128.  The result has q's type; rows in no sequence are not
+        written."""
+        tokens = q.shape[0]
+        if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("attentionPacked: q, k and v must all be bfloat16 or all float16")
+        if cu.dtype != torch.int32:
+            raise TypeError(f"attentionPacked: cu must be int32 (got {cu.dtype})")
+        if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous() or cu.device != self.device:
+            raise ValueError(f"attentionPacked: cu must be a contiguous vector on {self.device}")
+        if out is None:
+            out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
+        elif out.dtype != q.dtype:
+            raise TypeError("attentionPacked: the output must have q's dtype")
+        ld = []
+        for name, t, h in (("q", q, heads), ("k", k, kv_heads), ("v", v, kv_heads), ("out", out, heads)):
+            s = t.shape
+            if t.device != self.device or s[0] != tokens or not (
+                    (len(s) == 2 and s[1] == h * head_dim and t.stride(1) == 1) or
+                    (len(s) == 3 and s[1] == h and s[2] == head_dim and t.stride(2) == 1 and (t.stride(1) == head_dim or h == 1))):
+                raise ValueError(f"attentionPacked: {name} must be [{tokens}][{h * head_dim}] on {self.device}, contiguous within a row "
+                                 f"(got {tuple(s)}, strides {t.stride()})")
+            ld.append(max(t.stride(0), h * head_dim) if tokens <= 1 else t.stride(0))
+        rc = self._attn_calls.tpb_attention_packed(self._hv, self._stream(), out.data_ptr(), ld[3], q.data_ptr(), ld[0], k.data_ptr(), ld[1],
+                                              v.data_ptr(), ld[2], _TORCH_TO_TPB[q.dtype], cu.data_ptr(), cu.shape[0] - 1, tokens, heads,
+                                              kv_heads, head_dim, float(scale) if scale is not None else head_dim ** -0.5)
+        if rc != TPB_OK:
+            self._check(rc)
+        self.launches += 1
         return out
 
     def _gemm(self, y: torch.Tensor, w_bytes: np.ndarray, weight_scale: np.ndarray, rows: int,

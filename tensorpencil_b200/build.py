@@ -15,7 +15,7 @@ import subprocess
 import sys
 import sysconfig
 
-from ._lib import CALL_PATH
+from ._lib import ATTN_CALL_PATH, CALL_PATH
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -24,8 +24,9 @@ OUT_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(OUT_DIR, "libtpb200.so")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 PYCALL_SRC = os.path.join(CSRC, "pycall.c")
+PYCALL_ATTN_SRC = os.path.join(CSRC, "pycall_attn.c")
 
-SOURCES = ["api.cu", "prep.cu", "prep_fused.cu", "gemm_i8.cu", "gemm2_i8.cu", "gemm_splitk.cu", "gemm_w4.cu", "qgemv.cu", "qgemv_mma.cu", "qgemv_k.cu", "qgemv_kmma.cu", "offload.cu", "peer.cu", "attn.cu"]
+SOURCES = ["api.cu", "prep.cu", "prep_fused.cu", "gemm_i8.cu", "gemm2_i8.cu", "gemm_splitk.cu", "gemm_w4.cu", "qgemv.cu", "qgemv_mma.cu", "qgemv_k.cu", "qgemv_kmma.cu", "offload.cu", "peer.cu", "attn.cu", "attn_packed.cu", "kv_pages.cu", "kv_cache.cu", "kv_attn.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -50,15 +51,15 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_pycall(out: str, lib_dir: str) -> bool:
-    """The CPython entry to the hot calls (csrc/pycall.c) for the running interpreter, linked to lib_dir/libtpb200.so, by the compiler that
+def build_pycall(out: str, lib_dir: str, src: str = PYCALL_SRC) -> bool:
+    """A CPython entry to the hot calls (csrc/pycall.c, csrc/pycall_attn.c) for the running interpreter, linked to lib_dir/libtpb200.so, by the compiler that
     nvcc drives.  Without Python's headers it is left out, and the calls go through ctypes (_lib.load_calls)."""
     inc = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(inc, "Python.h")):
         sys.stderr.write(f"{inc}/Python.h not found: {os.path.basename(out)} is not built, calls go through ctypes\n")
         return False
     subprocess.run([_nvcc(), "-O2", "-Xcompiler", "-fPIC,-Wall", "-shared", "-cudart", "none", "-I", inc,
-                    "-I", os.path.join(ROOT, "include"), PYCALL_SRC, "-o", out, "-L", lib_dir, "-Xlinker", "-l:libtpb200.so",
+                    "-I", os.path.join(ROOT, "include"), src, "-o", out, "-L", lib_dir, "-Xlinker", "-l:libtpb200.so",
                     "-Xlinker", "-rpath,$ORIGIN"], check=True)
     return True
 
@@ -92,8 +93,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [nvcc, "-shared", "-o", LIB] + objs + ["-cudart", "static",
                                                      "-Xlinker", "--no-undefined"]
         subprocess.run(cmd, check=True, env=env)
-    if force or _stale(CALL_PATH, [PYCALL_SRC, headers[0]]):
-        build_pycall(CALL_PATH, OUT_DIR)
+    for out, src in ((CALL_PATH, PYCALL_SRC), (ATTN_CALL_PATH, PYCALL_ATTN_SRC)):
+        if force or _stale(out, [src, headers[0]]):
+            build_pycall(out, OUT_DIR, src)
     return LIB
 
 

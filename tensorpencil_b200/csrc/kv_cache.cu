@@ -1,0 +1,260 @@
+// Writing the 8-bit key / value cache and reading it back.
+//
+// A block -- the tokens of one page, one head -- has one scale, a power of two, so that the quotients value / scale and old scale / new scale are exact
+// in f32: quantising is one rounding (to int8, or to e4m3), and a block whose scale has to grow is rounded again by a shift.
+#include "kv_common.cuh"
+
+using namespace tpb_kv;
+
+namespace {
+
+// The smallest power of two s >= 2^-100 with amax <= limit * s, amax finite: limit = top * 2^p, 1 <= top < 2, so s has amax's exponent less
+// p, and one more where amax's mantissa is above top's.  At most 2^(127 - p): a larger one would let the largest f32 values round to 2^128; they
+// saturate at limit * 2^(127 - p) instead.
+template <int FORMAT>
+__device__ __forceinline__ float pow2_scale(float amax) {
+    constexpr int p = FORMAT == TPB_KV_S8 ? 6 : 8;                           // 127 = 0x1.fcp6, 448 = 0x1.cp8
+    constexpr uint32_t top = FORMAT == TPB_KV_S8 ? 0x7e0000u : 0x600000u;
+    const uint32_t b = __float_as_uint(amax);
+    const int e = (int)(b >> 23) - 127 - p + ((b & 0x7fffffu) > top ? 1 : 0);  // a subnormal amax gives an e below -100
+    return __uint_as_float((uint32_t)(min(max(e, -100), 127 - p) + 127) << 23);
+}
+
+// One CTA per (sequence, page it touches, head): threads 0-127 the keys, 128-255 the values, each with up to CHUNKS pieces of 16 values in
+// registers between the maximum and the rounding, so that the input is read once.  Bound by HBM for prompts, by the chain offsets ->
+// length -> page -> scale for a decode step.
+//
+// Grid x: sequence i has at least as many places as it can touch pages from cu[i] / page_tokens + 2 i on, so that a CTA finds its
+// sequence by a search and the launch needs no lengths on the host.
+template <typename T, int FORMAT, int HD, int CHUNKS>
+__global__ void __launch_bounds__(256)
+kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, const T *v, int64_t ld_v, const int32_t *seqs, const int32_t *cu,
+                 int n_seqs, int rows, uint32_t *status) {
+    __shared__ float s_max[8];
+    __shared__ int s_bad[8];
+    tpb_grid_dep_launch();
+    tpb_grid_dep_wait();
+    const int pt = c.page_tokens, x = (int)blockIdx.x, head = (int)blockIdx.y;
+    const int i = find_last(n_seqs, x, [&](int j) { return row_offset(cu, j, rows) / pt + 2 * j; });
+    const int r0 = row_offset(cu, i, rows), n_new = row_offset(cu, i + 1, rows) - r0;
+    if (n_new <= 0) return;
+    const int seq = __ldcg(seqs + i);
+    if (seq < 0 || seq >= c.max_seqs) {
+        report(status, kBadSeq);
+        return;
+    }
+    const int len = __ldcg(c.lens + seq);
+    if (len < n_new || (long long)len > (long long)c.max_pages * pt) {
+        report(status, kBadLen);
+        return;
+    }
+    if (__ldcg(c.tail + seq) != n_new) {
+        report(status, kBadTail);
+        return;
+    }
+    const int first = len - n_new;
+    const long long pg = (long long)first / pt + (x - (r0 / pt + 2 * i));
+    if (pg * pt >= len) return;
+    const int page = __ldcg(c.table + (size_t)seq * c.max_pages + pg);
+    if (page < 0 || page >= c.n_pages) {
+        report(status, kBadPage);
+        return;
+    }
+    const int p0 = (int)pg * pt;                                // position of the page's first slot
+    const int held = max(first - p0, 0), fill = min(len - p0, pt);   // slots [0, held) hold earlier tokens, [held, fill) are written
+    const bool is_v = threadIdx.x >= 128;
+    const int t = threadIdx.x & 127;
+    const T *src = (is_v ? v : k) + (int64_t)(r0 + p0 - first) * (is_v ? ld_v : ld_k) + (int64_t)head * HD;   // + slot * ld
+    const int64_t ld = is_v ? ld_v : ld_k;
+    const size_t block = ((size_t)layer * c.n_pages + page) * c.kv_heads + head;
+    uint8_t *dst = static_cast<uint8_t *>(is_v ? c.v : c.k) + block * (size_t)(pt * HD);
+    float *scale_at = (is_v ? c.v_scale : c.k_scale) + block;
+
+    float val[CHUNKS][16];
+    float amax = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++) {
+        const int slot = (j * 128 + t) / (HD / 16), d = (j * 128 + t) % (HD / 16) * 16;
+        if (slot >= held && slot < fill) {
+            load16(src + (int64_t)slot * ld + d, val[j]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                amax = fmaxf(amax, fabsf(val[j][e]));
+                bad |= !(fabsf(val[j][e]) <= 3.402823466e38f);
+            }
+        }
+    }
+    float old = held > 0 ? __ldcg(scale_at) : 0.0f;
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));       // non-negative floats order like their bits
+    bad = __any_sync(0xffffffffu, bad);
+    if ((threadIdx.x & 31) == 0) {
+        s_max[threadIdx.x >> 5] = amax;
+        s_bad[threadIdx.x >> 5] = bad;
+    }
+    __syncthreads();                                            // also: everybody has the old scale before it is replaced
+    const int w0 = is_v ? 4 : 0;
+    amax = fmaxf(fmaxf(s_max[w0], s_max[w0 + 1]), fmaxf(s_max[w0 + 2], s_max[w0 + 3]));
+    bad = s_bad[w0] | s_bad[w0 + 1] | s_bad[w0 + 2] | s_bad[w0 + 3];
+    bad |= !(old >= 0.0f && old <= 3.402823466e38f);
+    const float scale = bad ? __uint_as_float(0x7fc00000u) : fmaxf(old, pow2_scale<FORMAT>(amax));
+    if (t == 0) *scale_at = scale;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++) {
+        const int slot = (j * 128 + t) / (HD / 16);
+        uint4 *at = reinterpret_cast<uint4 *>(dst) + (j * 128 + t);
+        if (slot < held) {
+            if (scale == old || bad) continue;
+            const float ratio = old / scale;
+            const uint4 w = __ldcg(at);
+            uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float f[4];
+                unpack4<FORMAT>(u[e], f);
+#pragma unroll
+                for (int q = 0; q < 4; q++) f[q] *= ratio;
+                u[e] = pack4<FORMAT>(f);
+            }
+            *at = make_uint4(u[0], u[1], u[2], u[3]);
+        } else if (slot < fill) {
+            uint32_t u[4] = {0u, 0u, 0u, 0u};
+            if (!bad) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) val[j][e] = val[j][e] / scale;
+#pragma unroll
+                for (int e = 0; e < 4; e++) u[e] = pack4<FORMAT>(&val[j][4 * e]);
+            }
+            *at = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+}
+
+// A warp per row: finds its sequence and page, then 16 values a lane and step, keys and values.
+template <typename T, int FORMAT, int HD>
+__global__ void __launch_bounds__(256)
+kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_t ld_v, const int32_t *seqs, const int32_t *start,
+               const int32_t *cu, int n_seqs, int rows, uint32_t *status) {
+    tpb_grid_dep_launch();
+    tpb_grid_dep_wait();
+    const int lane = threadIdx.x & 31;
+    const int r = (int)(blockIdx.x * 8 + (threadIdx.x >> 5));
+    if (r >= rows) return;
+    const int i = find_last(n_seqs, r, [&](int j) { return row_offset(cu, j, rows); });
+    const int r0 = row_offset(cu, i, rows);
+    if (r < r0 || r >= row_offset(cu, i + 1, rows)) return;          // a row of no sequence
+    const int seq = __ldcg(seqs + i);
+    const int from = start ? __ldcg(start + i) : 0;
+    if (seq < 0 || seq >= c.max_seqs) {
+        report(status, kBadSeq);
+        return;
+    }
+    const int len = __ldcg(c.lens + seq);
+    const long long pos = (long long)from + (r - r0);
+    const bool inside = from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens;
+    int page = 0, slot = 0;
+    if (inside) {
+        page = __ldcg(c.table + (size_t)seq * c.max_pages + pos / c.page_tokens);
+        slot = (int)(pos % c.page_tokens);
+        if (page < 0 || page >= c.n_pages) {
+            report(status, kBadPage);
+            return;
+        }
+    }
+    const size_t block0 = ((size_t)layer * c.n_pages + page) * c.kv_heads;
+    const int pieces = c.kv_heads * (HD / 16);
+    for (int p = lane; p < 2 * pieces; p += 32) {
+        const bool is_v = p >= pieces;
+        const int q = is_v ? p - pieces : p;
+        const int head = q / (HD / 16), d = q % (HD / 16) * 16;
+        float f[16] = {};
+        if (inside) {
+            const float scale = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
+            const uint8_t *src = static_cast<const uint8_t *>(is_v ? c.v : c.k) + ((block0 + head) * c.page_tokens + slot) * HD + d;
+            const uint4 w = __ldcg(reinterpret_cast<const uint4 *>(src));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) unpack4<FORMAT>(u[e], &f[4 * e]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) f[e] *= scale;
+        }
+        store16((is_v ? v + (int64_t)r * ld_v : k + (int64_t)r * ld_k) + (int64_t)head * HD + d, f);
+    }
+}
+
+int check_batch(tpb_handle_t h, const char *what, const tpb_kv_cache *c, const void *k, int64_t ld_k, const void *v, int64_t ld_v, int dtype,
+                const int32_t *seqs, const int32_t *cu, int n_seqs, int64_t rows) {
+    TPB_CHECK_ARG(h, dtype == TPB_F32 || dtype == TPB_BF16 || dtype == TPB_F16, "%s: rows must be f32, bf16 or f16", what);
+    TPB_CHECK_ARG(h, n_seqs >= 0 && n_seqs < (1 << 24) && rows >= 0 && rows < (1 << 26), "%s: bad n_seqs / rows", what);
+    if (n_seqs == 0 || rows == 0) return TPB_OK;
+    TPB_CHECK_ARG(h, k && v && seqs && cu, "%s: null pointer", what);
+    const int64_t width = (int64_t)c->kv_heads * c->head_dim, mult = dtype == TPB_F32 ? 4 : 8;
+    TPB_CHECK_ARG(h, ld_k >= width && ld_v >= width && ld_k % mult == 0 && ld_v % mult == 0,
+                  "%s: ld_k and ld_v must be at least kv_heads * head_dim and multiples of %lld", what, (long long)mult);
+    TPB_CHECK_ARG(h, tpb_aligned16(k) && tpb_aligned16(v), "%s: k and v must be 16-byte aligned", what);
+    TPB_CHECK_ARG(h, ((reinterpret_cast<uintptr_t>(seqs) | reinterpret_cast<uintptr_t>(cu)) & 3u) == 0, "%s: seqs and cu must be 4-byte aligned", what);
+    return TPB_OK;
+}
+
+// Calls f with a null T * for the dtype of the rows.
+template <typename F>
+cudaError_t by_dtype(int dtype, F f) {
+    return dtype == TPB_F32 ? f((float *)nullptr) : dtype == TPB_BF16 ? f((__nv_bfloat16 *)nullptr) : f((__half *)nullptr);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, const void *k, int64_t ld_k, const void *v,
+                  int64_t ld_v, int dtype, const int32_t *seqs, const int32_t *cu, int n_seqs, int64_t rows) {
+    if (!h) return TPB_ERR_INVALID_ARG;
+    int rc = check_layer(h, c, layer, "kv_append");
+    if (rc == TPB_OK) rc = check_batch(h, "kv_append", c, k, ld_k, v, ld_v, dtype, seqs, cu, n_seqs, rows);
+    if (rc != TPB_OK || n_seqs == 0 || rows == 0) return rc;
+    tpb_device_guard guard(h->device);
+    TPB_CUDA(h, guard.err);
+    const dim3 grid((unsigned)(rows / c->page_tokens + 2 * (int64_t)n_seqs), (unsigned)c->kv_heads);
+    const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const auto launch = [&](auto kern) {
+            return tpb_launch_pdl(kern, grid, dim3(256), 0, (cudaStream_t)stream, *c, layer, (const T *)k, ld_k, (const T *)v, ld_v, seqs, cu, n_seqs,
+                                  (int)rows, h->d_status);
+        };
+        const int chunks = c->page_tokens * c->head_dim / 2048;             // 0 (half the threads have a piece) .. 4
+        if (c->format == TPB_KV_S8) {
+            if (c->head_dim == 64) return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_S8, 64, 1>) : launch(kv_append_kernel<T, TPB_KV_S8, 64, 2>);
+            return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_S8, 128, 1>)
+                               : chunks <= 2 ? launch(kv_append_kernel<T, TPB_KV_S8, 128, 2>) : launch(kv_append_kernel<T, TPB_KV_S8, 128, 4>);
+        }
+        if (c->head_dim == 64) return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 64, 1>) : launch(kv_append_kernel<T, TPB_KV_E4M3, 64, 2>);
+        return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 1>)
+                           : chunks <= 2 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 2>) : launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 4>);
+    });
+    TPB_CUDA(h, e);
+    return TPB_OK;
+}
+
+int tpb_kv_read(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, void *k, int64_t ld_k, void *v, int64_t ld_v,
+                int dtype, const int32_t *seqs, const int32_t *start, const int32_t *cu, int n_seqs, int64_t rows) {
+    if (!h) return TPB_ERR_INVALID_ARG;
+    int rc = check_layer(h, c, layer, "kv_read");
+    if (rc == TPB_OK) rc = check_batch(h, "kv_read", c, k, ld_k, v, ld_v, dtype, seqs, cu, n_seqs, rows);
+    if (rc != TPB_OK || n_seqs == 0 || rows == 0) return rc;
+    TPB_CHECK_ARG(h, (reinterpret_cast<uintptr_t>(start) & 3u) == 0, "kv_read: start must be 4-byte aligned");
+    tpb_device_guard guard(h->device);
+    TPB_CUDA(h, guard.err);
+    const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const auto launch = [&](auto kern) {
+            return tpb_launch_pdl(kern, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, *c, layer, (T *)k, ld_k, (T *)v, ld_v, seqs,
+                                  start, cu, n_seqs, (int)rows, h->d_status);
+        };
+        if (c->format == TPB_KV_S8) return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_S8, 64>) : launch(kv_read_kernel<T, TPB_KV_S8, 128>);
+        return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_E4M3, 64>) : launch(kv_read_kernel<T, TPB_KV_E4M3, 128>);
+    });
+    TPB_CUDA(h, e);
+    return TPB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,146 @@
+// What the kernels of the 8-bit key / value cache share: the cache as a kernel sees it, its checks, and the batch's lookups.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "tpb_internal.h"
+
+namespace tpb_kv {
+
+constexpr int64_t kMaxPagesInPool = 1 << 24;
+
+// Words of tpb_kv_cache::scratch.
+//   [0] number of page copies that the page operation leaves to its second kernel, [1] pages in use (compact)
+//   marks [max_seqs], offsets [max_seqs], then two page lists of n_pages each: free pages or copy sources, and copy destinations
+struct Scratch {
+    int32_t *head, *marks, *offsets, *list_a, *list_b;
+};
+__host__ __device__ inline Scratch scratch_of(const tpb_kv_cache &c) {
+    Scratch s;
+    s.head = c.scratch;
+    s.marks = c.scratch + 8;
+    s.offsets = s.marks + c.max_seqs;
+    s.list_a = s.offsets + c.max_seqs;
+    s.list_b = s.list_a + c.n_pages;
+    return s;
+}
+
+// codes of the handle's status word (tpb_status_poll): role 32 = a cache that does not fit the call
+constexpr uint32_t kBadSeq = (32u << 24) | 1u, kBadPage = (32u << 24) | 2u, kBadLen = (32u << 24) | 3u, kBadTail = (32u << 24) | 4u;
+
+int check_cache(tpb_handle_t h, const tpb_kv_cache *c, const char *what);   // the struct's own fields
+int check_layer(tpb_handle_t h, const tpb_kv_cache *c, int layer, const char *what);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void report(uint32_t *status, uint32_t code) { atomicCAS(status, 0u, code); }
+
+// An offset of the batch, clamped to the rows there are; data of other kernels of the stream, hence L2 loads.
+__device__ __forceinline__ int row_offset(const int32_t *cu, int i, int rows) {
+    const int v = __ldcg(cu + i);
+    return v < 0 ? 0 : (v > rows ? rows : v);
+}
+
+// The last i in [0, n) with key(i) <= x, key ascending and key(0) <= x; a whole warp calls it, 32 keys a step.  With keys out of order it still
+// ends, at some i in [0, n).
+template <typename Key>
+__device__ __forceinline__ int find_last(int n, int x, Key key) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int i = lo + lane * step;
+        const bool below = i < hi && (lane == 0 || key(i) <= x);
+        const int c = __popc(__ballot_sync(0xffffffffu, below));
+        lo += (c - 1) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
+// Sixteen consecutive values as floats; 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, float (&v)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p) + i);
+            v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (std::is_same<T, __half>::value) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+                    v[8 * i + 2 * e] = f.x; v[8 * i + 2 * e + 1] = f.y;
+                } else {
+                    v[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
+                    v[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store16(T *p, const float (&v)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            reinterpret_cast<float4 *>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&b);
+            } else {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&b);
+            }
+        }
+        reinterpret_cast<uint4 *>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+// One 32-bit word of four cached values.
+template <int FORMAT>
+__device__ __forceinline__ void unpack4(uint32_t w, float *v) {
+    if constexpr (FORMAT == TPB_KV_S8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (float)(int8_t)(w >> (8 * i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+            const float2 f = __half22float2(__half2(h));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+}
+// Four quotients (value / scale) rounded to nearest even, saturated at the format's limit.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t pack4(const float *v) {
+    uint32_t w = 0;
+    if constexpr (FORMAT == TPB_KV_S8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= ((uint32_t)max(-127, min(127, __float2int_rn(v[i]))) & 0xffu) << (8 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            w |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3) << (16 * i);
+    }
+    return w;
+}
+#endif
+
+}  // namespace tpb_kv

@@ -1,0 +1,199 @@
+"""What the calls of packed attention and of the 8-bit key / value cache refuse before anything is launched.  No device: the C entry
+points get a zeroed stand-in for a handle, which they only write their message to, and the Python methods CPU tensors.  Also the index
+arithmetic that the kernels' launches rely on."""
+import ctypes as C
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tensorpencil_b200 import _lib  # noqa: E402
+from tensorpencil_b200.backend import Backend  # noqa: E402
+from tensorpencil_b200.kv_cache import KvCache  # noqa: E402
+
+INVALID = _lib.TPB_ERR_INVALID_ARG
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from tensorpencil_b200 import build
+    build.build()
+    return _lib.load()
+
+
+@pytest.fixture()
+def handle():
+    buf = C.create_string_buffer(1 << 20)
+    at = (C.addressof(buf) + 255) & ~255
+    yield at
+    del buf
+
+
+PACKED = dict(out=4096, ld_out=256, q=4096, ld_q=256, k=4096, ld_k=128, v=4096, ld_v=128, dtype=_lib.TPB_BF16, cu=4096, n_seqs=2, tokens=10,
+              heads=4, kv_heads=2, head_dim=64, scale=0.1)
+
+
+@pytest.mark.parametrize("change", [dict(dtype=_lib.TPB_F32), dict(dtype=_lib.TPB_S32), dict(head_dim=96), dict(head_dim=256, heads=1, kv_heads=1),
+                                    dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(heads=258), dict(n_seqs=-1), dict(tokens=-1),
+                                    dict(tokens=1 << 26), dict(out=0), dict(q=0), dict(k=0), dict(v=0), dict(cu=0), dict(q=4104), dict(out=4098),
+                                    dict(cu=4097), dict(ld_q=248), dict(ld_out=252), dict(ld_k=127), dict(ld_k=64), dict(scale=-1.0),
+                                    dict(scale=float("nan")), dict(scale=float("inf"))])
+def test_attention_packed_refuses(lib, handle, change):
+    a = {**PACKED, **change}
+    assert lib.tpb_attention_packed(handle, None, *a.values()) == INVALID
+    assert lib.tpb_attention_packed(None, None, *PACKED.values()) == INVALID
+
+
+def test_nothing_to_do_is_no_error(lib, handle):
+    for change in (dict(tokens=0), dict(n_seqs=0)):
+        assert lib.tpb_attention_packed(handle, None, *{**PACKED, **change, "q": 0}.values()) == 0
+
+
+def desc(**change):
+    d = dict(k=4096, v=4096, k_scale=4096, v_scale=4096, table=4096, lens=4096, tail=4096, refs=4096, result=4096, scratch=4096, n_pages=100,
+             layers=2, kv_heads=2, page_tokens=16, head_dim=64, max_seqs=4, max_pages=10, format=0)
+    d.update(change)
+    return _lib.KvCacheDesc(**d)
+
+
+def calls_on(lib, h, c):
+    """Every call on a cache, with good arguments otherwise."""
+    return [lib.tpb_kv_extend(h, None, c, 4096, 4096, 1), lib.tpb_kv_truncate(h, None, c, 4096, None, 1), lib.tpb_kv_fork(h, None, c, 4096, 4096, 1, 1),
+            lib.tpb_kv_compact(h, None, c), lib.tpb_kv_append(h, None, c, 0, 4096, 128, 4096, 128, 0, 4096, 4096, 1, 1),
+            lib.tpb_kv_read(h, None, c, 0, 4096, 128, 4096, 128, 0, 4096, None, 4096, 1, 1),
+            lib.tpb_kv_attention(h, None, c, 0, 4096, 256, 4096, 256, 0, 4096, 4096, 1, 1, 4, 0.1, 0, 4096, 1 << 40)]
+
+
+@pytest.mark.parametrize("change", [dict(k=0), dict(v=0), dict(k_scale=0), dict(v_scale=0), dict(table=0), dict(lens=0), dict(tail=0), dict(refs=0),
+                                    dict(result=0), dict(scratch=0), dict(k=4097), dict(v=4104), dict(table=4098), dict(n_pages=0),
+                                    dict(n_pages=(1 << 24) + 1), dict(layers=0), dict(kv_heads=0), dict(kv_heads=65536, n_pages=1, layers=1),
+                                    dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=128), dict(head_dim=32), dict(head_dim=256),
+                                    dict(max_seqs=0), dict(max_pages=0), dict(format=2), dict(n_pages=1 << 24, layers=4),
+                                    dict(max_pages=1 << 27), dict(max_seqs=1 << 20, max_pages=1 << 11)])
+def test_every_call_refuses_a_bad_cache(lib, handle, change):
+    assert calls_on(lib, handle, C.addressof(desc(**change))) == [INVALID] * 7
+    assert calls_on(lib, handle, None) == [INVALID] * 7
+    assert calls_on(lib, None, C.addressof(desc())) == [INVALID] * 7
+
+
+def test_page_operations_refuse_bad_lists(lib, handle):
+    c = C.addressof(desc())
+    assert lib.tpb_kv_extend(handle, None, c, None, 4096, 1) == INVALID
+    assert lib.tpb_kv_extend(handle, None, c, 4096, None, 1) == INVALID
+    assert lib.tpb_kv_extend(handle, None, c, 4097, 4096, 1) == INVALID
+    assert lib.tpb_kv_extend(handle, None, c, 4096, 4096, -1) == INVALID
+    assert lib.tpb_kv_truncate(handle, None, c, None, None, 1) == INVALID
+    assert lib.tpb_kv_fork(handle, None, c, 4096, None, 1, 0) == INVALID
+
+
+ROWS = dict(layer=0, a=4096, ld_a=128, b=4096, ld_b=128, dtype=0, seqs=4096, cu=4096, n_seqs=1, rows=1)
+BAD_ROWS = [dict(layer=2), dict(layer=-1), dict(a=0), dict(b=0), dict(a=4100), dict(ld_a=64), dict(ld_b=130), dict(dtype=3), dict(dtype=9),
+            dict(dtype=1, ld_a=132), dict(seqs=0), dict(cu=0), dict(seqs=4097), dict(n_seqs=-1), dict(rows=-1), dict(rows=1 << 26)]
+
+
+@pytest.mark.parametrize("change", BAD_ROWS)
+def test_append_and_read_refuse(lib, handle, change):
+    c = C.addressof(desc())
+    a = {**ROWS, **change}
+    assert lib.tpb_kv_append(handle, None, c, *a.values()) == INVALID
+    r = list(a.values())
+    assert lib.tpb_kv_read(handle, None, c, *r[:7], None, *r[7:]) == INVALID
+
+
+@pytest.mark.parametrize("change", [dict(layer=2), dict(out=0), dict(q=0), dict(q=4100), dict(ld_out=128), dict(ld_q=250), dict(dtype=3), dict(seqs=0),
+                                    dict(cu=0), dict(cu=4099), dict(n_seqs=-1), dict(rows=-1), dict(heads=3), dict(heads=0), dict(heads=65536),
+                                    dict(scale=-0.5), dict(scale=float("nan")), dict(max_len=-1), dict(work=0), dict(work=4100)])
+def test_attention_refuses(lib, handle, change):
+    a = dict(layer=0, out=4096, ld_out=256, q=4096, ld_q=256, dtype=0, seqs=4096, cu=4096, n_seqs=1, rows=1, heads=4, scale=0.1, max_len=0, work=4096,
+             nbytes=1 << 40)
+    assert lib.tpb_kv_attention(handle, None, C.addressof(desc()), *{**a, **change}.values()) == INVALID
+
+
+def test_a_small_workspace_is_refused(lib, handle):
+    assert lib.tpb_kv_attention_workspace_bytes(None, 64) == 0 and lib.tpb_kv_attention_workspace_bytes(handle, 96) == 0
+    C.c_int.from_address(handle)                           # the stand-in has no SMs: its workspace is empty, so ask the sizes alone
+    assert lib.tpb_kv_scratch_bytes(100, 4) == 4 * (8 + 8 + 200)
+    assert [lib.tpb_kv_scratch_bytes(*a) for a in ((0, 4), (100, 0), ((1 << 24) + 1, 4), (-1, 1))] == [0] * 4
+
+
+def cpu_backend():
+    be = Backend.__new__(Backend)                          # no device, no library behind it: the checks come first
+    be.device = torch.device("cpu")
+    return be
+
+
+def test_attention_packed_refuses_tensors():
+    be = cpu_backend()
+    q, k = torch.zeros(10, 256, dtype=torch.bfloat16), torch.zeros(10, 128, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 10], dtype=torch.int32)
+    call = lambda q=q, k=k, v=k, cu=cu, heads=4, out=None: be.attentionPacked(q, k, v, cu, heads, 2, 64, out=out)      # noqa: E731
+    for bad in (dict(q=q.float(), k=k.float(), v=k.float()), dict(k=k.half()), dict(cu=cu.long()), dict(out=q.float())):
+        with pytest.raises(TypeError):
+            call(**bad)
+    for bad in (dict(q=q[:, :192]), dict(k=k[:9]), dict(v=k.t().contiguous().t()), dict(heads=8), dict(cu=cu.view(1, 2)), dict(out=q[:5]),
+                dict(cu=torch.zeros(4, dtype=torch.int32)[::2]), dict(q=q.view(10, 2, 128)), dict(q=q.to("meta"))):
+        with pytest.raises(ValueError):
+            call(**bad)
+
+
+def test_a_cache_refuses_tensors_that_do_not_fit():
+    be = cpu_backend()
+    shape = (1, 6, 2, 16, 64)
+    good = dict(k=torch.zeros(shape, dtype=torch.int8), v=torch.zeros(shape, dtype=torch.int8), k_scale=torch.zeros(shape[:3]), v_scale=torch.zeros(shape[:3]),
+                table=torch.zeros((3, 4), dtype=torch.int32), lens=torch.zeros(3, dtype=torch.int32), refs=torch.zeros(6, dtype=torch.int32),
+                tail=torch.zeros(3, dtype=torch.int32))
+    for name, t in (("k", good["k"].float()), ("v", good["v"].view(torch.uint8)), ("k_scale", good["k_scale"].half()), ("lens", good["lens"].long()),
+                    ("table", good["table"].float())):
+        with pytest.raises(TypeError):
+            KvCache.wrap(be, **{**good, name: t})
+    for name, t in (("k", good["k"][0]), ("v", good["v"][:, :5]), ("k_scale", good["k_scale"][:, :5]), ("lens", good["lens"][:2]),
+                    ("table", good["table"][0]), ("refs", good["refs"][:3]), ("tail", torch.zeros(6, dtype=torch.int32)[::2]),
+                    ("v_scale", good["v_scale"].to("meta"))):
+        with pytest.raises(ValueError):
+            KvCache.wrap(be, **{**good, name: t})
+    with pytest.raises(TypeError):
+        KvCache(be, 1, 4, 2, 64, 2, 2, dtype="int8")
+    with pytest.raises(ValueError):
+        KvCache(be, 1, 0, 2, 64, 2, 2)
+
+
+def test_cache_methods_refuse_tensors():
+    c = KvCache.__new__(KvCache)
+    c.be, c.kv_heads, c.head_dim = cpu_backend(), 2, 64
+    x, ids, cu = torch.zeros(5, 128), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for bad in (dict(k=x.double(), v=x.double()), dict(v=x.half()), dict(k=x.to(torch.int8))):
+        with pytest.raises(TypeError):
+            c.append(0, **{"k": x, "v": x, "seqs": ids, "cu": cu, **bad})
+    for bad in (dict(k=x[:, :64]), dict(v=x[:4]), dict(v=x.t().contiguous().t()), dict(k=x.to("meta"))):
+        with pytest.raises(ValueError):
+            c.append(0, **{"k": x, "v": x, "seqs": ids, "cu": cu, **bad})
+    with pytest.raises(TypeError):
+        c._ints("seqs", ids.long())
+    with pytest.raises(ValueError):
+        c._ints("cu", cu, 3)
+    with pytest.raises(ValueError):
+        c._rows("q", torch.zeros(5, 256), 5, 8, torch.float32)
+
+
+def test_places_of_the_append_launch():
+    """Sequence i's places cu[i] / page + 2 i .. cu[i + 1] / page + 2 (i + 1) - 1 are as many as the pages that its new tokens can touch,
+    wherever they begin, and the launch has them all."""
+    rnd = random.Random(3)
+    for _ in range(400):
+        page, n = rnd.choice([16, 32, 64]), rnd.randint(1, 9)
+        new = [rnd.choice([0, 1, rnd.randint(0, 5 * page)]) for _ in range(n)]
+        cu = [sum(new[:i]) for i in range(n + 1)]
+        place = [cu[i] // page + 2 * i for i in range(n + 1)]
+        assert place[n] <= cu[n] // page + 2 * n               # the launch's grid
+        for i in range(n):
+            first = rnd.randint(0, 10 * page)
+            touched = (first + new[i] - 1) // page - first // page + 1 if new[i] else 0
+            assert touched <= place[i + 1] - place[i]
+
+
+def test_tables_of_a_scratch_hold_every_list():
+    """marks and offsets a sequence, two lists a page, eight words in front: the order that the kernels cut the scratch in."""
+    lib = _lib.load()
+    for pages, seqs in ((1, 1), (17, 3), (70001, 1300)):
+        assert lib.tpb_kv_scratch_bytes(pages, seqs) // 4 == 8 + seqs + seqs + pages + pages

@@ -1,0 +1,535 @@
+"""The 8-bit key / value cache on the GPU: page operations and quantising against a model in Python, bit for bit; attention against the
+formula in 64 bits (bounds: attn_reference.py)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from attn_reference import HALF_STEP, Model, attend, tolerance  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def be():
+    from tensorpencil_b200.backend import Backend
+    b = Backend(0)
+    yield b
+    b.close()
+
+
+def i32(values):
+    return torch.tensor(list(values), dtype=torch.int32).cuda()
+
+
+def offsets(lens):
+    return i32(np.cumsum([0] + list(lens)))
+
+
+def both(be, n_pages=40, max_seqs=8, max_pages=12, page=16, kv=2, hd=64, fmt="s8", layers=1):
+    from tensorpencil_b200.kv_cache import KvCache
+    return (KvCache(be, layers, n_pages, kv, hd, max_seqs, max_pages, page, fmt), Model(n_pages, max_seqs, max_pages, page, kv, hd, fmt, layers))
+
+
+def same_tables(c, m):
+    assert c.table.tolist() == m.table
+    assert c.lens.tolist() == m.lens and c.tail.tolist() == m.tail and c.refs.tolist() == m.refs
+    r = c.result.tolist()
+    assert r == m.result, (r, m.result)
+
+
+def same_values(c, m, layer=0, dtype=torch.float32):
+    seqs = [s for s in range(m.max_seqs) if m.lens[s]]
+    if not seqs:
+        return
+    lens = [m.lens[s] for s in seqs]
+    got = c.read(layer, i32(seqs), offsets(lens), sum(lens), dtype=dtype)
+    for name, g in zip("kv", got):
+        want = np.concatenate([m.read(layer, name, s) for s in seqs]).reshape(sum(lens), -1)
+        g = g.double().cpu().numpy()
+        if dtype != torch.float32:
+            want = torch.from_numpy(want).to(dtype).double().numpy()
+        assert np.array_equal(g, want, equal_nan=True), name
+
+
+def values(rng, n, kv, hd, dt, big=1.0):
+    x = rng.standard_normal((n, kv, hd)) * big * np.exp2(rng.integers(-3, 4, (n, kv, 1)))
+    return torch.from_numpy(x).to(DT[dt]).cuda()
+
+
+def append(c, m, seqs, xs, layer=0):
+    """xs: one (k, v) a sequence, [n][kv][hd]."""
+    k, v = (torch.cat([x[i] for x in xs]) for i in (0, 1))
+    c.append(layer, k, v, i32(seqs), offsets([x[0].shape[0] for x in xs]))
+    for s, x in zip(seqs, xs):
+        for name, t in zip("kv", x):
+            if t.shape[0]:
+                m.append(layer, name, s, t.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("page,hd,kv", [(16, 64, 2), (16, 128, 3), (32, 128, 1), (64, 64, 5), (64, 128, 2), (32, 64, 1)])
+def test_append_and_read_bit_for_bit(be, page, hd, kv, dt, fmt):
+    c, m = both(be, n_pages=60, page=page, hd=hd, kv=kv, fmt=fmt)
+    rng = np.random.default_rng(page + hd + kv)
+    for step, lens in enumerate([{0: 1, 3: 40, 5: 2 * page}, {0: 5, 3: 1, 5: 1}, {3: 1}, {0: page - 6, 1: 3, 3: page + 1, 5: 1}, {0: 1, 1: 1, 3: 1, 5: 1}]):
+        seqs = list(lens)[::-1]
+        n = [lens[s] for s in seqs]
+        c.extend(i32(seqs), i32(n))
+        m.extend(seqs, n)
+        same_tables(c, m)
+        append(c, m, seqs, [tuple(values(rng, k, kv, hd, dt, 2.0 ** step) for _ in range(2)) for k in n])     # scales grow with the steps
+        same_values(c, m)
+    assert c.check() == c.result.tolist()[1]
+    assert np.array_equal(c.k_scale[0].cpu().numpy()[np.array(m.refs) > 0], m.scale["k"][0][np.array(m.refs) > 0].astype(np.float32))
+    same_values(c, m, dtype=torch.bfloat16)
+    same_values(c, m, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+def test_blocks_at_the_edges_of_the_quantiser(be, fmt):
+    """Zeros, the smallest and largest values, an amax at the limit times a power of two and next to it, ties, NaN and infinities."""
+    c, m = both(be, fmt=fmt, kv=1, hd=64, n_pages=80)
+    limit = {"s8": 127.0, "e4m3": 448.0}[fmt]
+    near = lambda f, d: float(np.nextafter(np.float32(f), np.float32(d)))      # noqa: E731
+    tops = [0.0, 1e-45, 1e-38, 1e-30, 3.0e38, 3.4028234e38, limit, near(limit, 0), near(limit, 1e9), limit * 2.0 ** -9, near(limit * 2.0 ** -9, 1e9),
+            limit * 2.0 ** 40, 1.0, 2.0, near(1.0, 0)]
+    seqs = [0, 1]
+    per = [16 * 8, 16 * (len(tops) - 8)]
+    c.extend(i32(seqs), i32(per))
+    m.extend(seqs, per)
+    rng = np.random.default_rng(0)
+    xs = []
+    for part in (tops[:8], tops[8:]):
+        x = np.concatenate([np.clip(rng.integers(-255, 256, (16, 1, 64)) / 254.0, -1, 1) * t for t in part]).astype(np.float32)
+        for i, t in enumerate(part):
+            x[16 * i, 0, 0] = t
+        xs.append((torch.from_numpy(x).cuda(), torch.from_numpy(-x[::-1].copy()).cuda()))
+    append(c, m, seqs, xs)
+    same_values(c, m)
+    for s, bad in ((2, float("nan")), (3, float("inf")), (4, -float("inf"))):
+        c.extend(i32([s]), i32([20]))
+        m.extend([s], [20])
+        k, v = values(rng, 20, 1, 64, "f32"), values(rng, 20, 1, 64, "f32")
+        k[3, 0, 5] = bad
+        append(c, m, [s], [(k, v)])
+        c.extend(i32([s]), i32([1]))
+        m.extend([s], [1])
+        append(c, m, [s], [(values(rng, 1, 1, 64, "f32"), values(rng, 1, 1, 64, "f32"))])
+    same_values(c, m)
+    c.check()
+
+
+def test_read_of_parts_and_behind_the_end(be):
+    c, m = both(be, kv=2, hd=64)
+    rng = np.random.default_rng(3)
+    c.extend(i32([0, 1]), i32([37, 5]))
+    m.extend([0, 1], [37, 5])
+    append(c, m, [0, 1], [tuple(values(rng, n, 2, 64, "f32") for _ in range(2)) for n in (37, 5)])
+    out = tuple(torch.full((30, 2 * 64 + 4), 9.0).cuda() for _ in range(2))
+    c.read(0, i32([1, 0]), i32([2, 12, 25]), 30, start=i32([3, 30]), out=tuple(t[:, :128] for t in out))
+    for name, t in zip("kv", out):
+        t = t.cpu().numpy()
+        want = np.full((30, 128), 9.0)
+        want[2:12], want[12:25] = 0.0, 0.0
+        want[2:4], want[12:19] = m.read(0, name, 1)[3:5].reshape(2, -1), m.read(0, name, 0)[30:].reshape(7, -1)
+        assert np.array_equal(t[:, :128], want) and (t[:, 128:] == 9.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+@pytest.mark.parametrize("seed", range(6))
+def test_random_page_operations_follow_the_model(be, seed, fmt):
+    """Extensions, appends, forks of both kinds, cuts, frees and compactions in any order, refused ones among them."""
+    rng = np.random.default_rng(seed)
+    page, kv, hd, layers = [16, 32, 64][seed % 3], 2, [64, 128][seed % 2], 2
+    c, m = both(be, n_pages=26 if seed % 2 else 300, max_seqs=10, max_pages=9, page=page, kv=kv, hd=hd, fmt=fmt, layers=layers)
+    for _ in range(60):
+        op = rng.choice(["extend", "extend", "extend", "truncate", "free", "fork", "copy", "compact"])
+        ids = [int(i) for i in rng.permutation(10)[:rng.integers(1, 5)]]
+        if rng.random() < 0.05:
+            ids.append(ids[0] if rng.random() < 0.5 else 10)
+        if op == "extend":
+            n = [int(rng.choice([0, 1, 3, page, 2 * page + 1])) for _ in ids]
+            c.extend(i32(ids), i32(n))
+            m.extend(ids, n)
+            same_tables(c, m)
+            if m.result[0] == 0:
+                xs = [[tuple(values(rng, k, kv, hd, "f32") for _ in range(2)) for k in n] for _ in range(layers)]
+                for layer in range(layers):
+                    append(c, m, ids, xs[layer], layer)
+        elif op == "truncate":
+            n = [int(rng.integers(0, m.lens[i] + 1)) if 0 <= i < 10 else 0 for i in ids]
+            if rng.random() < 0.05:
+                n[0] += 1000
+            c.truncate(i32(ids), i32(n))
+            m.truncate(ids, n)
+        elif op == "free":
+            c.truncate(i32(ids))
+            m.truncate(ids)
+        elif op in ("fork", "copy"):
+            free = [i for i in range(10) if m.lens[i] == 0]
+            used = [i for i in range(10) if m.lens[i]]
+            if not free or not used:
+                continue
+            dst = [int(d) for d in rng.permutation(free)[:rng.integers(1, 4)]]
+            src = [int(rng.choice(used)) for _ in dst]
+            if rng.random() < 0.1:
+                dst[-1] = int(rng.choice(used))
+            c.fork(i32(src), i32(dst), share=op == "fork")
+            m.fork(src, dst, op == "fork")
+        else:
+            c.compact()
+            m.compact()
+        same_tables(c, m)
+        for layer in range(layers):
+            same_values(c, m, layer)
+        assert all(0 <= p < m.n_pages for s in range(10) for p in m.table[s][:m.pages(m.lens[s])])
+    be.status_poll()
+
+
+def test_a_large_pool(be):
+    """More pages than one step of the scans covers, a number that no vector load divides, and long lists."""
+    n_pages, n = 70001, 600
+    c, m = both(be, n_pages=n_pages, max_seqs=1300, max_pages=140, page=16, kv=1, hd=64)
+    rng = np.random.default_rng(1)
+    ids, lens = [int(i) for i in rng.permutation(600)], [int(x) for x in rng.integers(0, 2000, n)]
+    for call in ("extend", "free", "fork", "compact", "cut"):
+        if call == "extend":
+            c.extend(i32(ids), i32(lens)), m.extend(ids, lens)
+        elif call == "free":
+            c.truncate(i32(ids[::3])), m.truncate(ids[::3])
+        elif call == "fork":
+            src, dst = ids[1::3], [600 + i for i in range(len(ids[1::3]))]
+            c.fork(i32(src), i32(dst)), m.fork(src, dst, True)
+        elif call == "compact":
+            c.compact(), m.compact()
+        else:
+            live = [s for s in range(1300) if m.lens[s] > 50]
+            to = [m.lens[s] - 33 for s in live]
+            c.truncate(i32(live), i32(to)), m.truncate(live, to)
+        same_tables(c, m)
+    be.status_poll()
+
+
+def test_refused_operations_change_nothing_and_say_why(be):
+    from tensorpencil_b200 import _lib
+    c, m = both(be, n_pages=5, max_seqs=4, max_pages=4, kv=1)
+    for op, arg, status in ((c.extend, (i32([0]), i32([70])), _lib.TPB_ERR_INVALID_ARG),           # longer than a table row
+                            (c.extend, (i32([0, 1]), i32([50, 40])), _lib.TPB_ERR_OOM),
+                            (c.extend, (i32([0, 0]), i32([1, 1])), _lib.TPB_ERR_INVALID_ARG),
+                            (c.extend, (i32([-1]), i32([1])), _lib.TPB_ERR_INVALID_ARG),
+                            (c.extend, (i32([1]), i32([-1])), _lib.TPB_ERR_INVALID_ARG),
+                            (c.truncate, (i32([0]), i32([1])), _lib.TPB_ERR_INVALID_ARG),
+                            (c.truncate, (i32([4]),), _lib.TPB_ERR_INVALID_ARG),
+                            (c.fork, (i32([0]), i32([0])), _lib.TPB_ERR_INVALID_ARG)):
+        op(*arg)
+        with pytest.raises(_lib.TpbError) as e:
+            c.check()
+        assert e.value.status == status
+        m.result = c.result.tolist()
+        same_tables(c, m)
+
+
+def test_tokens_that_no_extension_made_room_for_are_not_written(be):
+    from tensorpencil_b200 import _lib
+    c, m = both(be, n_pages=2, kv=1)
+    rng = np.random.default_rng(0)
+    c.extend(i32([0]), i32([20]))
+    m.extend([0], [20])
+    append(c, m, [0], [tuple(values(rng, 20, 1, 64, "f32") for _ in range(2))])
+    c.extend(i32([0]), i32([20]))                          # not enough pages: refused, and so is what follows
+    x = values(rng, 20, 1, 64, "f32")
+    c.append(0, x, x, i32([0]), i32([0, 20]))
+    with pytest.raises(_lib.TpbError) as e:
+        be.status_poll()
+    assert e.value.status == _lib.TPB_ERR_STATE
+    same_values(c, m)
+    for seqs in ([7], [8], [-1]):                          # an empty sequence, and ids out of range
+        c.append(0, x, x, i32(seqs), i32([0, 20]))
+        with pytest.raises(_lib.TpbError) as e:
+            be.status_poll()
+        assert e.value.status == _lib.TPB_ERR_STATE
+    same_values(c, m)
+
+
+# -- attention -----------------------------------------------------------------------------
+
+
+def filled(be, lens, fmt, page, kv, hd, seed, spare=6):
+    """A cache whose sequences' pages lie out of order, with random contents."""
+    n_pages = sum(-(-n // page) for n in lens) + spare
+    c, m = both(be, n_pages=n_pages, max_seqs=len(lens) + 1, max_pages=max(1, max(-(-n // page) for n in lens)) + 1, page=page, kv=kv, hd=hd, fmt=fmt)
+    rng = np.random.default_rng(seed)
+    order = [int(p) for p in rng.permutation(n_pages)]
+    lim = 127 if fmt == "s8" else 448
+    for s, n in enumerate(lens):
+        m.lens[s] = n
+        for p in range(-(-n // page)):
+            m.table[s][p] = order.pop()
+            m.refs[m.table[s][p]] = 1
+    for name, t, sc in (("k", c.k, c.k_scale), ("v", c.v, c.v_scale)):
+        x = np.clip(rng.standard_normal(m.q[name].shape) * lim / 4, -lim, lim)
+        q = torch.from_numpy(x)
+        q = torch.round(q).to(torch.int8) if fmt == "s8" else q.to(torch.float8_e4m3fn)
+        m.q[name] = q.double().numpy()
+        m.scale[name] = np.exp2(rng.integers(-1, 2, m.scale[name].shape)) * 4.0 / lim * (1.0 + 0.25 * rng.random(m.scale[name].shape))
+        m.scale[name] = m.scale[name].astype(np.float32).astype(np.float64)
+        t.copy_(q.cuda())
+        sc.copy_(torch.from_numpy(m.scale[name]).float())
+    c.table.copy_(torch.tensor(m.table, dtype=torch.int32))
+    c.lens.copy_(i32(m.lens))
+    c.refs.copy_(i32(m.refs))
+    return c, m
+
+
+def check_attention(c, m, out, q, seqs, n_new, heads, dt, scale=None):
+    kv, hd = c.kv_heads, c.head_dim
+    scale = hd ** -0.5 if scale is None else scale
+    got, q = out.double().cpu().numpy(), q.double().cpu().numpy()
+    at = 0
+    for s, n in zip(seqs, n_new):
+        k, v = m.read(0, "k", s), m.read(0, "v", s)
+        last = m.lens[s] - n + np.arange(n)
+        for h in range(heads):
+            mine, hk = slice(h * hd, (h + 1) * hd), h // (heads // kv)
+            o, a, e = attend(q[at:at + n, mine], k[:, hk], v[:, hk], last, scale)
+            # q and the weights in two f16 terms each: what is left of them is below 2^-21 of a row's largest
+            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], 2.0 ** -21) + len(k) * 2.0 ** -33 * (np.abs(v).max() if len(k) else 0)
+            err = np.abs(got[at:at + n, mine] - o)
+            assert (err <= tol).all(), (s, n, h, float((err / tol).max()), float(err.max()))
+        at += n
+
+
+ATT = [([1], 1, 2, 1, 64, 16), ([16, 17, 15], 1, 4, 4, 128, 16), ([200, 1, 64, 63, 65], 1, 8, 2, 128, 32), ([777], 1, 7, 1, 64, 64),
+       ([300, 5, 90], 4, 6, 2, 128, 16), ([130, 40], 5, 16, 1, 64, 32), ([2500], 2, 12, 4, 128, 16), ([3000, 2], 8, 8, 8, 64, 64),
+       ([40, 500], 9, 5, 1, 128, 64), ([1000], 33, 4, 2, 64, 16), ([260], 1, 40, 1, 128, 32), ([9000], 1, 3, 1, 128, 32)]
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,new,heads,kv,hd,page", ATT)
+def test_attention_matches_the_formula(be, lens, new, heads, kv, hd, page, dt, fmt):
+    c, m = filled(be, lens, fmt, page, kv, hd, sum(lens) + heads)
+    seqs = list(range(len(lens)))[::-1]
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn((new * len(seqs), heads * hd), generator=g).to(DT[dt]).cuda()
+    out = c.attention(0, q, i32(seqs), offsets([new] * len(seqs)), heads)
+    be.status_poll()
+    check_attention(c, m, out, q, seqs, [new] * len(seqs), heads, dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_different_numbers_of_queries_and_rows_that_see_nothing(be, dt):
+    """0 to 20 queries a sequence, some of sequences that are shorter than that (their first rows see nothing: zeros), an empty one."""
+    lens, new, heads, kv, hd = [90, 3, 0, 400, 18], [7, 5, 2, 0, 20], 6, 2, 64
+    c, m = filled(be, lens, "s8", 16, kv, hd, 5)
+    rows = sum(new)
+    g = torch.Generator().manual_seed(2)
+    wide_q = torch.randn((rows + 3, heads * hd + 8), generator=g).to(DT[dt]).cuda()
+    wide = torch.full((rows + 3, heads * hd + 8), 5.0, dtype=DT[dt]).cuda()
+    q, out = wide_q[:, :heads * hd], wide[:, :heads * hd]
+    c.attention(0, q, i32(range(5)), offsets(new), heads, out=out)
+    be.status_poll()
+    check_attention(c, m, out[:rows], q[:rows], range(5), new, heads, dt)
+    assert (out[7:9] == 0).all() and (out[12:14] == 0).all() and (out[14:16] == 0).all()
+    assert (wide[rows:] == 5.0).all() and (wide[:, heads * hd:] == 5.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+def test_stale_bytes_scales_and_tables_behind_the_end_are_not_part_of_it(be, fmt):
+    """Whatever lies behind a sequence's last token -- NaN among it -- in its last page, in free pages and in the table."""
+    lens, heads, kv, hd, page = [50, 129, 33], 4, 2, 64, 32
+    c, m = filled(be, lens, fmt, page, kv, hd, 8)
+    q = torch.randn((3, heads * hd), generator=torch.Generator().manual_seed(0)).cuda()
+    clean = c.attention(0, q, i32([0, 1, 2]), offsets([1] * 3), heads)
+    free = [p for p in range(m.n_pages) if m.refs[p] == 0]
+    for t, sc in ((c.k, c.k_scale), (c.v, c.v_scale)):
+        raw = t.view(torch.uint8)
+        raw[:, free] = 0x7f                                # NaN in e4m3
+        sc[:, free] = float("nan")
+        for s, n in enumerate(lens):
+            raw[0, m.table[s][n // page], :, n % page:] = 0x7f
+    c.table[0, 2:] = 10 ** 9
+    c.table[1, 5:] = -7
+    out = c.attention(0, q, i32([0, 1, 2]), offsets([1] * 3), heads)
+    be.status_poll()
+    assert torch.equal(out, clean)
+
+
+def test_a_block_with_a_nan_reaches_the_heads_that_see_it(be):
+    lens, heads, kv, hd = [100, 40], 4, 2, 64
+    c, m = filled(be, lens, "s8", 16, kv, hd, 8)
+    q = torch.randn((2, heads * hd), generator=torch.Generator().manual_seed(0)).cuda()
+    clean = c.attention(0, q, i32([0, 1]), offsets([1, 1]), heads)
+    c.k_scale[0, m.table[0][3], 0] = float("nan")
+    c.v_scale[0, m.table[0][1], 1] = float("nan")
+    out = c.attention(0, q, i32([0, 1]), offsets([1, 1]), heads)
+    assert torch.isnan(out[0]).all() and torch.equal(out[1], clean[1])
+
+
+@pytest.mark.parametrize("fmt,dt", [("s8", "f32"), ("e4m3", "bf16"), ("s8", "f16")])
+def test_scores_and_values_of_a_wide_range(be, fmt, dt):
+    """Queries from tiny to large, maxima that come late, value scales that differ by 2^40 from page to page."""
+    lens, heads, kv, hd, page = [700, 90], 8, 2, 128, 16
+    c, m = filled(be, lens, fmt, page, kv, hd, 4)
+    if dt != "f16":
+        rng = np.random.default_rng(0)
+        f = np.exp2(rng.integers(-20, 21, m.scale["v"].shape))
+        m.scale["v"] = (m.scale["v"] * f).astype(np.float32).astype(np.float64)
+        c.v_scale.copy_(torch.from_numpy(m.scale["v"]).float())
+    q = torch.randn((2, heads * hd), generator=torch.Generator().manual_seed(3)) * torch.exp2(torch.arange(heads * hd) // hd * 1.0 - 4)
+    q = q.to(DT[dt]).cuda()
+    out = c.attention(0, q, i32([0, 1]), offsets([1, 1]), heads)
+    # with values of very different sizes a weight's share of the largest product counts: all terms are below max |v| p
+    kvs = c.kv_heads
+    got = out.double().cpu().numpy()
+    for r, s in enumerate([0, 1]):
+        k, v = m.read(0, "k", s), m.read(0, "v", s)
+        for h in range(heads):
+            hk = h // (heads // kvs)
+            qq = q[r:r + 1, h * hd:(h + 1) * hd].double().cpu().numpy()
+            o, a, e = attend(qq, k[:, hk], v[:, hk], [lens[s] - 1], hd ** -0.5)
+            p = np.exp((k[:, hk] @ qq[0]) * hd ** -0.5 - ((k[:, hk] @ qq[0]) * hd ** -0.5).max())
+            biggest = (p / p.sum() * np.abs(v[:, hk]).max(1)).max()
+            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], 2.0 ** -21) + len(k) * 2.0 ** -30 * biggest
+            err = np.abs(got[r, h * hd:(h + 1) * hd] - o[0])
+            assert (err <= tol).all(), (s, h, float((err / tol).max()))
+
+
+def test_bad_entries_are_reported_and_skipped(be):
+    from tensorpencil_b200 import _lib
+    c, m = filled(be, [100, 40], "s8", 16, 1, 64, 3)
+    q = torch.randn((2, 2 * 64)).cuda()
+    c.attention(0, q, i32([0, 1]), offsets([1, 1]), 2)
+    be.status_poll()
+    for what, to in (("table", 10 ** 6), ("table", -1), ("lens", 10 ** 6), ("lens", -3), ("id", 3), ("id", -1)):
+        seqs = i32([0, to if what == "id" else 1])
+        old = (c.table.clone(), c.lens.clone())
+        if what == "table":
+            c.table[1, 1] = to
+        if what == "lens":
+            c.lens[1] = to
+        out = c.attention(0, q, seqs, offsets([1, 1]), 2)
+        with pytest.raises(_lib.TpbError) as e:
+            be.status_poll()
+        assert e.value.status == _lib.TPB_ERR_STATE
+        check_attention(c, m, out[:1], q[:1], [0], [1], 2, "f32")
+        c.table.copy_(old[0]), c.lens.copy_(old[1])
+
+
+def test_max_len_is_a_hint(be):
+    c, m = filled(be, [5000, 40, 1200], "e4m3", 16, 2, 128, 3)
+    q = torch.randn((3, 8 * 128)).cuda()
+    for hint in (0, 40, 200, 5000, 10 ** 9):
+        check_attention(c, m, c.attention(0, q, i32([0, 1, 2]), offsets([1, 1, 1]), 8, max_len=hint), q, [0, 1, 2], [1] * 3, 8, "f32")
+
+
+def test_many_sequences(be):
+    rng = np.random.default_rng(2)
+    lens = [int(n) for n in rng.integers(0, 60, 700)]
+    lens[100], lens[650] = 900, 2000
+    c, m = filled(be, lens, "s8", 16, 1, 64, 3)
+    seqs = [int(s) for s in rng.permutation(700)]
+    q = torch.randn((700, 2 * 64)).cuda()
+    out = c.attention(0, q, i32(seqs), offsets([1] * 700), 2)
+    be.status_poll()
+    some = [i for i in range(700) if i % 13 == 0 or seqs[i] in (100, 650)]
+    check_attention(c, m, out[some], q[some], [seqs[i] for i in some], [1] * len(some), 2, "f32")
+
+
+def test_two_streams_and_the_same_bits_again(be):
+    c, m = filled(be, [3000, 170, 1000], "s8", 32, 2, 128, 3)
+    q = torch.randn((2, 3, 8 * 128)).cuda()
+    want = [c.attention(0, q[i], i32([0, 1, 2]), offsets([1] * 3), 8) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ids, cu = i32([0, 1, 2]), offsets([1] * 3)
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(c.attention(0, q[i], ids, cu, 8))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_a_decode_loop_prompt_to_compaction(be):
+    """Prompts through packed attention and into the cache, decoding with drafts that are cut back, beams, a freed sequence and a compaction, two
+    layers: every step's attention against the formula on the cache's values."""
+    kv, heads, hd, page, layers = 2, 6, 64, 16, 2
+    c, m = both(be, n_pages=60, max_seqs=6, max_pages=20, page=page, kv=kv, hd=hd, fmt="e4m3", layers=layers)
+    rng = np.random.default_rng(9)
+
+    def step(seqs, n, dt="bf16"):
+        c.extend(i32(seqs), i32(n))
+        m.extend(seqs, n)
+        same_tables(c, m)
+        cu = offsets(n)
+        for layer in range(layers):
+            xs = [tuple(values(rng, k, kv, hd, dt) for _ in range(2)) for k in n]
+            append(c, m, seqs, xs, layer)
+            q = values(rng, sum(n), heads, hd, dt).reshape(sum(n), -1)
+            out = c.attention(layer, q, i32(seqs), cu, heads)
+            if layer == 0:
+                check_attention(c, m, out, q, seqs, n, heads, dt)
+        return xs
+
+    prompts = [70, 33]
+    step([0, 1], prompts)
+    k, v = (torch.cat([values(rng, n, kv, hd, "bf16").reshape(n, -1) for n in prompts]) for _ in range(2))
+    be.attentionPacked(values(rng, 103, heads, hd, "bf16").reshape(103, -1), k, v, offsets(prompts), heads, kv, hd)
+    for _ in range(3):
+        step([1, 0], [1, 1])
+    step([0, 1], [5, 5], "f32")                             # five drafts each, some rejected
+    to = [m.lens[0] - 3, m.lens[1] - 4]
+    c.truncate(i32([0, 1]), i32(to)), m.truncate([0, 1], to)
+    c.fork(i32([0, 0, 1]), i32([2, 3, 4])), m.fork([0, 0, 1], [2, 3, 4], True)
+    same_tables(c, m)
+    step([4, 2, 0, 3, 1], [1] * 5)
+    c.truncate(i32([0, 1])), m.truncate([0, 1])
+    c.compact(), m.compact()
+    same_tables(c, m)
+    step([2, 3, 4], [1, 2, 1], "f16")
+    for layer in range(layers):
+        same_values(c, m, layer)
+    assert c.check() == m.result[1]
+
+
+def test_a_captured_step_replays_while_the_lengths_grow(be):
+    kv, heads, hd = 2, 8, 128
+    c, m = both(be, n_pages=40, max_seqs=3, max_pages=12, page=16, kv=kv, hd=hd)
+    rng = np.random.default_rng(4)
+    seqs, one, cu = i32([2, 0]), i32([1, 1]), i32([0, 1, 2])
+    c.extend(seqs, i32([30, 15]))
+    m.extend([2, 0], [30, 15])
+    append(c, m, [2, 0], [tuple(values(rng, n, kv, hd, "f32") for _ in range(2)) for n in (30, 15)])
+    k, v, q = (torch.zeros((2, h * hd)).cuda() for h in (kv, kv, heads))
+    out = torch.zeros((2, heads * hd)).cuda()
+
+    def step():
+        c.extend(seqs, one)
+        c.append(0, k, v, seqs, cu)
+        c.attention(0, q, seqs, cu, heads, out=out)
+
+    graphs = []
+    for _ in range(2):                                      # two graphs of the same step, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        graphs.append(g)
+    for i in range(8):
+        for t, h in ((k, kv), (v, kv), (q, heads)):
+            t.copy_(values(rng, 2, h, hd, "f32").reshape(2, -1))
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        m.extend([2, 0], [1, 1])
+        for j, s in enumerate([2, 0]):
+            m.append(0, "k", s, k[j:j + 1].view(1, kv, hd).double().cpu().numpy())
+            m.append(0, "v", s, v[j:j + 1].view(1, kv, hd).double().cpu().numpy())
+        same_tables(c, m)
+        same_values(c, m)
+        check_attention(c, m, out, q, [2, 0], [1, 1], heads, "f32")
