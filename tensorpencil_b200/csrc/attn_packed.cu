@@ -1,44 +1,532 @@
-// Causal attention over packed prompts.
+// Causal attention over packed prompts for sm_100a: softmax(q k^T * scale) v per head on tcgen05 (kind::f16), grouped-query heads,
+// head_dim 64 or 128, any number of sequences of any lengths.
+//
+// One pass over the keys with the running maximum and sum of the softmax: per tile of 128 keys
+//   S = Q K^T          M 128 rows x N 128 keys x K head_dim, both operands from shared memory, f32 in tensor memory
+//   P = exp2(S c - m)  one thread a row: its 128 scores in registers, reference point m and sum l per row
+//   O += P V           M 128 x N head_dim x K 128; P (16 bits, two a column) lies over the first half of S and is read from tensor
+//                      memory; V is the B operand as it lies in memory, head_dim contiguous ("MN-major"): no transpose pass
+//
+// Rows.  A tile's 128 rows are (token, query head of the group) pairs of one kv head: 128 / g tokens x g heads.  All of a group's heads
+// share the K and V tiles, and short prompts fill a tile g times sooner than with one head a tile.  A CTA has two such tiles, A
+// and B, of consecutive tokens: while the tensor pipe works for one, the other's softmax runs.
+//
+// Roles: warps 0-3 / 4-7 softmax and output of tile A / B, warp 8 TMA, warp 9 MMA, warps 10 and 11 look V over.  MMAs of one thread execute in
+// issue order, which is what frees the buffers: S_x(j+1) is issued after P_x(j) V(j).  Every wait is bounded.
+//
+// What a row must not see.  Scores of later tokens, other sequences and rows past the end are replaced before the maximum and
+// their weights set to zero, so K's values there do not matter.  V's do, 0 * NaN being NaN: in the tiles that some row sees only a part of,
+// warps 10 and 11 replace every NaN and infinity in shared memory by zero before the product and write down, per column,
+// the first key of each kind that belongs to the sequence; the epilogue adds it to the rows that see that key.
+#include <climits>
+#include <type_traits>
+
+#include "gemm_common.cuh"
 #include "kv_common.cuh"
 
-namespace {
-
+using namespace tpb_gemm;
 using tpb_kv::find_last;
 using tpb_kv::row_offset;
 
-// A warp per (token, head): one pass over the visible tokens with the running maximum and sum, each lane HD / 32 dimensions.
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kAtomBytes = 16384;     // [128 rows][64 values of 16 bits] in the 128-byte swizzle layout
+constexpr int kThreads = 384;
+constexpr int kStages = 2;
+constexpr float kLazy = 8.0f;         // the reference point moves when the maximum has grown by more than 2^8
+
+template <int HD>
+struct Layout {
+    static constexpr int kAtoms = HD / 64;
+    static constexpr int kQ = 0;                                          // tiles A, B
+    static constexpr int kK = kQ + 2 * kAtoms * kAtomBytes;
+    static constexpr int kV = kK + kStages * kAtoms * kAtomBytes;
+    static constexpr int kBar = kV + kStages * kAtoms * kAtomBytes;
+    static constexpr int kBad = kBar + 256;                               // [3][HD] first NaN, +inf, -inf of a column
+    static constexpr int kBytes = kBad + 3 * HD * 4 + 1024;
+};
+
+struct PackedParams {
+    void *out;
+    long long ld_out;             // elements
+    const int32_t *cu;
+    int n_seqs, tokens;
+    int group, kv_heads, tile_tokens;      // query heads a kv head, 128 / group
+    unsigned slots;
+    float scale_log2;
+    uint32_t *status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld_16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+// V as B operand, head_dim contiguous: 8-key groups 1024 bytes apart (stride offset), the two halves of a 128-wide head an
+// atom apart (leading offset).
+__device__ __forceinline__ uint64_t make_mn_major_desc(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(kAtomBytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// kind::f16, f32 accumulation, both operands of type T; N columns; B MN-major or K-major
+template <typename T>
+__device__ __forceinline__ uint32_t make_idesc(int n, bool b_mn) {
+    const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(256)
-attn_packed_kernel(T *out, int64_t ld_out, const T *q, int64_t ld_q, const T *k, int64_t ld_k, const T *v, int64_t ld_v, const int32_t *cu,
-                   int n_seqs, int tokens, int heads, int kv_heads, float scale) {
+__global__ void __launch_bounds__(kThreads, 1)
+attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                   const PackedParams p) {
+    using L = Layout<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bars = smem_base + L::kBar;
+    const auto q_full = [&](int x) { return bars + 8u * x; };
+    const auto k_full = [&](int s) { return bars + 8u * (2 + s); };
+    const auto k_empty = [&](int s) { return bars + 8u * (4 + s); };
+    const auto v_full = [&](int s) { return bars + 8u * (6 + s); };
+    const auto v_empty = [&](int s) { return bars + 8u * (8 + s); };
+    const auto v_seen = [&](int s) { return bars + 8u * (10 + s); };     // looked over
+    const auto s_full = [&](int x) { return bars + 8u * (12 + x); };
+    const auto p_half = [&](int x) { return bars + 8u * (14 + x); };     // the first 64 keys' weights
+    const auto p_full = [&](int x) { return bars + 8u * (16 + x); };
+    const auto o_done = [&](int x) { return bars + 8u * (18 + x); };
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBar + 192);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + L::kBar + 200);
+    volatile int *any_bad = reinterpret_cast<volatile int *>(gen + L::kBar + 204);
+    int *bad = reinterpret_cast<int *>(gen + L::kBad);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    constexpr int PER = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int r = (int)(w / heads), head = (int)(w % heads);
-    if (r >= tokens) return;
-    const int i = find_last(n_seqs, r, [&](int j) { return row_offset(cu, j, tokens); });
-    const int r0 = row_offset(cu, i, tokens);
-    if (r < r0 || r >= row_offset(cu, i + 1, tokens)) return;
-    const int hk = head / (heads / kv_heads);
-    float qv[PER], o[PER] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < PER; e++) qv[e] = (float)q[(int64_t)r * ld_q + (int64_t)head * HD + lane * PER + e] * scale;
-    for (int j = r0; j <= r; j++) {
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < PER; e++) s += qv[e] * (float)k[(int64_t)j * ld_k + (int64_t)hk * HD + lane * PER + e];
-#pragma unroll
-        for (int of = 16; of > 0; of >>= 1) s += __shfl_xor_sync(0xffffffffu, s, of);
-        const float mn = fmaxf(m, s), a = m == mn ? 1.0f : __expf(m - mn), p = __expf(s - mn);
-        l = l * a + p;
-#pragma unroll
-        for (int e = 0; e < PER; e++) o[e] = o[e] * a + p * (float)v[(int64_t)j * ld_v + (int64_t)hk * HD + lane * PER + e];
-        m = mn;
+
+    // Which rows.  Sequence s has at least as many places as it has pairs of tiles from cu[s] / (2 tile_tokens) + s on; the last tiles of a sequence,
+    // which see the most keys, come first.
+    const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const int slot = (int)(p.slots - 1u - blockIdx.x / (unsigned)p.kv_heads);
+    const int pair_tokens = 2 * p.tile_tokens;
+    const int seq = find_last(p.n_seqs, slot, [&](int i) { return row_offset(p.cu, i, p.tokens) / pair_tokens + i; });
+    const int start = row_offset(p.cu, seq, p.tokens), len = row_offset(p.cu, seq + 1, p.tokens) - start;
+    const long long first = (long long)(slot - (start / pair_tokens + seq)) * pair_tokens;      // position of tile A's first token
+    if (first < 0 || first >= len) return;
+    const int pos0 = (int)first;
+    // keys that a tile's last token sees, and the tiles of keys they take; B may have no tokens at all
+    const int end_a = min(pos0 + p.tile_tokens, len), end_b = min(pos0 + pair_tokens, len);
+    const int tiles_a = (end_a + kTile - 1) / kTile;
+    const int tiles_b = end_b > end_a ? (end_b + kTile - 1) / kTile : 0;
+    const int tiles = max(tiles_a, tiles_b);
+    const int look_from = (pos0 + 1) / kTile;           // first tile of keys that tile A's first token does not see as a whole
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; s++) {
+            mbar_init(q_full(s), 1);
+            mbar_init(k_full(s), 1);
+            mbar_init(k_empty(s), 1);
+            mbar_init(v_full(s), 1);
+            mbar_init(v_empty(s), 1);
+            mbar_init(v_seen(s), 2);
+            mbar_init(s_full(s), 1);
+            mbar_init(p_half(s), 4);
+            mbar_init(p_full(s), 4);
+            mbar_init(o_done(s), 1);
+        }
+        *abort_flag = 0;
+        *any_bad = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    for (int i = threadIdx.x; i < 3 * HD; i += kThreads) bad[i] = INT_MAX;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp < 8) {
+        // ---------------- softmax + output: a thread per row ----------------
+        const int x = warp >> 2;
+        const int r = (warp & 3) * 32 + lane;
+        const int tok = r / p.group, hq = r - tok * p.group;
+        const int pos = pos0 + x * p.tile_tokens + tok;
+        const bool row_ok = tok < p.tile_tokens && pos < len;
+        const int lim = row_ok ? pos + 1 : 0;                    // keys that the row sees
+        const int my_tiles = x ? tiles_b : tiles_a;
+        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem_base + t_lane + (uint32_t)(x * 128);
+        const uint32_t t_o = tmem_base + t_lane + 256u + (uint32_t)(x * HD);
+        float m_run = -3.402823466e38f, l_run = 0.0f;
+        bool ok = true;
+        const auto do_tile = [&](auto masked_tag, const int j) -> bool {
+            constexpr bool MASKED = decltype(masked_tag)::value;
+            const bool good = mbar_wait(s_full(x), (uint32_t)j & 1u, abort_flag, p.status, (14u << 24) | 1u, true);
+            if (!__all_sync(0xffffffffu, good)) return false;
+            tc_fence_after();
+            const int left = lim - j * kTile;                    // columns >= left are hidden
+            // The scores are read out of tensor memory twice, 32 columns ahead of their use: once for the maximum, once for the weights.
+            uint32_t v[2][32];
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tc_ld_32x32(t_s, v[0]);
 #pragma unroll
-    for (int e = 0; e < PER; e++) out[(int64_t)r * ld_out + (int64_t)head * HD + lane * PER + e] = (T)(o[e] / l);
+            for (int c = 0; c < 4; c++) {
+                tc_wait_ld_dep(v[c & 1]);
+                tc_ld_32x32(t_s + (uint32_t)(((c + 1) & 3) * 32), v[(c + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float a = !MASKED || c * 32 + i < left ? __uint_as_float(v[c & 1][i]) : -INFINITY;
+                    const float b = !MASKED || c * 32 + i + 1 < left ? __uint_as_float(v[c & 1][i + 1]) : -INFINITY;
+                    m4[(i >> 1) & 3] = fmaxf(fmaxf(m4[(i >> 1) & 3], a), b);
+                }
+            }
+            const float m_cand = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+            const float m_new = (m_cand > m_run + kLazy) ? m_cand : m_run;
+            const float alpha = ex2(m_run - m_new);
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                // O holds the products up to tile j - 1: s_full of tile j was committed behind them
+#pragma unroll 1
+                for (int c = 0; c < HD / 16; c++) {
+                    uint32_t o[16];
+                    tc_ld_16(t_o + (uint32_t)(c * 16), o);
+                    tc_wait_ld_16(o);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tc_st_16(t_o + (uint32_t)(c * 16), o);
+                }
+            }
+            const uint64_t c2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-m_new, -m_new);
+            uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t pk[16];
+                tc_wait_ld_dep(v[c & 1]);
+                if (c < 3) tc_ld_32x32(t_s + (uint32_t)((c + 1) * 32), v[(c + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float a0, a1;
+                    unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), c2, nm2), a0, a1);
+                    float e0 = ex2(a0), e1 = ex2(a1);
+                    if (MASKED) {
+                        if (c * 32 + 2 * i >= left) e0 = 0.0f;
+                        if (c * 32 + 2 * i + 1 >= left) e1 = 0.0f;
+                    }
+                    sum2[i & 1] = add_f2(sum2[i & 1], pack_f2(e0, e1));
+                    pk[i] = pack2<T>(e0, e1);
+                }
+                tc_st_16(t_s + (uint32_t)(c * 16), pk);
+                if (c & 1) {
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c == 1 ? p_half(x) : p_full(x));
+                }
+            }
+            float s0, s1;
+            unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
+            l_run = l_run * alpha + (s0 + s1);
+            m_run = m_new;
+            return true;
+        };
+        // a tile of keys that every row of this tile sees as a whole needs no mask
+        const int whole = pos0 + x * p.tile_tokens + 1;
+        const bool rows_full = end_b - pos0 >= (x + 1) * p.tile_tokens && p.tile_tokens * p.group == kTile;
+        for (int j = 0; ok && j < my_tiles; j++)
+            ok = rows_full && (j + 1) * kTile <= whole ? do_tile(std::false_type{}, j) : do_tile(std::true_type{}, j);
+        if (ok && my_tiles > 0) {
+            ok = mbar_wait(o_done(x), 0, abort_flag, p.status, (14u << 24) | 3u, true);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                tc_fence_after();
+                const float inv_l = 1.0f / l_run;
+                T *dst = static_cast<T *>(p.out) + (long long)(start + pos) * p.ld_out + (long long)(head * p.group + hq) * HD;
+                const bool fix = *any_bad != 0;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t v[32];
+                    tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
+                    tc_wait_ld_dep(v);
+                    if (!row_ok) continue;
+                    if (fix) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            float o = __uint_as_float(v[i]);
+                            const int col = c * 32 + i;
+                            if (lim > bad[col]) o += __uint_as_float(0x7fc00000u);
+                            if (lim > bad[HD + col]) o += INFINITY;
+                            if (lim > bad[2 * HD + col]) o -= INFINITY;
+                            v[i] = __float_as_uint(o);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            w[e] = pack2<T>(__uint_as_float(v[8 * i + 2 * e]) * inv_l, __uint_as_float(v[8 * i + 2 * e + 1]) * inv_l);
+                        reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+    } else {
+        if (warp == 8) {
+            // ---------------- TMA ----------------
+            if (lane == 0) {
+                const uint32_t q_bytes = (uint32_t)(L::kAtoms * 128 * p.tile_tokens * p.group);
+                const auto load_q = [&](int x) {
+                    mbar_arrive_expect_tx(q_full(x), q_bytes);
+                    for (int a = 0; a < L::kAtoms; a++)
+                        tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, head * p.group,
+                                    start + pos0 + x * p.tile_tokens);
+                };
+                bool ok = true;
+                load_q(0);
+                for (int j = 0; ok && j < tiles; j++) {
+                    const int st = j % kStages;
+                    const uint32_t ph = (uint32_t)(j / kStages) & 1u;
+                    ok = mbar_wait(k_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x10u | st, true);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(k_full(st), L::kAtoms * kAtomBytes);
+                    for (int a = 0; a < L::kAtoms; a++)
+                        tma_load_3d(smem_base + L::kK + (st * L::kAtoms + a) * kAtomBytes, &map_k, k_full(st), a * 64, head, start + j * kTile);
+                    if (j == 0 && tiles_b > 0) load_q(1);
+                    ok = mbar_wait(v_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x20u | st, true);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(v_full(st), L::kAtoms * kAtomBytes);
+                    for (int a = 0; a < L::kAtoms; a++)
+                        tma_load_3d(smem_base + L::kV + (st * L::kAtoms + a) * kAtomBytes, &map_v, v_full(st), a * 64, head, start + j * kTile);
+                }
+            }
+        } else if (warp == 9) {
+            // ---------------- MMA ----------------
+            if (lane == 0) {
+                const uint32_t idesc_qk = make_idesc<T>(kTile, false), idesc_pv = make_idesc<T>(HD, true);
+                const auto issue_qk = [&](int x, int t) {
+                    const uint32_t ka = smem_base + L::kK + (t % kStages) * L::kAtoms * kAtomBytes;
+                    const uint32_t qa = smem_base + L::kQ + x * L::kAtoms * kAtomBytes;
+#pragma unroll
+                    for (int a = 0; a < L::kAtoms; a++) {
+                        const uint64_t qd = make_kmajor_sw128_desc(qa + a * kAtomBytes), kd = make_kmajor_sw128_desc(ka + a * kAtomBytes);
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++)
+                            tc_mma_ss(tmem_base + (uint32_t)(x * 128), qd + 2u * kk, kd + 2u * kk, idesc_qk, (a | kk) ? 1u : 0u);
+                    }
+                    tc_commit(s_full(x));
+                };
+                const auto issue_pv = [&](int x, int t, int part) {
+                    const uint64_t vd = make_mn_major_desc(smem_base + L::kV + (t % kStages) * L::kAtoms * kAtomBytes);
+#pragma unroll
+                    for (int k2 = 0; k2 < 4; k2++) {
+                        const int kk = 4 * part + k2;           // 16 keys: 8 columns of P, 2048 bytes of V
+                        tc_mma_ts(tmem_base + 256u + (uint32_t)(x * HD), tmem_base + (uint32_t)(x * 128 + 8 * kk), vd + 128u * kk, idesc_pv,
+                                  (t > 0 || kk > 0) ? 1u : 0u);
+                    }
+                };
+                bool ok = mbar_wait(q_full(0), 0, abort_flag, p.status, (13u << 24) | 1u);
+                if (ok) ok = mbar_wait(k_full(0), 0, abort_flag, p.status, (13u << 24) | 2u);
+                if (ok) {
+                    tc_fence_after();
+                    issue_qk(0, 0);
+                    if (tiles_b > 0) {
+                        ok = mbar_wait(q_full(1), 0, abort_flag, p.status, (13u << 24) | 9u);
+                        if (ok) issue_qk(1, 0);
+                    }
+                    tc_commit(k_empty(0));
+                }
+                for (int j = 0; ok && j < tiles; j++) {
+                    const int st = j % kStages;
+                    const bool more = j + 1 < tiles;
+                    ok = mbar_wait(v_seen(st), (uint32_t)(j / kStages) & 1u, abort_flag, p.status, (13u << 24) | 3u);
+                    bool k_there = false;
+                    for (int x = 0; ok && x < 2; x++) {
+                        const int mine = x ? tiles_b : tiles_a;
+                        if (j < mine) {
+                            ok = mbar_wait(p_half(x), (uint32_t)j & 1u, abort_flag, p.status, (13u << 24) | 4u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_pv(x, j, 0);
+                            ok = mbar_wait(p_full(x), (uint32_t)j & 1u, abort_flag, p.status, (13u << 24) | 5u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_pv(x, j, 1);
+                            if (j + 1 == mine) tc_commit(o_done(x));
+                        }
+                        if (x == 1) tc_commit(v_empty(st));
+                        if (j + 1 < mine) {
+                            if (!k_there) {
+                                ok = mbar_wait(k_full((j + 1) % kStages), (uint32_t)((j + 1) / kStages) & 1u, abort_flag, p.status, (13u << 24) | 6u);
+                                if (!ok) break;
+                                tc_fence_after();
+                                k_there = true;
+                            }
+                            issue_qk(x, j + 1);
+                        }
+                    }
+                    if (ok && more) tc_commit(k_empty((j + 1) % kStages));
+                }
+            }
+        } else {
+            // ---------------- V: warps 10 and 11, half of a tile's rows each ----------------
+            constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;      // exponent all ones: NaN or infinity
+            constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+            bool ok = true;
+            for (int j = 0; ok && j < tiles; j++) {
+                const int st = j % kStages;
+                ok = mbar_wait(v_full(st), (uint32_t)(j / kStages) & 1u, abort_flag, p.status, (15u << 24) | 1u, true);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (j >= look_from) {
+                    for (int a = 0; a < L::kAtoms; a++) {
+                        const uint32_t base = smem_base + L::kV + (st * L::kAtoms + a) * kAtomBytes + (uint32_t)(warp - 10) * (kAtomBytes / 2);
+#pragma unroll 4
+                        for (int i = lane; i < kAtomBytes / 32; i += 32) {
+                            const uint4 w = ld_shared_v4(base + 16u * i);
+                            const uint32_t hit = (((w.x & kExp) + kOne) | ((w.y & kExp) + kOne) | ((w.z & kExp) + kOne) | ((w.w & kExp) + kOne)) & 0x80008000u;
+                            if (hit) {
+                                const int row = (warp - 10) * 64 + i / 8, key = j * kTile + row;
+                                const int col0 = a * 64 + ((i & 7) ^ (row & 7)) * 8;
+                                uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                                for (int e = 0; e < 8; e++) {
+                                    const uint32_t h = (u[e >> 1] >> (16 * (e & 1))) & 0xffffu, ex = kExp & 0xffffu;
+                                    if ((h & ex) != ex) continue;
+                                    if (key < len) {
+                                        const int kind = (h & ~(ex | 0x8000u) & 0xffffu) != 0 ? 0 : (h & 0x8000u) ? 2 : 1;
+                                        atomicMin(bad + kind * HD + col0 + e, key);
+                                        *any_bad = 1;
+                                    }
+                                    u[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
+                                }
+                                st_shared_v4(base + 16u * i, u[0], u[1], u[2], u[3]);
+                            }
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_seen(st));
+            }
+        }
+    }
+
+    // ---------------- teardown ----------------
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {          // copies may be in flight: let them land before the memory goes
+        for (int i = 0; i < 200; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    }
+}
+
+// [tokens][heads][hd] with rows ld elements apart; a box is 64 columns x `box_heads` heads x `box_tokens` tokens, swizzled by 128 bytes
+int make_map(tpb_handle_t h, CUtensorMap *map, int dtype, const void *base, int64_t tokens, int heads, int hd, int64_t ld, int box_heads,
+             int box_tokens) {
+    const cuuint64_t dim[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t stride[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult r = reinterpret_cast<EncodeTiledFn>(h->encode_tiled)(
+        map, dtype == TPB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dim, stride, box,
+        step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return tpb_fail(h, TPB_ERR_CUDA, "cuTensorMapEncodeTiled (packed attention) failed (%d)", (int)r);
+    return TPB_OK;
+}
+
+template <typename T, int HD>
+int launch_packed(tpb_handle_t h, cudaStream_t st, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const PackedParams &p) {
+    static tpb_per_device_once smem_set;
+    TPB_CUDA(h, tpb_set_max_smem_once(h, attn_packed_kernel<T, HD>, Layout<HD>::kBytes, smem_set));
+    TPB_CUDA(h, tpb_launch_pdl(attn_packed_kernel<T, HD>, dim3(p.slots * (unsigned)p.kv_heads), dim3(kThreads), (size_t)Layout<HD>::kBytes, st, mq, mk,
+                               mv, p));
+    return TPB_OK;
 }
 
 }  // namespace
@@ -63,18 +551,31 @@ int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t
                   "attention_packed: row strides must be multiples of 8 elements");
     TPB_CHECK_ARG(h, tpb_aligned16(out) && tpb_aligned16(q) && tpb_aligned16(k) && tpb_aligned16(v) && (reinterpret_cast<uintptr_t>(cu) & 3u) == 0,
                   "attention_packed: pointers must be 16-byte aligned (cu: 4)");
+    PackedParams p;
+    p.out = out;
+    p.ld_out = ld_out;
+    p.cu = cu;
+    p.n_seqs = n_seqs;
+    p.tokens = (int)tokens;
+    p.group = heads / kv_heads;
+    p.kv_heads = kv_heads;
+    p.tile_tokens = kTile / p.group;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.status = h->d_status;
+    const int64_t slots = tokens / (2 * p.tile_tokens) + n_seqs;
+    TPB_CHECK_ARG(h, slots * kv_heads < INT32_MAX, "attention_packed: tokens * heads exceeds the grid");
+    p.slots = (unsigned)slots;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
-    const auto run = [&](auto *tag) {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        const auto launch = [&](auto kern) {
-            return tpb_launch_pdl(kern, dim3((unsigned)((tokens * heads + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, (T *)out, ld_out, (const T *)q,
-                                  ld_q, (const T *)k, ld_k, (const T *)v, ld_v, cu, n_seqs, (int)tokens, heads, kv_heads, scale);
-        };
-        return head_dim == 64 ? launch(attn_packed_kernel<T, 64>) : launch(attn_packed_kernel<T, 128>);
-    };
-    TPB_CUDA(h, dtype == TPB_BF16 ? run((__nv_bfloat16 *)nullptr) : run((__half *)nullptr));
-    return TPB_OK;
+    CUtensorMap mq, mk, mv;
+    int rc = make_map(h, &mq, dtype, q, tokens, heads, head_dim, ld_q, p.group, p.tile_tokens);
+    if (rc == TPB_OK) rc = make_map(h, &mk, dtype, k, tokens, kv_heads, head_dim, ld_k, 1, kTile);
+    if (rc == TPB_OK) rc = make_map(h, &mv, dtype, v, tokens, kv_heads, head_dim, ld_v, 1, kTile);
+    if (rc != TPB_OK) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == TPB_BF16)
+        return head_dim == 64 ? launch_packed<__nv_bfloat16, 64>(h, st, mq, mk, mv, p) : launch_packed<__nv_bfloat16, 128>(h, st, mq, mk, mv, p);
+    return head_dim == 64 ? launch_packed<__half, 64>(h, st, mq, mk, mv, p) : launch_packed<__half, 128>(h, st, mq, mk, mv, p);
 }
 
 }  // extern "C"
