@@ -524,7 +524,9 @@ int tpb_kv_compact(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c);
  *          behind the sequence's end read as zero.
  * attention  rows are the queries of the sequence's last cu[i+1] - cu[i] tokens, causal among themselves:
  *          out[r] = sum_{j <= p(r)} softmax_j(scale * q[r] . k[j]) v[j],  p(r) = lens - (cu[i+1] - r); zero where p(r) < 0.
- *          heads a multiple of kv_heads, scale finite and not negative.  f32 accuracy: q and the probabilities are split in two f16 terms, the cache's values are exact.
+ *          heads a multiple of kv_heads, scale finite and not negative.  f32 accuracy for f32 and f16 rows:
+ *          q and the probabilities are split in two f16 terms; bf16 rows: one f16 term each (q's is exact).  The cache's values are exact; an
+ *          e4m3 byte that a row of the batch sees must not be NaN (append writes none).
  *          max_len: an upper bound of the lengths that the host knows (0 = none): a hint that saves a launch for short sequences.
  *          workspace: tpb_kv_attention_workspace_bytes(h, head_dim) bytes, 16-byte aligned, of this call alone while it runs. */
 int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, const void *k, int64_t ld_k, const void *v,

@@ -284,6 +284,12 @@ def filled(be, lens, fmt, page, kv, hd, seed, spare=6):
     return c, m
 
 
+# What the weights lose before the second product.  f32 and f16 rows: two f16 terms, hi = rn(w) and lo = rn(w - hi), |w - hi - lo| <= 2^-11 |w - hi| <=
+# 2^-22 w, or below the smallest f16 step relative to the reference (added apart).  bf16 rows: one f16 term, |w - rn(w)| <= 2^-11 w, an eighth of
+# the half step of the bf16 result.
+WEIGHTS = {"f32": 2.0 ** -21, "f16": 2.0 ** -21, "bf16": HALF_STEP["f16"]}
+
+
 def check_attention(c, m, out, q, seqs, n_new, heads, dt, scale=None):
     kv, hd = c.kv_heads, c.head_dim
     scale = hd ** -0.5 if scale is None else scale
@@ -295,8 +301,8 @@ def check_attention(c, m, out, q, seqs, n_new, heads, dt, scale=None):
         for h in range(heads):
             mine, hk = slice(h * hd, (h + 1) * hd), h // (heads // kv)
             o, a, e = attend(q[at:at + n, mine], k[:, hk], v[:, hk], last, scale)
-            # q and the weights in two f16 terms each: what is left of them is below 2^-21 of a row's largest
-            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], 2.0 ** -21) + len(k) * 2.0 ** -33 * (np.abs(v).max() if len(k) else 0)
+            # q in two f16 terms (bf16: exact in one): what is left of it is below 2^-21 of a row's largest
+            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], WEIGHTS[dt]) + len(k) * 2.0 ** -33 * (np.abs(v).max() if len(k) else 0)
             err = np.abs(got[at:at + n, mine] - o)
             assert (err <= tol).all(), (s, n, h, float((err / tol).max()), float(err.max()))
         at += n
@@ -393,7 +399,7 @@ def test_scores_and_values_of_a_wide_range(be, fmt, dt):
             o, a, e = attend(qq, k[:, hk], v[:, hk], [lens[s] - 1], hd ** -0.5)
             p = np.exp((k[:, hk] @ qq[0]) * hd ** -0.5 - ((k[:, hk] @ qq[0]) * hd ** -0.5).max())
             biggest = (p / p.sum() * np.abs(v[:, hk]).max(1)).max()
-            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], 2.0 ** -21) + len(k) * 2.0 ** -30 * biggest
+            tol = tolerance(o, a, e * (1 + 2.0 ** 4), hd, HALF_STEP[dt], WEIGHTS[dt]) + len(k) * 2.0 ** -30 * biggest
             err = np.abs(got[r, h * hd:(h + 1) * hd] - o[0])
             assert (err <= tol).all(), (s, h, float((err / tol).max()))
 
