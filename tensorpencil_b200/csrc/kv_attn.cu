@@ -3,21 +3,26 @@
 //   out[r] = sum_j softmax_j(scale q[r] . k[j]) v[j],   k = ks * qk, v = vs * qv with one scale a page and head
 //
 // Bound by the cache's bytes, which are read once: 2 * head_dim a token and kv head.  What carries that:
-//   - All query rows that share a kv head (tokens x heads of the group) are one operand of mma.sync m16n8k16 (f16, f32 sums).  The
-//     cached values are exact in f16.  A tcgen05 tile would have 128 rows where a decode step has 1 to 32; a row is the other operand's cost here.
-//   - f32 accuracy (SPLIT): a row takes two of the sixteen, q = hi + lo in f16 (after scaling the row by a power of two), and the weights
-//     likewise; a group of up to eight rows leaves the second half of the tile empty anyway.  bf16 queries are exact in one f16 term, and
-//     weights of one f16 term (2^-12) are below a bf16 result's half step (2^-9): no split there, sixteen rows a tile.
-//   - Page scales are uniform over a step of 16 tokens (a page holds 16, 32 or 64): ks multiplies scores, vs the weights.
-//   - A warp owns its data path: 16 tokens of K and V a step by cp.async into a ring of its own, no barrier between warps.  Bytes lie in shared
-//     memory with their 16-byte pieces permuted so that K's 16-byte reads and V's 4-byte reads are free of bank conflicts; the
-//     order of dimensions within the products is the one in which a thread finds its bytes, and q is laid out to match.
-//   - The work of all (sequence, kv head, row tile)s is one line of units of 64 tokens, cut into equal pieces, one a CTA.  A CTA that has
+//   - All query rows that share a kv head (tokens x heads of the group) are the N side of mma.sync m16n8k16 (f16, f32 sums), eight a tile;
+//     tokens (K q^T) and dimensions (V^T P^T) are the M side, so that a decode step's few rows leave nothing of a product unused, as they
+//     would of a tcgen05 tile of 128 rows.  The cached values are exact in f16.
+//   - f32 accuracy (SPLIT) for f32 and f16 rows: q = hi + lo in f16 (after scaling the row by a power of two), and the weights likewise, two
+//     products each.  bf16 queries are exact in one f16 term, and weights of one f16 term (2^-12) are below a bf16 result's half step (2^-9).
+//   - K's int8 goes into the product as it is: byte ^ 0x80 in the low byte of an f16 is the number (128 + k) 2^-24, and the sum's start value
+//     takes the 128 sum(q) off again (a fixed number a row).  V's cancels less well over a long sequence and is converted exactly.
+//   - Page scales are uniform over a piece of 16 tokens (a page holds 16, 32 or 64): ks multiplies scores, vs the weights.
+//   - A warp owns its data path: K and V of 16 or 32 tokens a step by cp.async into a ring of its own, no barrier between warps, and the next
+//     run's first step is on its way while a run's sums are merged.  Bytes lie in shared memory with their 16-byte pieces
+//     permuted so that K's 16-byte reads and V's 4-byte reads are free of bank conflicts; the order of dimensions within the products is the one in
+//     which a thread finds its bytes, and q is laid out to match.
+//   - The work of all (sequence, kv head, row tile)s is one line of units of tokens, cut into equal pieces, one a CTA.  A CTA that has
 //     not all of a sequence's tokens leaves a partial result; a second kernel joins them in the order of the tokens, so the
 //     result is the same from run to run.
 //
 // Softmax.  Per row two running references, both whole numbers in log2 units so that every rescaling is exact: ms >= max s - kLazy for the sum
-// l = sum 2^(s - ms), and mw for the weights w = 2^(s - mw + kUp) vs, whose size depends on the page's scale as well.
+// l = sum 2^(s - ms), and mw for the weights w = 2^(s + log2 vs - mw + kUp), whose size depends on the page's scale as well.
+#include <algorithm>
+
 #include "kv_common.cuh"
 
 using namespace tpb_kv;
@@ -26,23 +31,28 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
-constexpr int kUnit = 64;            // tokens of a unit of work: one step of every warp
-constexpr int kStep = 16;            // tokens of a warp's step
-constexpr int kMinUnits = 4;         // a CTA takes at least so many units: shorter pieces cost more in joining than they gain
+constexpr int kPiece = 16;           // tokens with one page and scale
+constexpr int kMinTokens = 256;      // a CTA takes at least so many: shorter runs cost more in joining than they gain
 constexpr int kRing = 16384;         // bytes of a warp's ring
 constexpr float kLazy = 6.0f, kUp = 6.0f;      // w < 2^(kLazy + kUp + 1) fits f16
 
-template <int HD, bool SPLIT, int MT>
+template <int HD, bool SPLIT, int NT>
 struct Cfg {
-    static constexpr int kRows = (SPLIT ? 8 : 16) * MT;                  // rows of a tile
+    static constexpr int kRows = 8 * NT;                                 // rows of a tile
+    static constexpr int kHalves = NT <= 2 ? 2 : 1;                      // pieces of a warp's step
+    static constexpr int kStep = kHalves * kPiece;                       // tokens of a warp's step
+    static constexpr int kUnit = kWarps * kStep;                         // tokens of a unit of work: one step of every warp
     static constexpr int kStageBytes = 2 * kStep * HD;
-    static constexpr int kStages = kRing / kStageBytes;                  // 4 (head_dim 128) or 8
-    static constexpr int kSteps = HD / 16;                               // k steps of q k^T
-    static constexpr int kQf = MT > 1 ? MT * kSteps * 32 * 16 : 0;       // q's fragments in shared memory (MT = 1: in registers)
-    static constexpr int kSmem = kWarps * kRing + kQf;
-    static constexpr int kMergeLd = kRows * (HD + 4) * 4 <= kRing ? HD + 4 : HD;      // a warp's sums lie over its ring on their way to the others
-    static_assert(kRows * kMergeLd * 4 <= kRing && kRows <= 32, "sums fit the ring and a slot");
-    static constexpr int kCtas = MT == 1 ? 3 : 2;                        // per SM
+    static constexpr int kStages = kRing / kStageBytes;                  // 2 to 8
+    static constexpr int kSteps = HD / 16;                               // k steps of K q^T
+    static constexpr int kTerms = SPLIT ? 2 : 1;
+    static constexpr bool kQRegs = NT * kTerms <= 2 && HD * NT * kTerms <= 256;      // q's fragments in registers
+    static constexpr int kQf = kQRegs ? 0 : NT * kSteps * kTerms * 32 * 8;           // or in shared memory
+    static constexpr int kMergeLd = HD + 4;
+    static constexpr int kMerge = kRows * kMergeLd * 4;                  // where the warps' sums are added up
+    static constexpr int kSmem = kWarps * kRing + kMerge + kQf;
+    static constexpr int kCtas = NT == 1 ? 3 : 2;                        // per SM
+    static_assert(kRows <= 32, "rows fit a slot");
 };
 constexpr int kMaxCtas = 3, kMaxRows = 32;
 
@@ -70,6 +80,7 @@ struct AttnParams {
     float scale_log2;
     int whole;                           // sequences are not cut: a unit is all of one
     float *ws;
+    void *notes;                         // a JoinNote a CTA
     uint32_t *status;
 };
 
@@ -80,11 +91,12 @@ struct Chunk {
     int len[kThreads], row0[kThreads], n_q[kThreads], seq[kThreads];
     long long warp_sum[kThreads / 32];
 };
-__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : max(1, (len + kUnit - 1) / kUnit); }
+template <int UNIT>
+__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : max(1, (len + UNIT - 1) / UNIT); }
 
 // Loads sequences base .. base + kThreads - 1, the first of which begins at unit `cum`; returns the unit behind the last.  `tell`: report ids and
 // lengths out of range (such a sequence has no units: its rows are not written).
-template <int RT>
+template <int RT, int UNIT>
 __device__ long long load_chunk(const AttnParams &p, Chunk &ck, int base, long long cum, bool tell) {
     const int i = base + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long units = 0;
@@ -101,7 +113,7 @@ __device__ long long load_chunk(const AttnParams &p, Chunk &ck, int base, long l
                 if (len < 0 || (long long)len > (long long)p.c.max_pages * p.c.page_tokens) {
                     if (tell) report(p.status, kBadLen);
                 } else {
-                    units = (long long)tiles_of(p, len) * p.c.kv_heads * (((long long)n_q * p.group + RT - 1) / RT);
+                    units = (long long)tiles_of<UNIT>(p, len) * p.c.kv_heads * (((long long)n_q * p.group + RT - 1) / RT);
                 }
             }
         }
@@ -147,11 +159,11 @@ struct Segment {
     int head, row_tile, t0, t1, tiles;   // tiles [t0, t1) of `tiles`
     long long first;                     // unit of tile 0
 };
-template <int RT>
+template <int RT, int UNIT>
 __device__ __forceinline__ Segment segment_at(const AttnParams &p, const Chunk &ck, long long u, long long u_end) {
     Segment s;
     s.idx = find_in_chunk(ck, u);
-    s.tiles = tiles_of(p, ck.len[s.idx]);
+    s.tiles = tiles_of<UNIT>(p, ck.len[s.idx]);
     const long long rel = u - ck.start[s.idx];
     const long long which = rel / s.tiles;
     s.t0 = (int)(rel - which * s.tiles);
@@ -162,8 +174,9 @@ __device__ __forceinline__ Segment segment_at(const AttnParams &p, const Chunk &
     s.first = u - s.t0;
     return s;
 }
+template <int UNIT>
 __device__ __forceinline__ long long units_per_cta(const AttnParams &p, long long total, int ctas) {
-    return max((total + ctas - 1) / ctas, (long long)(p.whole ? 1 : kMinUnits));
+    return max((total + ctas - 1) / ctas, (long long)(p.whole ? 1 : kMinTokens / UNIT));
 }
 
 // ---- arithmetic -------------------------------------------------------------------------------
@@ -173,10 +186,21 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }       // -126 <= e <= 127
-__device__ __forceinline__ void mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+// d = a b + c
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {          // of 16-bit values, row lane / 4
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -189,28 +213,39 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = half2_bits(a - f.x, b - f.y);
 }
-// int8 pairs in the low bytes of both halves -> f16: 0x6400 | (x ^ 0x80) is 1024 + 128 + x
+// int8 pairs in the low bytes of both halves -> f16, exactly: 0x6400 | (x ^ 0x80) is 1024 + 128 + x
 __device__ __forceinline__ uint32_t s8_pair(uint32_t w) {
     uint32_t b;
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(b) : "r"(w), "r"(0x00ff00ffu), "r"(0x64806480u));     // (w & mask) ^ bias
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&b), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+// (128 + x) 2^-24 as subnormal f16
+__device__ __forceinline__ uint32_t s8_pair_raw(uint32_t w) {
+    uint32_t b;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(b) : "r"(w), "r"(0x00ff00ffu), "r"(0x00800080u));
+    return b;
+}
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
     return (uint32_t)h.x | ((uint32_t)h.y << 16);
 }
-// Four consecutive bytes of K as the two registers of a k step: (bytes 0, 2), (1, 3) of s8, (0, 1), (2, 3) of e4m3.
+// (a & m) | (b & n) with m = the signs, n = e4m3's exponent and mantissa at the top of an f16's lower fifteen bits: value * 2^-8
+__device__ __forceinline__ uint32_t e4m3_bits(uint32_t sign, uint32_t rest) { return (sign & 0x80008000u) | (rest & 0x3f803f80u); }
+// Four consecutive bytes of K as the two registers of a k step, bytes (0, 2) and (1, 3), times kUnitOfK.  e4m3 by shifts and masks: the conversion
+// instruction runs at a quarter of their rate, and V keeps its pipe busy.
 template <int FORMAT>
 __device__ __forceinline__ void k_regs(uint32_t w, uint32_t &b0, uint32_t &b1) {
     if constexpr (FORMAT == TPB_KV_S8) {
-        b0 = s8_pair(w);
-        b1 = s8_pair(w >> 8);
+        b0 = s8_pair_raw(w);
+        b1 = s8_pair_raw(w >> 8);
     } else {
-        b0 = e4m3_pair(w & 0xffffu);
-        b1 = e4m3_pair(w >> 16);
+        b0 = e4m3_bits(w << 8, w << 7);
+        b1 = e4m3_bits(w, w >> 1);
     }
 }
+template <int FORMAT>
+constexpr float kPerUnitOfK = FORMAT == TPB_KV_S8 ? 16777216.0f : 256.0f;      // 2^24, 2^8
 // Four columns of V for two tokens: v[e] = (a's byte e, b's byte e).
 template <int FORMAT>
 __device__ __forceinline__ void v_regs(uint32_t a, uint32_t b, uint32_t (&v)[4]) {
@@ -243,8 +278,11 @@ __device__ __forceinline__ int piece_at(int tok, int piece) {
     return tok * HD + ((piece ^ (tok & 7)) << 4);
 }
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {     // bytes 16, or 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -297,446 +335,577 @@ __device__ __forceinline__ float finish_scale(float ms, float l, float mw, float
     return ex2(e - h) / l;
 }
 
-template <int HD, int FORMAT, bool SPLIT, int MT>
-__global__ void __launch_bounds__(kThreads, Cfg<HD, SPLIT, MT>::kCtas)
+// What the join needs to know of the run that CTA c began and did not end; rows = 0: nothing to join.
+struct JoinNote {
+    int rows, last_cta;
+    long long out_row;               // of the run's first row; the rest by row tile, head and group
+    int row_tile, head;
+};
+__host__ __device__ inline size_t note_floats(int ctas) { return (size_t)ctas * (sizeof(JoinNote) / 4); }
+
+template <int HD, int FORMAT, bool SPLIT, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<HD, SPLIT, NT>::kCtas)
 kv_attention_kernel(const AttnParams p) {
-    using C = Cfg<HD, SPLIT, MT>;
-    constexpr int RT = C::kRows;
-    constexpr int R = SPLIT ? 1 : 2;                       // rows a thread has per m tile: g, and g + 8
+    using C = Cfg<HD, SPLIT, NT>;
+    constexpr int RT = C::kRows, UNIT = C::kUnit, H = C::kHalves, TERMS = C::kTerms;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Chunk ck;
-    __shared__ float s_ms[kWarps][RT], s_l[kWarps][RT], s_mw[kWarps][RT], s_rs[MT > 1 ? RT : 1];
+    __shared__ float s_ms[kWarps][RT], s_l[kWarps][RT], s_mw[kWarps][RT], s_rs[C::kQRegs ? 1 : RT], s_bias[C::kQRegs ? 1 : RT];
+    tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    tpb_grid_dep_launch();                                 // behind the wait: the join may look at lengths as soon as it starts
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
     long long total = 0;
-    for (int base = 0; base < p.n_seqs; base += kThreads) total = load_chunk<RT>(p, ck, base, total, blockIdx.x == 0);
-    const long long per = units_per_cta(p, total, (int)gridDim.x);
+    for (int base = 0; base < p.n_seqs; base += kThreads) total = load_chunk<RT, UNIT>(p, ck, base, total, blockIdx.x == 0);
+    const long long per = units_per_cta<UNIT>(p, total, (int)gridDim.x);
     long long u = per * blockIdx.x;
     const long long u_end = min(u + per, total);
-    if (u >= u_end) return;
-    int base = 0;
-    if (p.n_seqs > kThreads) {
-        long long behind = load_chunk<RT>(p, ck, 0, 0, false);
-        while (u >= behind) {
-            base += kThreads;
-            behind = load_chunk<RT>(p, ck, base, behind, false);
-        }
-    }
-
-    const uint32_t ring = smem_addr(smem) + warp * kRing;
-    uint4 *qf_smem = reinterpret_cast<uint4 *>(smem + kWarps * kRing);
-    while (u < u_end) {
-        while (u >= ck.start[kThreads]) {
-            base += kThreads;
-            load_chunk<RT>(p, ck, base, ck.start[kThreads], false);
-        }
-        const Segment s = segment_at<RT>(p, ck, u, u_end);
-        const int len = ck.len[s.idx], n_q = ck.n_q[s.idx], row0 = ck.row0[s.idx], seq = ck.seq[s.idx];
-        const int n_rows = n_q * p.group - s.row_tile * RT;           // of this tile, if below RT
-        const auto token_row = [&](int r) { return (s.row_tile * RT + r) / p.group; };      // which of the sequence's queries row r belongs to
-
-        // ---- q: scaled by a power of two to a largest value in [2^10, 2^11), as f16 terms ----
-        uint4 qf[MT == 1 ? C::kSteps : 1];
-        float rs[R];                                                  // MT = 1: scale log2(e) / that power
-        const auto build_q = [&](int mt, uint4 *dst, int stride, float (&r_s)[R]) {
-            float v[R][HD / 64][16];
-#pragma unroll
-            for (int e = 0; e < R; e++) {
-                const int r = mt * (SPLIT ? 8 : 16) + g + 8 * e;
-                const int flat = s.row_tile * RT + r, tok = flat / p.group;
-                float amax = 0.0f;
-#pragma unroll
-                for (int cc = 0; cc < HD / 64; cc++) {
-                    load_q(p, HD, row0 + tok, s.head * p.group + flat - tok * p.group, 16 * (t + 4 * cc), r < n_rows, v[e][cc]);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) amax = fmaxf(amax, fabsf(v[e][cc][i]));
-                }
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int ex = max((int)(__float_as_uint(amax) >> 23) - 127, -116);       // 0: all zero, or below 2^-116
-                const float up = pow2i(min(10 - ex, 126));
-                r_s[e] = p.scale_log2 * pow2i(max(ex - 10, -126));
-#pragma unroll
-                for (int cc = 0; cc < HD / 64; cc++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) v[e][cc][i] *= up;
+    JoinNote note = {};
+    if (u < u_end) {
+        int base = 0;
+        if (p.n_seqs > kThreads) {
+            long long behind = load_chunk<RT, UNIT>(p, ck, 0, 0, false);
+            while (u >= behind) {
+                base += kThreads;
+                behind = load_chunk<RT, UNIT>(p, ck, base, behind, false);
             }
-#pragma unroll
-            for (int cc = 0; cc < HD / 64; cc++)
-#pragma unroll
-                for (int k4 = 0; k4 < 4; k4++) {
-                    // the pairs in which a thread finds K's bytes
-                    constexpr int i1 = FORMAT == TPB_KV_S8 ? 2 : 1, i2 = FORMAT == TPB_KV_S8 ? 1 : 2;
-                    uint4 a;
-                    if (SPLIT) {
-                        split2(v[0][cc][4 * k4], v[0][cc][4 * k4 + i1], a.x, a.y);
-                        split2(v[0][cc][4 * k4 + i2], v[0][cc][4 * k4 + 3], a.z, a.w);
-                    } else {
-                        a.x = half2_bits(v[0][cc][4 * k4], v[0][cc][4 * k4 + i1]);
-                        a.y = half2_bits(v[R - 1][cc][4 * k4], v[R - 1][cc][4 * k4 + i1]);
-                        a.z = half2_bits(v[0][cc][4 * k4 + i2], v[0][cc][4 * k4 + 3]);
-                        a.w = half2_bits(v[R - 1][cc][4 * k4 + i2], v[R - 1][cc][4 * k4 + 3]);
-                    }
-                    dst[(cc * 4 + k4) * stride] = a;
-                }
-        };
-        if constexpr (MT == 1) {
-            build_q(0, qf, 1, rs);
-        } else {
-            for (int mt = warp; mt < MT; mt += kWarps) {
-                float r_s[R];
-                build_q(mt, qf_smem + mt * C::kSteps * 32 + lane, 32, r_s);
-#pragma unroll
-                for (int e = 0; e < R; e++)
-                    if (t == 0) s_rs[mt * (SPLIT ? 8 : 16) + g + 8 * e] = r_s[e];
-            }
-            __syncthreads();
         }
+        // where this lane's bytes lie in a stage: the pieces that it copies, K's 16 bytes of a token, V's words of two tokens
+        const uint32_t ring = smem_addr(smem) + warp * kRing;
+        float *merge = reinterpret_cast<float *>(smem + kWarps * kRing);
+        uint2 *qf_smem = reinterpret_cast<uint2 *>(smem + kWarps * kRing + C::kMerge);
+        constexpr int CP = HD / 32;                        // pieces a lane copies of a 16-token piece of K or V
+        uint32_t cp_at[CP], k_at[HD / 64], v_at[2];
+#pragma unroll
+        for (int i = 0; i < CP; i++) cp_at[i] = piece_at<HD>((lane + 32 * i) / (HD / 16), (lane + 32 * i) % (HD / 16));
+#pragma unroll
+        for (int cc = 0; cc < HD / 64; cc++) k_at[cc] = piece_at<HD>(token_of_col<HD>(g), t + 4 * cc);
+#pragma unroll
+        for (int i = 0; i < 2; i++) v_at[i] = C::kStep * HD + piece_at<HD>(token_of_col<HD>(2 * t + i), g >> 2) + 4 * (g & 3);
 
-        // ---- the sequence's tokens [tok0, tok1), 16 a step, every fourth step this warp's ----
-        const int tok0 = s.t0 * kUnit, tok1 = p.whole ? len : min(s.t1 * kUnit, len);
-        const int n_steps = tok1 > tok0 + warp * kStep ? (tok1 - tok0 - warp * kStep + kUnit - 1) / kUnit : 0;
-        const auto step_tok = [&](int n) { return tok0 + n * kUnit + warp * kStep; };
-        const int32_t *row = p.c.table + (size_t)seq * p.c.max_pages;
-        // pages and scales of 32 steps, a step a lane, and of the 32 behind them
+        // ---- the run at hand: its tokens [mine0, tok1), every kWarps-th step this warp's ----
+        Segment s = {};
+        int len, n_q, row0, tok1, mine0, n_steps, now0;
+        const int32_t *row;
+        // Places and scales of 32 pieces, a piece a lane, and of the 32 behind them.
         struct Ahead {
-            int page;
+            int at;                                         // row of the cache of the piece's first token and this head; -1: no piece there, or no page
             float ks, vs;
-        };
+        } now, next;
+        constexpr int kBatch = 32 / H;                      // steps
         const auto look = [&](int n0) {
             Ahead a;
-            a.page = -1;
+            a.at = -1;
             a.ks = a.vs = 0.0f;
-            if (n0 + lane < n_steps) {
-                a.page = __ldcg(row + step_tok(n0 + lane) / p.c.page_tokens);
-                if (a.page < 0 || a.page >= p.c.n_pages) {
+            const int piece = n0 * H + lane, tok = mine0 + piece / H * UNIT + piece % H * kPiece;
+            if (tok < tok1) {
+                const int page = __ldcg(row + tok / p.c.page_tokens);
+                if (page < 0 || page >= p.c.n_pages) {
                     report(p.status, kBadPage);
-                    a.page = -1;
                 } else {
-                    const size_t block = ((size_t)p.layer * p.c.n_pages + a.page) * p.c.kv_heads + s.head;
+                    const int block = (int)(((long long)p.layer * p.c.n_pages + page) * p.c.kv_heads) + s.head;
+                    a.at = block * p.c.page_tokens + (tok & (p.c.page_tokens - 1));
                     a.ks = __ldcg(p.c.k_scale + block);
                     a.vs = __ldcg(p.c.v_scale + block);
                 }
             }
             return a;
         };
-        Ahead now = look(0), next = n_steps > 32 ? look(32) : now;
-        int now0 = 0;
         const auto issue = [&](int n) {                     // step n's bytes into its stage; an empty group behind the end
             if (n < n_steps) {
-                const int page = __shfl_sync(0xffffffffu, n < now0 + 32 ? now.page : next.page, n & 31);
-                const int tok = step_tok(n), valid = page < 0 ? 0 : min(kStep, tok1 - tok);
-                const size_t at = ((((size_t)p.layer * p.c.n_pages + max(page, 0)) * p.c.kv_heads + s.head) * p.c.page_tokens + tok % p.c.page_tokens) * HD;
                 const uint32_t st = ring + (n % C::kStages) * C::kStageBytes;
 #pragma unroll
-                for (int i = 0; i < HD / 32; i++) {
-                    const int c = lane + 32 * i, ct = c / (HD / 16), cp = c % (HD / 16);
-                    const bool in = ct < valid;
-                    const size_t from = at + (in ? (size_t)c * 16 : 0);
-                    cp16(st + piece_at<HD>(ct, cp), static_cast<const uint8_t *>(p.c.k) + from, in ? 16 : 0);
-                    cp16(st + kStep * HD + piece_at<HD>(ct, cp), static_cast<const uint8_t *>(p.c.v) + from, in ? 16 : 0);
+                for (int h = 0; h < H; h++) {
+                    const int at = __shfl_sync(0xffffffffu, n < now0 + kBatch ? now.at : next.at, (n * H + h) & 31);
+                    const int valid = at < 0 ? 0 : min(kPiece, tok1 - (mine0 + n * UNIT + h * kPiece));
+                    const size_t from = (size_t)(uint32_t)max(at, 0) * HD + lane * 16;
+                    const uint8_t *k = static_cast<const uint8_t *>(p.c.k) + from, *v = static_cast<const uint8_t *>(p.c.v) + from;
+                    const uint32_t dst = st + h * (kPiece * HD);
+                    if (valid == kPiece) {
+#pragma unroll
+                        for (int i = 0; i < CP; i++) {
+                            cp16(dst + cp_at[i], k + i * 512);
+                            cp16(dst + cp_at[i] + C::kStep * HD, v + i * 512);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < CP; i++) {
+                            const bool in = (lane + 32 * i) / (HD / 16) < valid;
+                            cp16_or_zero(dst + cp_at[i], in ? k + i * 512 : p.c.k, in);
+                            cp16_or_zero(dst + cp_at[i] + C::kStep * HD, in ? v + i * 512 : p.c.v, in);
+                        }
+                    }
                 }
             }
             cp_commit();
         };
-        for (int n = 0; n < C::kStages - 1; n++) issue(n);
-
-        float o[MT][HD / 8][4];
-        float ms[MT][R], l[MT][R], mw[MT][R];
-        int last[MT][R];                                     // the last token that the row sees
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-            for (int nt = 0; nt < HD / 8; nt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[mt][nt][e] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < R; e++) {
-                ms[mt][e] = mw[mt][e] = -INFINITY;
-                l[mt][e] = 0.0f;
-                const int r = mt * (SPLIT ? 8 : 16) + g + 8 * e;
-                last[mt][e] = r < n_rows ? len - n_q + token_row(r) : -1;
+        // Makes the run that begins at unit u the one at hand and sets its first steps on their way.
+        const auto begin = [&]() {
+            while (u >= ck.start[kThreads]) {
+                base += kThreads;
+                load_chunk<RT, UNIT>(p, ck, base, ck.start[kThreads], false);
             }
-        }
-        const int all_see = len - n_q + token_row(0);        // up to here every row of the tile sees every token
+            s = segment_at<RT, UNIT>(p, ck, u, u_end);
+            len = ck.len[s.idx];
+            n_q = ck.n_q[s.idx];
+            row0 = ck.row0[s.idx];
+            row = p.c.table + (size_t)ck.seq[s.idx] * p.c.max_pages;
+            tok1 = p.whole ? len : min(s.t1 * UNIT, len);
+            mine0 = s.t0 * UNIT + warp * C::kStep;
+            n_steps = tok1 > mine0 ? (tok1 - mine0 + UNIT - 1) / UNIT : 0;
+            now0 = 0;
+            now = look(0);
+            next = now;
+            for (int n = 0; n < C::kStages - 1; n++) issue(n);
+            if (n_steps > kBatch) next = look(kBatch);
+        };
+        begin();
+        while (true) {
+            const int n_rows = n_q * p.group - s.row_tile * RT;           // of this tile, if below RT
+            const auto token_row = [&](int r) { return (s.row_tile * RT + r) / p.group; };      // which of the sequence's queries row r belongs to
 
-        for (int n = 0; n < n_steps; n++) {
-            if (n == now0 + 32) {
-                now = next;
-                now0 = n;
-                if (n + 32 < n_steps) next = look(n + 32);
-            }
-            cp_wait<C::kStages - 2>();
-            __syncwarp();
-            const uint32_t st = ring + (n % C::kStages) * C::kStageBytes;
-            const int tok = step_tok(n);
-            const float ks = __shfl_sync(0xffffffffu, now.ks, n & 31), vs = __shfl_sync(0xffffffffu, now.vs, n & 31);
-            const bool skip = __shfl_sync(0xffffffffu, now.page, n & 31) < 0;
-
-            // ---- scores: two tiles of 8 tokens ----
-            float sc[MT][2][4];
+            // ---- q: scaled by a power of two to a largest value in [2^10, 2^11), as f16 terms: row g of a tile, the dimensions of t's bytes ----
+            uint2 qf[C::kQRegs ? NT : 1][C::kQRegs ? C::kSteps : 1][TERMS];
+            float rs[C::kQRegs ? NT : 1][2], bias[C::kQRegs ? NT : 1][2];     // of rows 2t and 2t + 1: scale log2(e) / that power, -128 2^-24 sum q
+            const auto build_q = [&](int nt, uint2 *dst, int stride, float &r_s, float &sum) {
+                const int r = nt * 8 + g, flat = s.row_tile * RT + r, tok = flat / p.group;
+                float v[HD / 64][16];
+                float amax = 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+                for (int cc = 0; cc < HD / 64; cc++) {
+                    load_q(p, HD, row0 + tok, s.head * p.group + flat - tok * p.group, 16 * (t + 4 * cc), r < n_rows, v[cc]);
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sc[mt][j][e] = 0.0f;
-#pragma unroll
-            for (int cc = 0; cc < HD / 64; cc++) {
-                uint4 w[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) w[j] = lds128(st + piece_at<HD>(8 * j + token_of_col<HD>(g), t + 4 * cc));
-#pragma unroll
-                for (int k4 = 0; k4 < 4; k4++) {
-                    uint32_t b[2][2];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) k_regs<FORMAT>(k4 == 0 ? w[j].x : k4 == 1 ? w[j].y : k4 == 2 ? w[j].z : w[j].w, b[j][0], b[j][1]);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        const uint4 a = MT == 1 ? qf[MT == 1 ? cc * 4 + k4 : 0] : qf_smem[(mt * C::kSteps + cc * 4 + k4) * 32 + lane];
-#pragma unroll
-                        for (int j = 0; j < 2; j++) mma(sc[mt][j], a, b[j][0], b[j][1]);
-                    }
+                    for (int i = 0; i < 16; i++) amax = fmaxf(amax, fabsf(v[cc][i]));
                 }
-            }
-            // ---- softmax of the step ----
-            const uint32_t vb = __float_as_uint(vs) & 0x7fffffffu;
-            const int vex = (int)(vb >> 23);                               // 0: zero or below 2^-126; 255: not finite
-            const float ve = vex == 255 ? 0.0f : (float)(max(vex, 1) - 127);
-            const float vm = vex == 255 ? vs : vex == 0 ? vs * 0x1p126f : __uint_as_float((__float_as_uint(vs) & 0x807fffffu) | 0x3f800000u);
-            const bool hide = tok + kStep - 1 > all_see || skip;
-            uint4 pf[MT];
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int ex = max((int)(__float_as_uint(amax) >> 23) - 127, -116);       // -116: all zero, or below 2^-116
+                const float up = pow2i(min(10 - ex, 126));
+                r_s = p.scale_log2 * pow2i(max(ex - 10, -126));
+                sum = 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float x[R][4];                                             // (tile j, column 2t + e) at 2 j + e
+                for (int cc = 0; cc < HD / 64; cc++)
 #pragma unroll
-                for (int e = 0; e < R; e++) {
-                    const float f = ks * (MT == 1 ? rs[e] : s_rs[MT > 1 ? mt * (SPLIT ? 8 : 16) + g + 8 * e : 0]);
-                    float mx = -INFINITY;
+                    for (int k4 = 0; k4 < 4; k4++) {
+                        uint2 b[2];
+                        split2(v[cc][4 * k4] * up, v[cc][4 * k4 + 2] * up, b[0].x, b[1].x);       // the pairs in which a thread finds K's bytes
+                        split2(v[cc][4 * k4 + 1] * up, v[cc][4 * k4 + 3] * up, b[0].y, b[1].y);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float raw = SPLIT ? sc[mt][i >> 1][i & 1] + sc[mt][i >> 1][2 + (i & 1)] : sc[mt][i >> 1][2 * e + (i & 1)];
-                        x[e][i] = raw * f;
-                        if (hide && (skip || tok + 8 * (i >> 1) + token_of_col<HD>(2 * t + (i & 1)) > last[mt][e])) x[e][i] = -INFINITY;
-                        mx = fmaxf(mx, x[e][i]);
-                    }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    // references that grow only when they have to, to whole numbers
-                    const float as = mx > ms[mt][e] + kLazy ? ceilf(mx) : ms[mt][e];
-                    const float aw = mx + ve > mw[mt][e] + kLazy ? ceilf(mx + ve) : mw[mt][e];
-                    if (as != ms[mt][e]) {
-                        l[mt][e] *= ex2(ms[mt][e] - as);
-                        ms[mt][e] = as;
-                    }
-                    const bool grow = aw != mw[mt][e];
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f2 = grow ? ex2(mw[mt][e] - aw) : 1.0f;
-#pragma unroll
-                        for (int nt = 0; nt < HD / 8; nt++) {
-                            o[mt][nt][2 * e] *= f2;
-                            o[mt][nt][2 * e + 1] *= f2;
-                            if (SPLIT) {
-                                o[mt][nt][2] *= f2;
-                                o[mt][nt][3] *= f2;
-                            }
+                        for (int e = 0; e < TERMS; e++) {
+                            dst[((cc * 4 + k4) * TERMS + e) * stride] = b[e];
+                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&b[e].x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&b[e].y));
+                            sum += (f0.x + f0.y) + (f1.x + f1.y);
                         }
-                        mw[mt][e] = aw;
                     }
-                    const float off = ve - mw[mt][e] + kUp;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const bool gone = x[e][i] == -INFINITY;             // hidden (or a score of -inf): no weight, whatever the references are
-                        sum += gone ? 0.0f : ex2(x[e][i] - ms[mt][e]);
-                        x[e][i] = gone ? 0.0f : ex2(x[e][i] + off) * vm;
-                    }
-                    l[mt][e] += sum;
-                }
-                if (SPLIT) {
-                    split2(x[0][0], x[0][1], pf[mt].x, pf[mt].y);
-                    split2(x[0][2], x[0][3], pf[mt].z, pf[mt].w);
-                } else {
-                    pf[mt] = make_uint4(half2_bits(x[0][0], x[0][1]), half2_bits(x[R - 1][0], x[R - 1][1]), half2_bits(x[0][2], x[0][3]),
-                                        half2_bits(x[R - 1][2], x[R - 1][3]));
-                }
-            }
-            // ---- weights times values ----
-            const uint32_t sv = st + kStep * HD + 4 * (g & 3);
-            int at[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) at[i] = 8 * (i >> 1) + token_of_col<HD>(2 * t + (i & 1));
-#pragma unroll
-            for (int i4 = 0; i4 < HD / 32; i4++) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = lds32(sv + piece_at<HD>(at[i], 2 * i4 + (g >> 2)));
-                uint32_t b0[4], b1[4];
-                v_regs<FORMAT>(w[0], w[1], b0);
-                v_regs<FORMAT>(w[2], w[3], b1);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) mma(o[mt][4 * i4 + e], pf[mt], b0[e], b1[e]);
-            }
-            __syncwarp();
-            issue(n + C::kStages - 1);
-        }
-        cp_wait<0>();
-
-        // ---- the four warps' sums ----
-        float *mine = reinterpret_cast<float *>(smem + warp * kRing);
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int e = 0; e < R; e++) {
-                const int r = mt * (SPLIT ? 8 : 16) + g + 8 * e;
-                float sum = l[mt][e];
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t == 0) {
-                    s_ms[warp][r] = ms[mt][e];
-                    s_l[warp][r] = sum;
-                    s_mw[warp][r] = mw[mt][e];
-                }
+                sum *= FORMAT == TPB_KV_S8 ? -128.0f / 16777216.0f : 0.0f;
+            };
+            if constexpr (C::kQRegs) {
 #pragma unroll
-                for (int i4 = 0; i4 < HD / 32; i4++) {
-                    float a[8];
+                for (int nt = 0; nt < NT; nt++) {
+                    float r_s, sum;
+                    build_q(nt, &qf[nt][0][0], 1, r_s, sum);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        a[q] = o[mt][4 * i4 + q][2 * e] + (SPLIT ? o[mt][4 * i4 + q][2] : 0.0f);
-                        a[4 + q] = o[mt][4 * i4 + q][2 * e + 1] + (SPLIT ? o[mt][4 * i4 + q][3] : 0.0f);
+                    for (int e = 0; e < 2; e++) {
+                        rs[nt][e] = __shfl_sync(0xffffffffu, r_s, 4 * (2 * t + e));
+                        bias[nt][e] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e));
                     }
-                    float4 *dst = reinterpret_cast<float4 *>(mine + r * C::kMergeLd + 32 * i4 + 8 * t);
-                    dst[0] = make_float4(a[0], a[1], a[2], a[3]);
-                    dst[1] = make_float4(a[4], a[5], a[6], a[7]);
                 }
-            }
-        __syncthreads();
-        const bool whole = s.t0 == 0 && s.t1 == s.tiles;
-        const Part part = part_of(p.ws, HD, (int)blockIdx.x, s.t0 == 0 ? 1 : 0);
-        for (int i = threadIdx.x; i < min(RT, n_rows) * (HD / 4); i += kThreads) {
-            const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-            float big_s = -INFINITY, big_w = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                big_s = fmaxf(big_s, s_ms[w][r]);
-                big_w = fmaxf(big_w, s_mw[w][r]);
-            }
-            float sum = 0.0f, a[4] = {};
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                sum += s_l[w][r] * part_factor(s_ms[w][r], big_s);
-                const float f = part_factor(s_mw[w][r], big_w);
-                const float4 x = *reinterpret_cast<const float4 *>(smem + w * kRing + (r * C::kMergeLd + d) * 4);
-                a[0] += x.x * f;
-                a[1] += x.y * f;
-                a[2] += x.z * f;
-                a[3] += x.w * f;
-            }
-            if (whole) {
-                float second;
-                const float f = finish_scale(big_s, sum, big_w, second);
-                const int flat = s.row_tile * RT + r, tok = flat / p.group;
-                store4(p, (long long)(row0 + tok) * p.ld_out + (long long)(s.head * p.group + flat - tok * p.group) * HD + d, a[0] * f * second,
-                       a[1] * f * second, a[2] * f * second, a[3] * f * second);
             } else {
-                *reinterpret_cast<float4 *>(part.o + (size_t)r * HD + d) = make_float4(a[0], a[1], a[2], a[3]);
-                if (d == 0) {
-                    part.ms[r] = big_s;
-                    part.l[r] = sum;
-                    part.mw[r] = big_w;
+                for (int nt = warp; nt < NT; nt += kWarps) {
+                    float r_s, sum;
+                    build_q(nt, qf_smem + nt * C::kSteps * TERMS * 32 + lane, 32, r_s, sum);
+                    if (t == 0) {
+                        s_rs[nt * 8 + g] = r_s;
+                        s_bias[nt * 8 + g] = sum;
+                    }
+                }
+                __syncthreads();
+            }
+
+            float o[NT][HD / 16][4];                             // dimensions by g, rows 2t and 2t + 1
+            float ms[NT][2], l[NT][2], mw[NT][2];
+            int last[NT][2];                                     // the last token that the row sees
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[nt][m][e] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    ms[nt][e] = mw[nt][e] = -INFINITY;
+                    l[nt][e] = 0.0f;
+                    const int r = nt * 8 + 2 * t + e;
+                    last[nt][e] = r < n_rows ? len - n_q + token_row(r) : -1;
                 }
             }
+            const int all_see = len - n_q + token_row(0);        // up to here every row of the tile sees every token
+
+            for (int n = 0; n < n_steps; n++) {
+                if (n == now0 + kBatch) {
+                    now = next;
+                    now0 = n;
+                    if (n + kBatch < n_steps) next = look(n + kBatch);
+                }
+                cp_wait<C::kStages - 2>();
+                __syncwarp();                               // everybody's bytes of step n are there, and everybody is done with step n - 1
+                issue(n + C::kStages - 1);
+                const uint32_t st = ring + (n % C::kStages) * C::kStageBytes;
+                const int tok = mine0 + n * UNIT;
+                float ks[H], lv[H];
+                bool skip[H], any_skip = false;
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    const int from = (n * H + h) & 31;
+                    ks[h] = __shfl_sync(0xffffffffu, now.ks, from);
+                    const float vs = __shfl_sync(0xffffffffu, now.vs, from);
+                    lv[h] = vs < 1.17549435e-38f ? -1000.0f : lg2(vs);     // a page of zeros: no weight; NaN stays NaN
+                    skip[h] = __shfl_sync(0xffffffffu, now.at, from) < 0;
+                    any_skip |= skip[h];
+                }
+
+                // ---- scores: sc[.][h] = tokens g and g + 8 of piece h (as token_of_col has them), rows 2t and 2t + 1 ----
+                float sc[NT][H][4];
+#pragma unroll
+                for (int cc = 0; cc < HD / 64; cc++) {
+                    uint4 w[H][2];
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) w[h][j] = lds128(st + k_at[cc] + (2 * h + j) * (8 * HD));
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; k4++) {
+                        uint2 q[NT][TERMS];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < TERMS; e++)
+                                q[nt][e] = C::kQRegs ? qf[C::kQRegs ? nt : 0][C::kQRegs ? cc * 4 + k4 : 0][e]
+                                                     : qf_smem[((nt * C::kSteps + cc * 4 + k4) * TERMS + e) * 32 + lane];
+#pragma unroll
+                        for (int h = 0; h < H; h++) {
+                            uint32_t a[2][2];
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                k_regs<FORMAT>(k4 == 0 ? w[h][j].x : k4 == 1 ? w[h][j].y : k4 == 2 ? w[h][j].z : w[h][j].w, a[j][0], a[j][1]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int e = 0; e < TERMS; e++) {
+                                    float(&d)[4] = sc[nt][h];
+                                    if (cc == 0 && k4 == 0 && e == 0) {
+                                        const float b0 = C::kQRegs ? bias[C::kQRegs ? nt : 0][0] : s_bias[C::kQRegs ? 0 : nt * 8 + 2 * t];
+                                        const float b1 = C::kQRegs ? bias[C::kQRegs ? nt : 0][1] : s_bias[C::kQRegs ? 0 : nt * 8 + 2 * t + 1];
+                                        mma(d, a[0][0], a[1][0], a[0][1], a[1][1], q[nt][e], b0, b1, b0, b1);
+                                    } else {
+                                        mma(d, a[0][0], a[1][0], a[0][1], a[1][1], q[nt][e], d[0], d[1], d[2], d[3]);
+                                    }
+                                }
+                        }
+                    }
+                }
+                // ---- softmax of the step ----
+                const bool hide = any_skip || tok + C::kStep - 1 > all_see;
+                uint2 pf[NT][H][TERMS];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float f[2][H], mx[2], mxw[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float r_s = C::kQRegs ? rs[C::kQRegs ? nt : 0][e] : s_rs[C::kQRegs ? 0 : nt * 8 + 2 * t + e];
+                        mx[e] = mxw[e] = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < H; h++) {
+                            f[e][h] = ks[h] * r_s * kPerUnitOfK<FORMAT>;
+                            if (hide) {
+#pragma unroll
+                                for (int j = 0; j < 2; j++)
+                                    if (skip[h] || tok + h * kPiece + 8 * j + token_of_col<HD>(g) > last[nt][e]) sc[nt][h][2 * j + e] = -INFINITY;
+                            }
+                            const float top = fmaxf(sc[nt][h][e], sc[nt][h][2 + e]) * f[e][h];
+                            mx[e] = fmaxf(mx[e], top);
+                            mxw[e] = fmaxf(mxw[e], top + lv[h]);
+                        }
+                    }
+#pragma unroll
+                    for (int of = 4; of < 32; of <<= 1)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], of));
+                            mxw[e] = fmaxf(mxw[e], __shfl_xor_sync(0xffffffffu, mxw[e], of));
+                        }
+                    // references that grow only when they have to, to whole numbers
+                    const bool grow = mx[0] > ms[nt][0] + kLazy || mxw[0] > mw[nt][0] + kLazy || mx[1] > ms[nt][1] + kLazy || mxw[1] > mw[nt][1] + kLazy;
+                    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float as = mx[e] > ms[nt][e] + kLazy ? ceilf(mx[e]) : ms[nt][e];
+                            const float aw = mxw[e] > mw[nt][e] + kLazy ? ceilf(mxw[e]) : mw[nt][e];
+                            if (as != ms[nt][e]) l[nt][e] *= ex2(ms[nt][e] - as);
+                            const float f2 = aw != mw[nt][e] ? ex2(mw[nt][e] - aw) : 1.0f;
+                            ms[nt][e] = as;
+                            mw[nt][e] = aw;
+#pragma unroll
+                            for (int m = 0; m < HD / 16; m++) {
+                                o[nt][m][e] *= f2;
+                                o[nt][m][2 + e] *= f2;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int e = i & 1;
+                            const float y = sc[nt][h][i];
+                            float a = ex2(fmaf(y, f[e][h], -ms[nt][e])), b = ex2(fmaf(y, f[e][h], lv[h] - mw[nt][e] + kUp));
+                            if (hide && y == -INFINITY) a = b = 0.0f;      // whatever the references and the page's scales are
+                            l[nt][e] += a;
+                            w[i] = b;
+                        }
+                        uint32_t p0[2], p1[2];
+                        if (SPLIT) {
+                            split2(w[0], w[1], p0[0], p0[1]);
+                            split2(w[2], w[3], p1[0], p1[1]);
+                        } else {
+                            p0[0] = half2_bits(w[0], w[1]);
+                            p1[0] = half2_bits(w[2], w[3]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < TERMS; e++) pf[nt][h][e] = make_uint2(transpose8x8(p0[e]), transpose8x8(p1[e]));
+                    }
+                }
+                // ---- values times weights ----
+#pragma unroll
+                for (int i4 = 0; i4 < HD / 32; i4++)
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        // piece 2 i4 + (g >> 2) of the token: the permutation is an exclusive or, and stages begin at multiples of 128 bytes
+                        const uint32_t a0 = (st + v_at[0]) ^ (i4 * 32), a1 = (st + v_at[1]) ^ (i4 * 32);
+                        uint32_t w[4];
+                        w[0] = lds32(a0 + h * (kPiece * HD));
+                        w[1] = lds32(a1 + h * (kPiece * HD));
+                        w[2] = lds32(a0 + h * (kPiece * HD) + 8 * HD);
+                        w[3] = lds32(a1 + h * (kPiece * HD) + 8 * HD);
+                        uint32_t b0[4], b1[4];
+                        v_regs<FORMAT>(w[0], w[1], b0);
+                        v_regs<FORMAT>(w[2], w[3], b1);
+#pragma unroll
+                        for (int m = 0; m < 2; m++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int e = 0; e < TERMS; e++) {
+                                    float(&d)[4] = o[nt][2 * i4 + m];
+                                    mma(d, b0[2 * m], b0[2 * m + 1], b1[2 * m], b1[2 * m + 1], pf[nt][h][e], d[0], d[1], d[2], d[3]);
+                                }
+                    }
+            }
+            cp_wait<0>();
+            __syncwarp();
+
+            // ---- the next run's first steps set off, then the four warps' sums are added up, in the order of the warps ----
+            const Segment done = s;
+            const int done_row0 = row0;
+            u += s.t1 - s.t0;
+            if (u < u_end) begin();
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float sum = l[nt][e];
+#pragma unroll
+                    for (int of = 4; of < 32; of <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, of);
+                    if (g == 0) {
+                        const int r = nt * 8 + 2 * t + e;
+                        s_ms[warp][r] = ms[nt][e];
+                        s_l[warp][r] = sum;
+                        s_mw[warp][r] = mw[nt][e];
+                    }
+                }
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = nt * 8 + 2 * t + e;
+                    float big = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) big = fmaxf(big, s_mw[w][r]);
+                    const float f2 = part_factor(mw[nt][e], big);
+#pragma unroll
+                    for (int m = 0; m < HD / 16; m++) {
+                        o[nt][m][e] *= f2;
+                        o[nt][m][2 + e] *= f2;
+                    }
+                }
+#pragma unroll 1
+            for (int w = 0; w < kWarps; w++) {
+                if (warp == w) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+#pragma unroll
+                            for (int i4 = 0; i4 < HD / 32; i4++) {
+                                float4 *dst = reinterpret_cast<float4 *>(merge + (nt * 8 + 2 * t + e) * C::kMergeLd + 32 * i4 + 4 * g);
+                                float4 x = make_float4(o[nt][2 * i4][e], o[nt][2 * i4][2 + e], o[nt][2 * i4 + 1][e], o[nt][2 * i4 + 1][2 + e]);
+                                if (w > 0) {
+                                    const float4 y = *dst;
+                                    x = make_float4(y.x + x.x, y.y + x.y, y.z + x.z, y.w + x.w);
+                                }
+                                *dst = x;
+                            }
+                }
+                __syncthreads();
+            }
+            const bool whole = done.t0 == 0 && done.t1 == done.tiles;
+            const Part part = part_of(p.ws, HD, (int)blockIdx.x, done.t0 == 0 ? 1 : 0);
+            for (int i = threadIdx.x; i < min(RT, n_rows) * (HD / 4); i += kThreads) {
+                const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+                float big_s = -INFINITY, big_w = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) {
+                    big_s = fmaxf(big_s, s_ms[w][r]);
+                    big_w = fmaxf(big_w, s_mw[w][r]);
+                }
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) sum += s_l[w][r] * part_factor(s_ms[w][r], big_s);
+                const float4 a = *reinterpret_cast<const float4 *>(merge + r * C::kMergeLd + d);
+                if (whole) {
+                    float second;
+                    const float f = finish_scale(big_s, sum, big_w, second);
+                    const int flat = done.row_tile * RT + r, tok = flat / p.group;
+                    store4(p, (long long)(done_row0 + tok) * p.ld_out + (long long)(done.head * p.group + flat - tok * p.group) * HD + d, a.x * f * second,
+                           a.y * f * second, a.z * f * second, a.w * f * second);
+                } else {
+                    *reinterpret_cast<float4 *>(part.o + (size_t)r * HD + d) = a;
+                    if (d == 0) {
+                        part.ms[r] = big_s;
+                        part.l[r] = sum;
+                        part.mw[r] = big_w;
+                    }
+                }
+            }
+            if (done.t0 == 0 && !whole) {
+                note.rows = min(RT, n_rows);
+                note.last_cta = (int)((done.first + done.tiles - 1) / per);
+                note.out_row = done_row0;
+                note.row_tile = done.row_tile;
+                note.head = done.head;
+            }
+            if (u >= u_end) break;
+            __syncthreads();                                 // the sums are read
         }
-        __syncthreads();
-        u += s.t1 - s.t0;
     }
+    if (!p.whole && threadIdx.x == 0) reinterpret_cast<JoinNote *>(p.notes)[blockIdx.x] = note;
 }
 
-// Joins the partial results of the run that CTA blockIdx.x of the kernel above began and did not end: a thread per four dimensions of a row.
+// Joins the partial results of the runs that a CTA of the kernel above began and did not end: one CTA an SM, which looks at the notes of
+// every gridDim.x-th of them (a CTA a note cost three rounds of starting CTAs).  Four rows side by side, 256 threads a row: four dimensions each of
+// eight (head_dim 128) or sixteen interleaved shares of the parts.
+constexpr int kJoinRows = 4, kJoinThreads = 256 * kJoinRows;
 template <int HD, int RT>
-__global__ void __launch_bounds__(256)
-kv_attention_join_kernel(const AttnParams p, int ctas) {
-    __shared__ Chunk ck;
-    // This kernel starts once every CTA of the one before is past its own wait: lengths and offsets are there, partial results are not.
-    long long total = 0;
-    for (int base = 0; base < p.n_seqs; base += kThreads) total = load_chunk<RT>(p, ck, base, total, false);
-    const long long per = units_per_cta(p, total, ctas);
-    const long long u0 = per * blockIdx.x, u1 = min(u0 + per, total);
-    bool work = u0 < u1 && u1 < total;
-    Segment s = {};
-    if (work) {
-        if (p.n_seqs > kThreads) {
-            int base = 0;
-            long long behind = load_chunk<RT>(p, ck, 0, 0, false);
-            while (u1 - 1 >= behind) {
-                base += kThreads;
-                behind = load_chunk<RT>(p, ck, base, behind, false);
-            }
-        }
-        s = segment_at<RT>(p, ck, u1 - 1, u1);
-        work = s.first >= u0 && s.t1 < s.tiles;              // begins here and goes on
-    }
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const AttnParams p, int ctas) {
+    constexpr int kLanes = HD / 4, kShares = 256 / kLanes;
+    __shared__ float s_sum[kJoinRows][kShares];
+    __shared__ float4 s_o[kJoinRows][kShares][kLanes];
+    __shared__ float s_big[kJoinRows][2][8];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    if (!work) return;
-    const int n_q = ck.n_q[s.idx], row0 = ck.row0[s.idx];
-    const int n_rows = min(RT, n_q * p.group - s.row_tile * RT);
-    const int c0 = (int)blockIdx.x, c1 = (int)((s.first + s.tiles - 1) / per);
-    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += (int)blockDim.x) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-        float big_s = -INFINITY, big_w = -INFINITY;
+    const int rl = threadIdx.x / 256, tr = threadIdx.x % 256;
+    const int lane4 = tr % kLanes, share = tr / kLanes;
+    for (int c0 = (int)blockIdx.x; c0 < ctas; c0 += (int)gridDim.x) {
+        const JoinNote *from = reinterpret_cast<const JoinNote *>(p.notes) + c0;
+        const int rows = __ldcg(&from->rows), n = __ldcg(&from->last_cta) - c0 + 1, row_tile = __ldcg(&from->row_tile), head = __ldcg(&from->head);
+        const long long out_row = __ldcg(&from->out_row);
+        for (int r0 = 0; r0 < rows; r0 += kJoinRows) {
+            const int r = min(r0 + rl, rows - 1);
+            float big_s = -INFINITY, big_w = -INFINITY;
+            for (int c = tr; c < n; c += 256) {
+                const Part part = part_of(p.ws, HD, c0 + c, c == 0 ? 1 : 0);
+                big_s = fmaxf(big_s, __ldcg(part.ms + r));
+                big_w = fmaxf(big_w, __ldcg(part.mw + r));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                big_s = fmaxf(big_s, __shfl_xor_sync(0xffffffffu, big_s, o));
+                big_w = fmaxf(big_w, __shfl_xor_sync(0xffffffffu, big_w, o));
+            }
+            if ((tr & 31) == 0) {
+                s_big[rl][0][tr >> 5] = big_s;
+                s_big[rl][1][tr >> 5] = big_w;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                big_s = fmaxf(big_s, s_big[rl][0][w]);
+                big_w = fmaxf(big_w, s_big[rl][1][w]);
+            }
+            float sum = 0.0f;
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int c = c0; c <= c1; c++) {
-            const Part part = part_of(p.ws, HD, c, c == c0 ? 1 : 0);
-            big_s = fmaxf(big_s, __ldcg(part.ms + r));
-            big_w = fmaxf(big_w, __ldcg(part.mw + r));
+            for (int c = share; c < n; c += kShares) {
+                const Part part = part_of(p.ws, HD, c0 + c, c == 0 ? 1 : 0);
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part.o + (size_t)r * HD) + lane4);
+                sum += __ldcg(part.l + r) * part_factor(__ldcg(part.ms + r), big_s);
+                const float f = part_factor(__ldcg(part.mw + r), big_w);
+                a.x += x.x * f;
+                a.y += x.y * f;
+                a.z += x.z * f;
+                a.w += x.w * f;
+            }
+            s_o[rl][share][lane4] = a;
+            if (lane4 == 0) s_sum[rl][share] = sum;
+            __syncthreads();
+            if (share == 0 && r0 + rl < rows) {
+                sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kShares; k++) {
+                    sum += s_sum[rl][k];
+                    if (k == 0) continue;
+                    const float4 x = s_o[rl][k][lane4];
+                    a.x += x.x;
+                    a.y += x.y;
+                    a.z += x.z;
+                    a.w += x.w;
+                }
+                float second;
+                const float f = finish_scale(big_s, sum, big_w, second);
+                const int flat = row_tile * RT + r, tok = flat / p.group;
+                store4(p, (out_row + tok) * p.ld_out + (long long)(head * p.group + flat - tok * p.group) * HD + 4 * lane4, a.x * f * second,
+                       a.y * f * second, a.z * f * second, a.w * f * second);
+            }
+            __syncthreads();
         }
-        float sum = 0.0f, a[4] = {};
-#pragma unroll 4
-        for (int c = c0; c <= c1; c++) {
-            const Part part = part_of(p.ws, HD, c, c == c0 ? 1 : 0);
-            sum += __ldcg(part.l + r) * part_factor(__ldcg(part.ms + r), big_s);
-            const float f = part_factor(__ldcg(part.mw + r), big_w);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(part.o + (size_t)r * HD + d));
-            a[0] += x.x * f;
-            a[1] += x.y * f;
-            a[2] += x.z * f;
-            a[3] += x.w * f;
-        }
-        float second;
-        const float f = finish_scale(big_s, sum, big_w, second);
-        const int flat = s.row_tile * RT + r, tok = flat / p.group;
-        store4(p, (long long)(row0 + tok) * p.ld_out + (long long)(s.head * p.group + flat - tok * p.group) * HD + d, a[0] * f * second, a[1] * f * second,
-               a[2] * f * second, a[3] * f * second);
     }
 }
 
-template <int HD, int FORMAT, bool SPLIT, int MT>
-int launch_attention(tpb_handle_t h, cudaStream_t st, const AttnParams &p, bool may_split) {
-    using C = Cfg<HD, SPLIT, MT>;
+template <int HD, int FORMAT, bool SPLIT, int NT>
+int launch_attention(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
+    using C = Cfg<HD, SPLIT, NT>;
     static tpb_per_device_once smem_set;
-    TPB_CUDA(h, tpb_set_max_smem_once(h, kv_attention_kernel<HD, FORMAT, SPLIT, MT>, C::kSmem, smem_set));
+    TPB_CUDA(h, tpb_set_max_smem_once(h, kv_attention_kernel<HD, FORMAT, SPLIT, NT>, C::kSmem, smem_set));
     const int ctas = h->sm_count * C::kCtas;
-    TPB_CUDA(h, tpb_launch_pdl(kv_attention_kernel<HD, FORMAT, SPLIT, MT>, dim3((unsigned)ctas), dim3(kThreads), (size_t)C::kSmem, st, p));
-    if (may_split)
-        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)ctas), dim3(256), 0, st, p, ctas));
+    TPB_CUDA(h, tpb_launch_pdl(kv_attention_kernel<HD, FORMAT, SPLIT, NT>, dim3((unsigned)ctas), dim3(kThreads), (size_t)C::kSmem, st, p));
+    if (!p.whole)
+        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)h->sm_count), dim3(kJoinThreads), 0, st, p, ctas));
     return TPB_OK;
 }
 
-// Rows of a tile: the fewest m tiles that hold what a sequence of average size has, at most two of 128 dimensions or four of 64 (their sums are
-// in registers).
+// Rows of a tile: 8, 16 or 32, the fewest that hold what a sequence of average size has (their sums are in registers: no more than 32).
 template <int HD, int FORMAT, bool SPLIT>
-int by_rows(tpb_handle_t h, cudaStream_t st, const AttnParams &p, bool may_split) {
+int by_rows(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
     const int64_t rows = ((int64_t)p.rows + p.n_seqs - 1) / p.n_seqs * p.group;
-    const int64_t tiles = (rows + (SPLIT ? 8 : 16) - 1) / (SPLIT ? 8 : 16);
-    if (tiles <= 1) return launch_attention<HD, FORMAT, SPLIT, 1>(h, st, p, may_split);
-    if constexpr (HD == 64 && SPLIT)
-        if (tiles > 2) return launch_attention<HD, FORMAT, SPLIT, 4>(h, st, p, may_split);
-    return launch_attention<HD, FORMAT, SPLIT, 2>(h, st, p, may_split);
+    return rows <= 8 ? launch_attention<HD, FORMAT, SPLIT, 1>(h, st, p)
+                     : rows <= 16 ? launch_attention<HD, FORMAT, SPLIT, 2>(h, st, p) : launch_attention<HD, FORMAT, SPLIT, 4>(h, st, p);
+}
+template <int HD, int FORMAT>
+int by_type(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
+    return p.dtype == TPB_BF16 ? by_rows<HD, FORMAT, false>(h, st, p) : by_rows<HD, FORMAT, true>(h, st, p);
 }
 
 }  // namespace
@@ -745,7 +914,8 @@ extern "C" {
 
 size_t tpb_kv_attention_workspace_bytes(tpb_handle_t h, int head_dim) {
     if (!h || (head_dim != 64 && head_dim != 128)) return 0;
-    return (size_t)h->sm_count * kMaxCtas * 2 * slot_floats(head_dim) * sizeof(float);
+    const int ctas = h->sm_count * kMaxCtas;
+    return ((size_t)ctas * 2 * slot_floats(head_dim) + note_floats(ctas)) * sizeof(float);
 }
 
 int tpb_kv_attention(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, void *out, int64_t ld_out, const void *q,
@@ -786,21 +956,13 @@ int tpb_kv_attention(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c,
     p.group = heads / c->kv_heads;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.ws = static_cast<float *>(workspace);
+    p.notes = p.ws + (size_t)h->sm_count * kMaxCtas * 2 * slot_floats(c->head_dim);
     p.status = h->d_status;
     // sequences known to be short stay whole, which saves the second launch (a longer one that comes all the same is one CTA's work)
-    const bool may_split = max_len == 0 || max_len > kMinUnits * kUnit;
-    p.whole = !may_split;
+    p.whole = max_len > 0 && max_len <= kMinTokens;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool split = dtype != TPB_BF16;
-    const auto by_format = [&](auto hd_tag, auto split_tag) {
-        constexpr int HD = decltype(hd_tag)::value;
-        constexpr bool S = decltype(split_tag)::value;
-        return c->format == TPB_KV_S8 ? by_rows<HD, TPB_KV_S8, S>(h, st, p, may_split) : by_rows<HD, TPB_KV_E4M3, S>(h, st, p, may_split);
-    };
-    using I64 = std::integral_constant<int, 64>;
-    using I128 = std::integral_constant<int, 128>;
-    if (c->head_dim == 64) return split ? by_format(I64{}, std::true_type{}) : by_format(I64{}, std::false_type{});
-    return split ? by_format(I128{}, std::true_type{}) : by_format(I128{}, std::false_type{});
+    if (c->head_dim == 64) return c->format == TPB_KV_S8 ? by_type<64, TPB_KV_S8>(h, st, p) : by_type<64, TPB_KV_E4M3>(h, st, p);
+    return c->format == TPB_KV_S8 ? by_type<128, TPB_KV_S8>(h, st, p) : by_type<128, TPB_KV_E4M3>(h, st, p);
 }
 
 }  // extern "C"
