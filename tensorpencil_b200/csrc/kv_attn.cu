@@ -39,7 +39,7 @@ constexpr float kLazy = 6.0f, kUp = 6.0f;      // w < 2^(kLazy + kUp + 1) fits f
 template <int HD, bool SPLIT, int NT>
 struct Cfg {
     static constexpr int kRows = 8 * NT;                                 // rows of a tile
-    static constexpr int kHalves = NT <= 2 ? 2 : 1;                      // pieces of a warp's step
+    static constexpr int kHalves = NT <= 2 || HD == 64 ? 2 : 1;           // pieces of a warp's step
     static constexpr int kStep = kHalves * kPiece;                       // tokens of a warp's step
     static constexpr int kUnit = kWarps * kStep;                         // tokens of a unit of work: one step of every warp
     static constexpr int kStageBytes = 2 * kStep * HD;
@@ -91,8 +91,10 @@ struct Chunk {
     int len[kThreads], row0[kThreads], n_q[kThreads], seq[kThreads];
     long long warp_sum[kThreads / 32];
 };
+// A run costs about a unit of time more than its tokens do (48 sequences of 1 to 16000 tokens, 8 kv heads: CTAs that drew the short ones were
+// the last to end), so its units begin with one that has no tokens.
 template <int UNIT>
-__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : max(1, (len + UNIT - 1) / UNIT); }
+__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : 1 + (len + UNIT - 1) / UNIT; }
 
 // Loads sequences base .. base + kThreads - 1, the first of which begins at unit `cum`; returns the unit behind the last.  `tell`: report ids and
 // lengths out of range (such a sequence has no units: its rows are not written).
@@ -450,8 +452,8 @@ kv_attention_kernel(const AttnParams p) {
             n_q = ck.n_q[s.idx];
             row0 = ck.row0[s.idx];
             row = p.c.table + (size_t)ck.seq[s.idx] * p.c.max_pages;
-            tok1 = p.whole ? len : min(s.t1 * UNIT, len);
-            mine0 = s.t0 * UNIT + warp * C::kStep;
+            tok1 = p.whole ? len : min((s.t1 - 1) * UNIT, len);
+            mine0 = max(s.t0 - 1, 0) * UNIT + warp * C::kStep;
             n_steps = tok1 > mine0 ? (tok1 - mine0 + UNIT - 1) / UNIT : 0;
             now0 = 0;
             now = look(0);
@@ -611,7 +613,9 @@ kv_attention_kernel(const AttnParams p) {
                 uint2 pf[NT][H][TERMS];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
+                    // Does a score of any thread call for a larger reference?  Mostly not, and then no maximum over the row is needed.
                     float f[2][H], mx[2], mxw[2];
+                    bool grow = false;
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float r_s = C::kQRegs ? rs[C::kQRegs ? nt : 0][e] : s_rs[C::kQRegs ? 0 : nt * 8 + 2 * t + e];
@@ -628,19 +632,17 @@ kv_attention_kernel(const AttnParams p) {
                             mx[e] = fmaxf(mx[e], top);
                             mxw[e] = fmaxf(mxw[e], top + lv[h]);
                         }
+                        grow |= mx[e] > ms[nt][e] + kLazy || mxw[e] > mw[nt][e] + kLazy;
                     }
-#pragma unroll
-                    for (int of = 4; of < 32; of <<= 1)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], of));
-                            mxw[e] = fmaxf(mxw[e], __shfl_xor_sync(0xffffffffu, mxw[e], of));
-                        }
-                    // references that grow only when they have to, to whole numbers
-                    const bool grow = mx[0] > ms[nt][0] + kLazy || mxw[0] > mw[nt][0] + kLazy || mx[1] > ms[nt][1] + kLazy || mxw[1] > mw[nt][1] + kLazy;
                     if (__any_sync(0xffffffffu, grow)) {
+                        // references grow only when they have to, to whole numbers
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
+#pragma unroll
+                            for (int of = 4; of < 32; of <<= 1) {
+                                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], of));
+                                mxw[e] = fmaxf(mxw[e], __shfl_xor_sync(0xffffffffu, mxw[e], of));
+                            }
                             const float as = mx[e] > ms[nt][e] + kLazy ? ceilf(mx[e]) : ms[nt][e];
                             const float aw = mxw[e] > mw[nt][e] + kLazy ? ceilf(mxw[e]) : mw[nt][e];
                             if (as != ms[nt][e]) l[nt][e] *= ex2(ms[nt][e] - as);
@@ -804,83 +806,117 @@ kv_attention_kernel(const AttnParams p) {
     if (!p.whole && threadIdx.x == 0) reinterpret_cast<JoinNote *>(p.notes)[blockIdx.x] = note;
 }
 
-// Joins the partial results of the runs that a CTA of the kernel above began and did not end: one CTA an SM, which looks at the notes of
-// every gridDim.x-th of them (a CTA a note cost three rounds of starting CTAs).  Four rows side by side, 256 threads a row: four dimensions each of
-// eight (head_dim 128) or sixteen interleaved shares of the parts.
-constexpr int kJoinRows = 4, kJoinThreads = 256 * kJoinRows;
+// Joins the partial results of the run that CTA blockIdx.x of the kernel above began and did not end.  Its time is a chain of loads behind the end of
+// that kernel (starting it costs 1 us, a note 0.8), so a thread asks for references, sums and its share of the weighted values all
+// at once, before anything is known of their factors: 131000 tokens 10 us with one dependent load behind another, 5 drafted tokens 25.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinAhead = 8;        // parts of which a thread holds four dimensions
+constexpr int kJoinFactors = 2048;   // (part, row) pairs of a pass
 template <int HD, int RT>
-__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const AttnParams p, int ctas) {
-    constexpr int kLanes = HD / 4, kShares = 256 / kLanes;
-    __shared__ float s_sum[kJoinRows][kShares];
-    __shared__ float4 s_o[kJoinRows][kShares][kLanes];
-    __shared__ float s_big[kJoinRows][2][8];
+__global__ void __launch_bounds__(kJoinThreads, 2) kv_attention_join_kernel(const AttnParams p) {
+    constexpr int kLanes = HD / 4, kGroups = kJoinThreads / kLanes, kPer = kJoinFactors / kJoinThreads;
+    __shared__ float s_ms[kJoinFactors], s_mw[kJoinFactors], s_l[kJoinFactors];
+    __shared__ float s_big[2][32], s_sum[32];
+    __shared__ float4 s_o[kJoinThreads];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    const int rl = threadIdx.x / 256, tr = threadIdx.x % 256;
-    const int lane4 = tr % kLanes, share = tr / kLanes;
-    for (int c0 = (int)blockIdx.x; c0 < ctas; c0 += (int)gridDim.x) {
-        const JoinNote *from = reinterpret_cast<const JoinNote *>(p.notes) + c0;
-        const int rows = __ldcg(&from->rows), n = __ldcg(&from->last_cta) - c0 + 1, row_tile = __ldcg(&from->row_tile), head = __ldcg(&from->head);
-        const long long out_row = __ldcg(&from->out_row);
-        for (int r0 = 0; r0 < rows; r0 += kJoinRows) {
-            const int r = min(r0 + rl, rows - 1);
-            float big_s = -INFINITY, big_w = -INFINITY;
-            for (int c = tr; c < n; c += 256) {
+    const int c0 = (int)blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const JoinNote *from = reinterpret_cast<const JoinNote *>(p.notes) + c0;
+    const int rows = __ldcg(&from->rows), n = __ldcg(&from->last_cta) - c0 + 1, row_tile = __ldcg(&from->row_tile), head = __ldcg(&from->head);
+    const long long out_row = __ldcg(&from->out_row);
+    // few rows: four threads share a row's dimensions, each with every fourth part
+    const int shares = rows * 4 <= kGroups ? 4 : 1;
+    const int rows_at_once = min(min(kGroups / shares, 32), max(kJoinFactors / max(n, 1), 1));
+    const int lane4 = threadIdx.x % kLanes, group = threadIdx.x / kLanes, share = group % shares, rl = group / shares;
+    for (int r0 = 0; r0 < rows; r0 += rows_at_once) {
+        const int rg = min(rows_at_once, rows - r0);
+        const bool mine = rl < rg;
+        const auto load_o = [&](int c) {
+            return __ldcg(reinterpret_cast<const float4 *>(part_of(p.ws, HD, c0 + c, c == 0 ? 1 : 0).o + (size_t)(r0 + rl) * HD) + lane4);
+        };
+        float4 x[kJoinAhead];
+#pragma unroll
+        for (int i = 0; i < kJoinAhead; i++)
+            if (mine && share + i * shares < n) x[i] = load_o(share + i * shares);
+        float l[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int idx = threadIdx.x + i * kJoinThreads;
+            if (idx < n * rg) {
+                const int c = idx / rg, r = r0 + idx - c * rg;
                 const Part part = part_of(p.ws, HD, c0 + c, c == 0 ? 1 : 0);
-                big_s = fmaxf(big_s, __ldcg(part.ms + r));
-                big_w = fmaxf(big_w, __ldcg(part.mw + r));
+                s_ms[idx] = __ldcg(part.ms + r);
+                s_mw[idx] = __ldcg(part.mw + r);
+                l[i] = __ldcg(part.l + r);
+            }
+        }
+        __syncthreads();
+        for (int r = warp; r < rg; r += kJoinThreads / 32) {
+            float big_s = -INFINITY, big_w = -INFINITY;
+            for (int c = lane; c < n; c += 32) {
+                big_s = fmaxf(big_s, s_ms[c * rg + r]);
+                big_w = fmaxf(big_w, s_mw[c * rg + r]);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 big_s = fmaxf(big_s, __shfl_xor_sync(0xffffffffu, big_s, o));
                 big_w = fmaxf(big_w, __shfl_xor_sync(0xffffffffu, big_w, o));
             }
-            if ((tr & 31) == 0) {
-                s_big[rl][0][tr >> 5] = big_s;
-                s_big[rl][1][tr >> 5] = big_w;
+            if (lane == 0) {
+                s_big[0][r] = big_s;
+                s_big[1][r] = big_w;
             }
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 8; w++) {
-                big_s = fmaxf(big_s, s_big[rl][0][w]);
-                big_w = fmaxf(big_w, s_big[rl][1][w]);
-            }
-            float sum = 0.0f;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (int c = share; c < n; c += kShares) {
-                const Part part = part_of(p.ws, HD, c0 + c, c == 0 ? 1 : 0);
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part.o + (size_t)r * HD) + lane4);
-                sum += __ldcg(part.l + r) * part_factor(__ldcg(part.ms + r), big_s);
-                const float f = part_factor(__ldcg(part.mw + r), big_w);
-                a.x += x.x * f;
-                a.y += x.y * f;
-                a.z += x.z * f;
-                a.w += x.w * f;
-            }
-            s_o[rl][share][lane4] = a;
-            if (lane4 == 0) s_sum[rl][share] = sum;
-            __syncthreads();
-            if (share == 0 && r0 + rl < rows) {
-                sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kShares; k++) {
-                    sum += s_sum[rl][k];
-                    if (k == 0) continue;
-                    const float4 x = s_o[rl][k][lane4];
-                    a.x += x.x;
-                    a.y += x.y;
-                    a.z += x.z;
-                    a.w += x.w;
-                }
-                float second;
-                const float f = finish_scale(big_s, sum, big_w, second);
-                const int flat = row_tile * RT + r, tok = flat / p.group;
-                store4(p, (out_row + tok) * p.ld_out + (long long)(head * p.group + flat - tok * p.group) * HD + 4 * lane4, a.x * f * second,
-                       a.y * f * second, a.z * f * second, a.w * f * second);
-            }
-            __syncthreads();
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int idx = threadIdx.x + i * kJoinThreads;
+            if (idx < n * rg) {
+                const int r = idx % rg;
+                s_l[idx] = l[i] * part_factor(s_ms[idx], s_big[0][r]);
+                s_mw[idx] = part_factor(s_mw[idx], s_big[1][r]);
+            }
+        }
+        __syncthreads();
+        for (int r = warp; r < rg; r += kJoinThreads / 32) {
+            float sum = 0.0f;
+            for (int c = lane; c < n; c += 32) sum += s_l[c * rg + r];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) s_sum[r] = sum;
+        }
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto add = [&](const float4 &y, int c) {
+            const float f = s_mw[c * rg + rl];
+            a.x += y.x * f;
+            a.y += y.y * f;
+            a.z += y.z * f;
+            a.w += y.w * f;
+        };
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < kJoinAhead; i++)
+                if (share + i * shares < n) add(x[i], share + i * shares);
+#pragma unroll 4
+            for (int c = share + kJoinAhead * shares; c < n; c += shares) add(load_o(c), c);
+        }
+        s_o[threadIdx.x] = a;
+        __syncthreads();
+        if (mine && share == 0) {
+            for (int k = 1; k < shares; k++) {
+                const float4 y = s_o[threadIdx.x + k * kLanes];
+                a.x += y.x;
+                a.y += y.y;
+                a.z += y.z;
+                a.w += y.w;
+            }
+            float second;
+            const float f = finish_scale(s_big[0][rl], s_sum[rl], s_big[1][rl], second);
+            const int flat = row_tile * RT + r0 + rl, tok = flat / p.group;
+            store4(p, (out_row + tok) * p.ld_out + (long long)(head * p.group + flat - tok * p.group) * HD + 4 * lane4, a.x * f * second,
+                   a.y * f * second, a.z * f * second, a.w * f * second);
+        }
+        __syncthreads();
     }
 }
 
@@ -892,16 +928,17 @@ int launch_attention(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
     const int ctas = h->sm_count * C::kCtas;
     TPB_CUDA(h, tpb_launch_pdl(kv_attention_kernel<HD, FORMAT, SPLIT, NT>, dim3((unsigned)ctas), dim3(kThreads), (size_t)C::kSmem, st, p));
     if (!p.whole)
-        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)h->sm_count), dim3(kJoinThreads), 0, st, p, ctas));
+        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)ctas), dim3(kJoinThreads), 0, st, p));
     return TPB_OK;
 }
 
-// Rows of a tile: 8, 16 or 32, the fewest that hold what a sequence of average size has (their sums are in registers: no more than 32).
+// Rows of a tile: 8, 16, 24 or 32, the fewest that hold what a sequence of average size has (their sums are in registers: no more than 32).
 template <int HD, int FORMAT, bool SPLIT>
 int by_rows(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
     const int64_t rows = ((int64_t)p.rows + p.n_seqs - 1) / p.n_seqs * p.group;
     return rows <= 8 ? launch_attention<HD, FORMAT, SPLIT, 1>(h, st, p)
-                     : rows <= 16 ? launch_attention<HD, FORMAT, SPLIT, 2>(h, st, p) : launch_attention<HD, FORMAT, SPLIT, 4>(h, st, p);
+                     : rows <= 16 ? launch_attention<HD, FORMAT, SPLIT, 2>(h, st, p)
+                                  : rows <= 24 ? launch_attention<HD, FORMAT, SPLIT, 3>(h, st, p) : launch_attention<HD, FORMAT, SPLIT, 4>(h, st, p);
 }
 template <int HD, int FORMAT>
 int by_type(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
