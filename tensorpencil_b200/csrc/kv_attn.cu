@@ -228,26 +228,27 @@ __device__ __forceinline__ uint32_t s8_pair_raw(uint32_t w) {
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(b) : "r"(w), "r"(0x00ff00ffu), "r"(0x00800080u));
     return b;
 }
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// the two e4m3 values of the low or high half of a word -> f16
+template <int HALF>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+    uint32_t d;
+    if (HALF == 0) asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(w));
+    else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(w));
+    return d;
 }
-// (a & m) | (b & n) with m = the signs, n = e4m3's exponent and mantissa at the top of an f16's lower fifteen bits: value * 2^-8
-__device__ __forceinline__ uint32_t e4m3_bits(uint32_t sign, uint32_t rest) { return (sign & 0x80008000u) | (rest & 0x3f803f80u); }
-// Four consecutive bytes of K as the two registers of a k step, bytes (0, 2) and (1, 3), times kUnitOfK.  e4m3 by shifts and masks: the conversion
-// instruction runs at a quarter of their rate, and V keeps its pipe busy.
+// Four consecutive bytes of K as the two registers of a k step, times kPerUnitOfK: bytes (0, 2), (1, 3) of s8, (0, 1), (2, 3) of e4m3.
 template <int FORMAT>
 __device__ __forceinline__ void k_regs(uint32_t w, uint32_t &b0, uint32_t &b1) {
     if constexpr (FORMAT == TPB_KV_S8) {
         b0 = s8_pair_raw(w);
         b1 = s8_pair_raw(w >> 8);
     } else {
-        b0 = e4m3_bits(w << 8, w << 7);
-        b1 = e4m3_bits(w, w >> 1);
+        b0 = e4m3_pair<0>(w);
+        b1 = e4m3_pair<1>(w);
     }
 }
 template <int FORMAT>
-constexpr float kPerUnitOfK = FORMAT == TPB_KV_S8 ? 16777216.0f : 256.0f;      // 2^24, 2^8
+constexpr float kPerUnitOfK = FORMAT == TPB_KV_S8 ? 16777216.0f : 1.0f;        // 2^24
 // Four columns of V for two tokens: v[e] = (a's byte e, b's byte e).
 template <int FORMAT>
 __device__ __forceinline__ void v_regs(uint32_t a, uint32_t b, uint32_t (&v)[4]) {
@@ -258,10 +259,10 @@ __device__ __forceinline__ void v_regs(uint32_t a, uint32_t b, uint32_t (&v)[4])
         v[3] = s8_pair(__byte_perm(a, b, 0x0703));
     } else {
         const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);
-        v[0] = e4m3_pair(lo & 0xffffu);
-        v[1] = e4m3_pair(lo >> 16);
-        v[2] = e4m3_pair(hi & 0xffffu);
-        v[3] = e4m3_pair(hi >> 16);
+        v[0] = e4m3_pair<0>(lo);
+        v[1] = e4m3_pair<1>(lo);
+        v[2] = e4m3_pair<0>(hi);
+        v[3] = e4m3_pair<1>(hi);
     }
 }
 
@@ -490,8 +491,9 @@ kv_attention_kernel(const AttnParams p) {
 #pragma unroll
                     for (int k4 = 0; k4 < 4; k4++) {
                         uint2 b[2];
-                        split2(v[cc][4 * k4] * up, v[cc][4 * k4 + 2] * up, b[0].x, b[1].x);       // the pairs in which a thread finds K's bytes
-                        split2(v[cc][4 * k4 + 1] * up, v[cc][4 * k4 + 3] * up, b[0].y, b[1].y);
+                        constexpr int i1 = FORMAT == TPB_KV_S8 ? 2 : 1, i2 = 3 - i1;      // the pairs in which a thread finds K's bytes
+                        split2(v[cc][4 * k4] * up, v[cc][4 * k4 + i1] * up, b[0].x, b[1].x);
+                        split2(v[cc][4 * k4 + i2] * up, v[cc][4 * k4 + 3] * up, b[0].y, b[1].y);
 #pragma unroll
                         for (int e = 0; e < TERMS; e++) {
                             dst[((cc * 4 + k4) * TERMS + e) * stride] = b[e];
