@@ -25,8 +25,8 @@
 #include "kv_common.cuh"
 
 using namespace tpb_gemm;
-using tpb_kv::find_last;
-using tpb_kv::row_offset;
+using tpb_kv::find_sequence;
+using tpb_kv::Found;
 
 namespace {
 
@@ -188,8 +188,8 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
     const int slot = (int)(p.slots - 1u - blockIdx.x / (unsigned)p.kv_heads);
     const int pair_tokens = 2 * p.tile_tokens;
-    const int seq = find_last(p.n_seqs, slot, [&](int i) { return row_offset(p.cu, i, p.tokens) / pair_tokens + i; });
-    const int start = row_offset(p.cu, seq, p.tokens), len = row_offset(p.cu, seq + 1, p.tokens) - start;
+    const Found b = find_sequence(p.cu, nullptr, p.n_seqs, p.tokens, slot, [&](int i, int r) { return r / pair_tokens + i; });
+    const int seq = b.i, start = b.r0, len = b.r1 - b.r0;
     const long long first = (long long)(slot - (start / pair_tokens + seq)) * pair_tokens;      // position of tile A's first token
     if (first < 0 || first >= len) return;
     const int pos0 = (int)first;

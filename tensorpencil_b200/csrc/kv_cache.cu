@@ -20,94 +20,100 @@ __device__ __forceinline__ float pow2_scale(float amax) {
     return __uint_as_float((uint32_t)(min(max(e, -100), 127 - p) + 127) << 23);
 }
 
-// One CTA per (sequence, page it touches, head): threads 0-127 the keys, 128-255 the values, each with up to CHUNKS pieces of 16 values in
-// registers between the maximum and the rounding, so that the input is read once.  Bound by HBM for prompts, by the chain offsets ->
-// length -> page -> scale for a decode step.
+// One CTA per (sequence, page it touches), head, and keys or values: 128 threads with up to CHUNKS pieces of 16 values each in registers, as
+// they were loaded, between the maximum and the rounding, so that the input is read once.  Bound by HBM for prompts; for a
+// decode step by its chain of loads: offsets and id, length and tail, page and new values, old scale and old values -- what a step of it
+// brings is asked for before anything is decided.
 //
 // Grid x: sequence i has at least as many places as it can touch pages from cu[i] / page_tokens + 2 i on, so that a CTA finds its
 // sequence by a search and the launch needs no lengths on the host.
 template <typename T, int FORMAT, int HD, int CHUNKS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, const T *v, int64_t ld_v, const int32_t *seqs, const int32_t *cu,
                  int n_seqs, int rows, uint32_t *status) {
-    __shared__ float s_max[8];
-    __shared__ int s_bad[8];
+    __shared__ float s_max[4];
+    __shared__ int s_bad[4];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    const int pt = c.page_tokens, x = (int)blockIdx.x, head = (int)blockIdx.y;
-    const int i = find_last(n_seqs, x, [&](int j) { return row_offset(cu, j, rows) / pt + 2 * j; });
-    const int r0 = row_offset(cu, i, rows), n_new = row_offset(cu, i + 1, rows) - r0;
+    const int pt = c.page_tokens, shift = __ffs(pt) - 1, x = (int)blockIdx.x, head = (int)blockIdx.y, t = (int)threadIdx.x;
+    const bool is_v = blockIdx.z != 0;
+    const Found b = find_sequence(cu, seqs, n_seqs, rows, x, [&](int j, int r) { return (r >> shift) + 2 * j; });
+    const int n_new = b.r1 - b.r0;
     if (n_new <= 0) return;
-    const int seq = __ldcg(seqs + i);
-    if (seq < 0 || seq >= c.max_seqs) {
+    if (b.seq < 0 || b.seq >= c.max_seqs) {
         report(status, kBadSeq);
         return;
     }
-    const int len = __ldcg(c.lens + seq);
+    const int len = __ldcg(c.lens + b.seq), tail = __ldcg(c.tail + b.seq);
     if (len < n_new || (long long)len > (long long)c.max_pages * pt) {
         report(status, kBadLen);
         return;
     }
-    if (__ldcg(c.tail + seq) != n_new) {
+    if (tail != n_new) {
         report(status, kBadTail);
         return;
     }
     const int first = len - n_new;
-    const long long pg = (long long)first / pt + (x - (r0 / pt + 2 * i));
+    const long long pg = (long long)(first >> shift) + (x - ((b.r0 >> shift) + 2 * b.i));
     if (pg * pt >= len) return;
-    const int page = __ldcg(c.table + (size_t)seq * c.max_pages + pg);
+    const int page = __ldcg(c.table + (size_t)b.seq * c.max_pages + pg);
+    const int p0 = (int)pg * pt;                                // position of the page's first slot
+    const int held = max(first - p0, 0), fill = min(len - p0, pt);   // slots [0, held) hold earlier tokens, [held, fill) are written
+    const int64_t ld = is_v ? ld_v : ld_k;
+    const T *src = (is_v ? v : k) + (int64_t)(b.r0 + p0 - first) * ld + (int64_t)head * HD;   // + slot * ld
+    Raw16<T> raw[CHUNKS];
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++) {
+        const int slot = (j * 128 + t) / (HD / 16), d = (j * 128 + t) % (HD / 16) * 16;
+        if (slot >= held && slot < fill) load_raw(src + (int64_t)slot * ld + d, raw[j]);
+    }
     if (page < 0 || page >= c.n_pages) {
         report(status, kBadPage);
         return;
     }
-    const int p0 = (int)pg * pt;                                // position of the page's first slot
-    const int held = max(first - p0, 0), fill = min(len - p0, pt);   // slots [0, held) hold earlier tokens, [held, fill) are written
-    const bool is_v = threadIdx.x >= 128;
-    const int t = threadIdx.x & 127;
-    const T *src = (is_v ? v : k) + (int64_t)(r0 + p0 - first) * (is_v ? ld_v : ld_k) + (int64_t)head * HD;   // + slot * ld
-    const int64_t ld = is_v ? ld_v : ld_k;
     const size_t block = ((size_t)layer * c.n_pages + page) * c.kv_heads + head;
-    uint8_t *dst = static_cast<uint8_t *>(is_v ? c.v : c.k) + block * (size_t)(pt * HD);
+    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(is_v ? c.v : c.k) + block * (size_t)(pt * HD));
     float *scale_at = (is_v ? c.v_scale : c.k_scale) + block;
-
-    float val[CHUNKS][16];
+    const float old = held > 0 ? __ldcg(scale_at) : 0.0f;
+    uint4 before[CHUNKS];
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++)
+        if ((j * 128 + t) / (HD / 16) < held) before[j] = __ldcg(dst + j * 128 + t);
     float amax = 0.0f;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < CHUNKS; j++) {
-        const int slot = (j * 128 + t) / (HD / 16), d = (j * 128 + t) % (HD / 16) * 16;
+        const int slot = (j * 128 + t) / (HD / 16);
         if (slot >= held && slot < fill) {
-            load16(src + (int64_t)slot * ld + d, val[j]);
+            float f[16];
+            values_of(raw[j], f);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                amax = fmaxf(amax, fabsf(val[j][e]));
-                bad |= !(fabsf(val[j][e]) <= 3.402823466e38f);
+                amax = fmaxf(amax, fabsf(f[e]));
+                bad |= !(fabsf(f[e]) <= 3.402823466e38f);
             }
         }
     }
-    float old = held > 0 ? __ldcg(scale_at) : 0.0f;
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));       // non-negative floats order like their bits
     bad = __any_sync(0xffffffffu, bad);
-    if ((threadIdx.x & 31) == 0) {
-        s_max[threadIdx.x >> 5] = amax;
-        s_bad[threadIdx.x >> 5] = bad;
+    if ((t & 31) == 0) {
+        s_max[t >> 5] = amax;
+        s_bad[t >> 5] = bad;
     }
     __syncthreads();                                            // also: everybody has the old scale before it is replaced
-    const int w0 = is_v ? 4 : 0;
-    amax = fmaxf(fmaxf(s_max[w0], s_max[w0 + 1]), fmaxf(s_max[w0 + 2], s_max[w0 + 3]));
-    bad = s_bad[w0] | s_bad[w0 + 1] | s_bad[w0 + 2] | s_bad[w0 + 3];
-    bad |= !(old >= 0.0f && old <= 3.402823466e38f);
+    amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] | !(old >= 0.0f && old <= 3.402823466e38f);
     const float scale = bad ? __uint_as_float(0x7fc00000u) : fmaxf(old, pow2_scale<FORMAT>(amax));
     if (t == 0) *scale_at = scale;
+    // the quotient by a power of two is the product with its inverse; an old scale of the caller's own need not be one
+    const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    const float inv = pow2 ? 1.0f / scale : 0.0f, ratio = old / scale;
 #pragma unroll
     for (int j = 0; j < CHUNKS; j++) {
         const int slot = (j * 128 + t) / (HD / 16);
-        uint4 *at = reinterpret_cast<uint4 *>(dst) + (j * 128 + t);
         if (slot < held) {
             if (scale == old || bad) continue;
-            const float ratio = old / scale;
-            const uint4 w = __ldcg(at);
-            uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            uint32_t u[4] = {before[j].x, before[j].y, before[j].z, before[j].w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float f[4];
@@ -116,21 +122,23 @@ kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, cons
                 for (int q = 0; q < 4; q++) f[q] *= ratio;
                 u[e] = pack4<FORMAT>(f);
             }
-            *at = make_uint4(u[0], u[1], u[2], u[3]);
+            dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
         } else if (slot < fill) {
             uint32_t u[4] = {0u, 0u, 0u, 0u};
             if (!bad) {
+                float f[16];
+                values_of(raw[j], f);
 #pragma unroll
-                for (int e = 0; e < 16; e++) val[j][e] = val[j][e] / scale;
+                for (int e = 0; e < 16; e++) f[e] = pow2 ? f[e] * inv : f[e] / scale;
 #pragma unroll
-                for (int e = 0; e < 4; e++) u[e] = pack4<FORMAT>(&val[j][4 * e]);
+                for (int e = 0; e < 4; e++) u[e] = pack4<FORMAT>(&f[4 * e]);
             }
-            *at = make_uint4(u[0], u[1], u[2], u[3]);
+            dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
 }
 
-// A warp per row: finds its sequence and page, then 16 values a lane and step, keys and values.
+// A warp per row: finds its sequence and page, then 16 values a lane and step, keys and values, four steps' loads in flight.
 template <typename T, int FORMAT, int HD>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_t ld_v, const int32_t *seqs, const int32_t *start,
@@ -140,22 +148,19 @@ kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_
     const int lane = threadIdx.x & 31;
     const int r = (int)(blockIdx.x * 8 + (threadIdx.x >> 5));
     if (r >= rows) return;
-    const int i = find_last(n_seqs, r, [&](int j) { return row_offset(cu, j, rows); });
-    const int r0 = row_offset(cu, i, rows);
-    if (r < r0 || r >= row_offset(cu, i + 1, rows)) return;          // a row of no sequence
-    const int seq = __ldcg(seqs + i);
-    const int from = start ? __ldcg(start + i) : 0;
-    if (seq < 0 || seq >= c.max_seqs) {
+    const Found b = find_sequence(cu, seqs, n_seqs, rows, r, [&](int, int r0) { return r0; });
+    if (r < b.r0 || r >= b.r1) return;          // a row of no sequence
+    if (b.seq < 0 || b.seq >= c.max_seqs) {
         report(status, kBadSeq);
         return;
     }
-    const int len = __ldcg(c.lens + seq);
-    const long long pos = (long long)from + (r - r0);
+    const int from = start ? __ldcg(start + b.i) : 0, len = __ldcg(c.lens + b.seq), shift = __ffs(c.page_tokens) - 1;
+    const long long pos = (long long)from + (r - b.r0);
     const bool inside = from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens;
     int page = 0, slot = 0;
     if (inside) {
-        page = __ldcg(c.table + (size_t)seq * c.max_pages + pos / c.page_tokens);
-        slot = (int)(pos % c.page_tokens);
+        page = __ldcg(c.table + (size_t)b.seq * c.max_pages + (pos >> shift));
+        slot = (int)(pos & (c.page_tokens - 1));
         if (page < 0 || page >= c.n_pages) {
             report(status, kBadPage);
             return;
@@ -163,22 +168,36 @@ kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_
     }
     const size_t block0 = ((size_t)layer * c.n_pages + page) * c.kv_heads;
     const int pieces = c.kv_heads * (HD / 16);
-    for (int p = lane; p < 2 * pieces; p += 32) {
-        const bool is_v = p >= pieces;
-        const int q = is_v ? p - pieces : p;
-        const int head = q / (HD / 16), d = q % (HD / 16) * 16;
-        float f[16] = {};
-        if (inside) {
-            const float scale = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
-            const uint8_t *src = static_cast<const uint8_t *>(is_v ? c.v : c.k) + ((block0 + head) * c.page_tokens + slot) * HD + d;
-            const uint4 w = __ldcg(reinterpret_cast<const uint4 *>(src));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    constexpr int kAhead = 4;
+    for (int p0 = lane; p0 < 2 * pieces; p0 += 32 * kAhead) {
+        uint4 w[kAhead];
+        float scale[kAhead];
 #pragma unroll
-            for (int e = 0; e < 4; e++) unpack4<FORMAT>(u[e], &f[4 * e]);
-#pragma unroll
-            for (int e = 0; e < 16; e++) f[e] *= scale;
+        for (int e = 0; e < kAhead; e++) {
+            const int p = p0 + 32 * e;
+            if (inside && p < 2 * pieces) {
+                const bool is_v = p >= pieces;
+                const int q = is_v ? p - pieces : p, head = q / (HD / 16), d = q % (HD / 16) * 16;
+                scale[e] = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
+                w[e] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(is_v ? c.v : c.k) + ((block0 + head) * c.page_tokens + slot) * HD + d));
+            }
         }
-        store16((is_v ? v + (int64_t)r * ld_v : k + (int64_t)r * ld_k) + (int64_t)head * HD + d, f);
+#pragma unroll
+        for (int e = 0; e < kAhead; e++) {
+            const int p = p0 + 32 * e;
+            if (p >= 2 * pieces) break;
+            const bool is_v = p >= pieces;
+            const int q = is_v ? p - pieces : p;
+            float f[16] = {};
+            if (inside) {
+                const uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) unpack4<FORMAT>(u[i], &f[4 * i]);
+#pragma unroll
+                for (int i = 0; i < 16; i++) f[i] *= scale[e];
+            }
+            store16((is_v ? v + (int64_t)r * ld_v : k + (int64_t)r * ld_k) + (int64_t)q * 16, f);
+        }
     }
 }
 
@@ -214,11 +233,11 @@ int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, in
     if (rc != TPB_OK || n_seqs == 0 || rows == 0) return rc;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
-    const dim3 grid((unsigned)(rows / c->page_tokens + 2 * (int64_t)n_seqs), (unsigned)c->kv_heads);
+    const dim3 grid((unsigned)(rows / c->page_tokens + 2 * (int64_t)n_seqs), (unsigned)c->kv_heads, 2u);
     const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         const auto launch = [&](auto kern) {
-            return tpb_launch_pdl(kern, grid, dim3(256), 0, (cudaStream_t)stream, *c, layer, (const T *)k, ld_k, (const T *)v, ld_v, seqs, cu, n_seqs,
+            return tpb_launch_pdl(kern, grid, dim3(128), 0, (cudaStream_t)stream, *c, layer, (const T *)k, ld_k, (const T *)v, ld_v, seqs, cu, n_seqs,
                                   (int)rows, h->d_status);
         };
         const int chunks = c->page_tokens * c->head_dim / 2048;             // 0 (half the threads have a piece) .. 4

@@ -45,49 +45,70 @@ __device__ __forceinline__ int row_offset(const int32_t *cu, int i, int rows) {
     return v < 0 ? 0 : (v > rows ? rows : v);
 }
 
-// The last i in [0, n) with key(i) <= x, key ascending and key(0) <= x; a whole warp calls it, 32 keys a step.  With keys out of order it still
-// ends, at some i in [0, n).
+// Which sequence of the batch: the last i in [0, n) with key(i, cu[i]) <= x, key ascending and the first key <= x; a whole warp calls it.  Up to 32
+// sequences it is one round of loads that brings i's offsets and its id with it, up to 1024 two: these kernels' time for a
+// decode step is their chain of loads.  With offsets out of order it still ends, at some i in [0, n).  seqs may be null.
+struct Found {
+    int i, r0, r1, seq;      // cu[i], cu[i + 1], seqs[i]
+};
 template <typename Key>
-__device__ __forceinline__ int find_last(int n, int x, Key key) {
+__device__ __forceinline__ Found find_sequence(const int32_t *cu, const int32_t *seqs, int n, int rows, int x, Key key) {
     const int lane = threadIdx.x & 31;
     int lo = 0, hi = n;
-    while (hi - lo > 1) {
+    while (hi - lo > 32) {
         const int step = (hi - lo + 31) / 32;
         const int i = lo + lane * step;
-        const bool below = i < hi && (lane == 0 || key(i) <= x);
-        const int c = __popc(__ballot_sync(0xffffffffu, below));
-        lo += (c - 1) * step;
+        const bool below = i < hi && (lane == 0 || key(i, row_offset(cu, i, rows)) <= x);
+        lo += (__popc(__ballot_sync(0xffffffffu, below)) - 1) * step;
         hi = min(lo + step, hi);
     }
-    return lo;
+    const int j = min(lo + lane, hi - 1);
+    const int a = row_offset(cu, j, rows), b = row_offset(cu, j + 1, rows), s = seqs ? __ldcg(seqs + j) : 0;
+    const bool below = lo + lane < hi && (lane == 0 || key(j, a) <= x);
+    const int c = __popc(__ballot_sync(0xffffffffu, below)) - 1;
+    Found f;
+    f.i = lo + c;
+    f.r0 = __shfl_sync(0xffffffffu, a, c);
+    f.r1 = __shfl_sync(0xffffffffu, b, c);
+    f.seq = __shfl_sync(0xffffffffu, s, c);
+    return f;
 }
 
-// Sixteen consecutive values as floats; 16-byte aligned.
+// Sixteen consecutive values, 16-byte aligned: loaded as they are (they may wait in half the registers that floats take) ...
 template <typename T>
-__device__ __forceinline__ void load16(const T *p, float (&v)[16]) {
-    if constexpr (sizeof(T) == 4) {
+struct Raw16 {
+    uint4 w[sizeof(T)];        // 16 * sizeof(T) bytes
+};
+template <typename T>
+__device__ __forceinline__ void load_raw(const T *p, Raw16<T> &r) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p) + i);
-            v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
-        }
-    } else {
+    for (int i = 0; i < (int)sizeof(T); i++) r.w[i] = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
+}
+// ... and as floats
+template <typename T>
+__device__ __forceinline__ void values_of(const Raw16<T> &r, float (&v)[16]) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    for (int i = 0; i < (int)sizeof(T); i++) {
+        const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (std::is_same<T, __half>::value) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-                    v[8 * i + 2 * e] = f.x; v[8 * i + 2 * e + 1] = f.y;
-                } else {
-                    v[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-                    v[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                }
+        for (int e = 0; e < 4; e++) {
+            if constexpr (sizeof(T) == 4) {
+                v[4 * i + e] = __uint_as_float(w[e]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+                v[8 * i + 2 * e] = f.x; v[8 * i + 2 * e + 1] = f.y;
+            } else {
+                v[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
+                v[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
             }
         }
     }
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, float (&v)[16]) {
+    Raw16<T> r;
+    load_raw(p, r);
+    values_of(r, v);
 }
 template <typename T>
 __device__ __forceinline__ void store16(T *p, const float (&v)[16]) {

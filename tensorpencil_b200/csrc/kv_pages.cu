@@ -15,17 +15,6 @@ constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ int pages_of(const tpb_kv_cache &c, int len) { return (len + c.page_tokens - 1) / c.page_tokens; }
 
-// Sum over the block of one value a thread, for every thread; `buf` holds one word a warp and one more.
-__device__ __forceinline__ long long block_sum(long long v, long long *buf) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    long long s = 0;
-    for (int w = 0; w < kWarps; w++) s += buf[w];
-    return s;
-}
 // Exclusive scan over the block of one value a thread.
 __device__ __forceinline__ long long block_scan(long long v, long long *buf, long long &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -47,60 +36,70 @@ __device__ __forceinline__ long long block_scan(long long v, long long *buf, lon
     return base + inc - v;
 }
 
-// A warp's share of the pool: consecutive pages, a multiple of 128 of them (one int4 a lane and step).
-struct Share {
+// The pool's reference counts as a block sees them: a warp has consecutive pages, a multiple of 128 of them, four a lane and step.  The first
+// kHeld steps (16384 pages in all) stay in registers from one pass to the next; a pass behind those reads again.
+constexpr int kHeld = 4;
+constexpr int kOutside = 1;    // pages behind the pool's end are neither free ...
+struct Refs {
     int begin, end;
+    int4 held[kHeld];
 };
-__device__ __forceinline__ Share share_of(const tpb_kv_cache &c) {
-    const int per = (int)((c.n_pages + kWarps * 128 - 1) / (kWarps * 128)) * 128;
-    const long long b = (long long)per * (threadIdx.x >> 5);
-    Share s;
-    s.begin = (int)min(b, (long long)c.n_pages);
-    s.end = (int)min(b + per, (long long)c.n_pages);
-    return s;
-}
-// Four reference counts from page p on; pages past the pool's end read as `outside`.
-__device__ __forceinline__ int4 refs4(const tpb_kv_cache &c, int p, int end, int outside) {
+__device__ __forceinline__ int4 refs4(const tpb_kv_cache &c, int p, int end) {
+    int4 v = make_int4(kOutside, kOutside, kOutside, kOutside);
     if (p + 3 < end) {
         const int32_t *r = c.refs + p;
         if ((reinterpret_cast<uintptr_t>(r) & 15u) == 0) return __ldcg(reinterpret_cast<const int4 *>(r));
         return make_int4(__ldcg(r), __ldcg(r + 1), __ldcg(r + 2), __ldcg(r + 3));
     }
-    int4 v = make_int4(outside, outside, outside, outside);
     if (p < end) v.x = __ldcg(c.refs + p);
     if (p + 1 < end) v.y = __ldcg(c.refs + p + 1);
     if (p + 2 < end) v.z = __ldcg(c.refs + p + 2);
     return v;
 }
-
-// Pages for which pick(page, refs) holds, counted over the block (the total) and in front of this warp's share (`before`).
-template <typename Pick>
-__device__ long long count_pages(const tpb_kv_cache &c, long long *buf, long long &before, int outside, Pick pick) {
-    const Share s = share_of(c);
+__device__ __forceinline__ void load_refs(const tpb_kv_cache &c, Refs &f) {
+    const int per = (int)((c.n_pages + kWarps * 128 - 1) / (kWarps * 128)) * 128;
+    const long long b = (long long)per * (threadIdx.x >> 5);
+    f.begin = (int)min(b, (long long)c.n_pages);
+    f.end = (int)min(b + per, (long long)c.n_pages);
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) f.held[i] = refs4(c, f.begin + 128 * i + 4 * (threadIdx.x & 31), f.end);
+}
+// Calls fn(page, its reference count and those of the three behind it) for the lane's pages, in order, the whole warp together; fn returns whether
+// to go on.
+template <typename Fn>
+__device__ __forceinline__ void each_quad(const tpb_kv_cache &c, const Refs &f, Fn fn) {
     const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < kHeld; i++)
+        if (f.begin + 128 * i < f.end && !fn(f.begin + 128 * i + 4 * lane, f.held[i])) return;
+#pragma unroll 2
+    for (int p = f.begin + 128 * kHeld; p < f.end; p += 128)
+        if (!fn(p + 4 * lane, refs4(c, p + 4 * lane, f.end))) return;
+}
+
+// Pages for which pick(page, refs) holds, counted over the block (the total) and in front of this warp's pages (`before`).
+template <typename Pick>
+__device__ long long count_pages(const tpb_kv_cache &c, const Refs &f, long long *buf, long long &before, Pick pick) {
     int n = 0;
-#pragma unroll 4
-    for (int p = s.begin + 4 * lane; p < s.end; p += 128) {
-        const int4 r = refs4(c, p, s.end, outside);
+    each_quad(c, f, [&](int p, const int4 &r) {
         n += (int)pick(p, r.x) + (int)pick(p + 1, r.y) + (int)pick(p + 2, r.z) + (int)pick(p + 3, r.w);
-    }
+        return true;
+    });
     n = __reduce_add_sync(0xffffffffu, n);
     long long total;
-    const long long at = block_scan(lane == 0 ? n : 0, buf, total);
+    const long long at = block_scan((threadIdx.x & 31) == 0 ? n : 0, buf, total);
     before = __shfl_sync(0xffffffffu, at, 0);
     return total;
 }
 // Their indices in ascending order into list[0 .. want); `before` from count_pages with the same pick.
 template <typename Pick>
-__device__ void list_pages(const tpb_kv_cache &c, int32_t *list, long long before, long long want, int outside, Pick pick) {
-    const Share s = share_of(c);
+__device__ void list_pages(const tpb_kv_cache &c, const Refs &f, int32_t *list, long long before, long long want, Pick pick) {
     const int lane = threadIdx.x & 31;
     long long at = before;
-    for (int p0 = s.begin; p0 < s.end && at < want; p0 += 128) {
-        const int p = p0 + 4 * lane;
-        const int4 r = refs4(c, p, s.end, outside);
-        const bool f[4] = {pick(p, r.x), pick(p + 1, r.y), pick(p + 2, r.z), pick(p + 3, r.w)};
-        const int n = (int)f[0] + (int)f[1] + (int)f[2] + (int)f[3];
+    if (at >= want) return;
+    each_quad(c, f, [&](int p, const int4 &r) {
+        const bool q[4] = {pick(p, r.x), pick(p + 1, r.y), pick(p + 2, r.z), pick(p + 3, r.w)};
+        const int n = (int)q[0] + (int)q[1] + (int)q[2] + (int)q[3];
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -110,16 +109,16 @@ __device__ void list_pages(const tpb_kv_cache &c, int32_t *list, long long befor
         long long mine = at + inc - n;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (f[e]) {
+            if (q[e]) {
                 if (mine < want) list[mine] = p + e;
                 mine++;
             }
         at += __shfl_sync(0xffffffffu, inc, 31);
-    }
+        return at < want;
+    });
 }
 
 __device__ __forceinline__ bool is_free(int, int refs) { return refs == 0; }
-constexpr int kOutside = 1;    // pages behind the pool's end are not free
 
 __device__ __forceinline__ void set_result(const tpb_kv_cache &c, int status, long long free_pages, long long taken, long long needed) {
     if (threadIdx.x != 0) return;
@@ -129,63 +128,100 @@ __device__ __forceinline__ void set_result(const tpb_kv_cache &c, int status, lo
     c.result[3] = (int)min(needed, (long long)INT32_MAX);
 }
 
-// Every id of the list in range and none twice?  The same for all threads.  marks of the listed ids are 1 afterwards.
-__device__ bool distinct(const tpb_kv_cache &c, const int32_t *ids, int n, int32_t *marks) {
-    bool ok = true;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int id = __ldcg(ids + i);
-        if (id < 0 || id >= c.max_seqs) ok = false;
-        else marks[id] = 0;
+// A mark a sequence: bits in shared memory for up to kMarkBits sequences, else words of the cache's scratch (marks of the ids in question only).
+constexpr int kMarkBits = 32768;
+struct Marks {
+    uint32_t *bits;
+    int32_t *words;
+    bool small;
+    __device__ void clear(const int32_t *ids, int n, int max_seqs) const {
+        if (small) {
+            for (int i = threadIdx.x; i < (max_seqs + 31) / 32; i += kThreads) bits[i] = 0;
+        } else {
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                const int id = __ldcg(ids + i);
+                if (id >= 0 && id < max_seqs) words[id] = 0;
+            }
+        }
     }
-    if (!__syncthreads_and(ok)) return false;
-    for (int i = threadIdx.x; i < n; i += kThreads)
-        if (atomicAdd(marks + __ldcg(ids + i), 1) != 0) ok = false;
-    return __syncthreads_and(ok);
-}
+    __device__ bool set(int id) const {           // was it set?
+        if (small) return (atomicOr(bits + (id >> 5), 1u << (id & 31)) >> (id & 31)) & 1u;
+        return atomicAdd(words + id, 1) != 0;
+    }
+    __device__ bool test(int id) const { return small ? (bits[id >> 5] >> (id & 31)) & 1u : __ldcg(words + id) != 0; }
+};
+
+// The first entry of a list that a thread deals with is in a register: list[threadIdx.x].
+struct Listed {
+    const int32_t *list;
+    int mine;
+    __device__ Listed(const int32_t *l, int n) : list(l), mine(l && (int)threadIdx.x < n ? __ldcg(l + threadIdx.x) : 0) {}
+    __device__ int at(int i) const { return !list ? 0 : i == (int)threadIdx.x ? mine : __ldcg(list + i); }
+};
+
+// A CTA's bookkeeping is a chain of dependent loads and barriers, 0.3 to 0.5 us each, so what does not depend on one another is asked for
+// together (the lists, the reference counts), what a later pass needs stays in registers, and offsets and marks are in shared memory.
+// fork + truncate of 32 sequences over 1300 pages: 28 -> 17 us with the copies.
+constexpr int kSmallList = 1024;
 
 __global__ void __launch_bounds__(kThreads)
 kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new, int n) {
     __shared__ long long buf[kWarps];
+    __shared__ uint32_t bits[kMarkBits / 32];
+    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
     const Scratch sc = scratch_of(c);
+    const Listed ids(seqs, n), adds(n_new, n);
+    Refs refs;
+    load_refs(c, refs);
+    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
+    int32_t *offsets = n <= kSmallList ? small_offsets : sc.offsets;
     const long long most = (long long)c.max_pages * c.page_tokens;
-    bool ok = distinct(c, seqs, n, sc.marks);
+    marks.clear(seqs, n, c.max_seqs);
+    __syncthreads();
+    bool ok = true;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int id = ids.at(i);
+        if (id < 0 || id >= c.max_seqs || marks.set(id)) ok = false;
+    }
+    long long before = 0;
+    const long long free_pages = count_pages(c, refs, buf, before, is_free);
+    ok = __syncthreads_and(ok);
     long long need = 0;
     if (ok) {
         for (int i0 = 0; i0 < n; i0 += kThreads) {
             const int i = i0 + threadIdx.x;
             int want = 0;
             if (i < n) {
-                const int len = __ldcg(c.lens + __ldcg(seqs + i)), add = __ldcg(n_new + i);
+                const int len = __ldcg(c.lens + ids.at(i)), add = adds.at(i);
                 if (len < 0 || add < 0 || (long long)len + add > most) ok = false;
                 else want = pages_of(c, len + add) - pages_of(c, len);
             }
             long long total;
             const long long at = block_scan(want, buf, total);
-            if (i < n && ok) sc.offsets[i] = (int)min(need + at, (long long)INT32_MAX);
+            if (i < n) offsets[i] = (int)min(need + at, (long long)INT32_MAX);
             need += total;
         }
         ok = __syncthreads_and(ok);
     }
-    long long before = 0;
-    const long long free_pages = count_pages(c, buf, before, kOutside, is_free);
     if (!ok || need > free_pages) {
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int id = __ldcg(seqs + i);
+            const int id = ids.at(i);
             if (id >= 0 && id < c.max_seqs) c.tail[id] = 0;
         }
         set_result(c, ok ? TPB_ERR_OOM : TPB_ERR_INVALID_ARG, free_pages, 0, ok ? need : 0);
         return;
     }
-    list_pages(c, sc.list_a, before, need, kOutside, is_free);
+    int32_t *list = need <= kSmallList ? small_list : sc.list_a;
+    list_pages(c, refs, list, before, need, is_free);
     __syncthreads();
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < n; i += kWarps) {
-        const int id = __ldcg(seqs + i), len = __ldcg(c.lens + id), add = __ldcg(n_new + i);
-        const int p0 = pages_of(c, len), p1 = pages_of(c, len + add), at = sc.offsets[i];
+        const int id = __ldcg(seqs + i), add = __ldcg(n_new + i), len = __ldcg(c.lens + id);
+        const int p0 = pages_of(c, len), p1 = pages_of(c, len + add), at = offsets[i];
         for (int p = p0 + lane; p < p1; p += 32) {
-            const int page = sc.list_a[at + p - p0];
+            const int page = list[at + p - p0];
             c.table[(size_t)id * c.max_pages + p] = page;
             c.refs[page] = 1;
         }
@@ -198,113 +234,159 @@ kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new
     set_result(c, TPB_OK, free_pages - need, need, need);
 }
 
+// Entries p0 .. p1 of a sequence's row of the table, a lane each, as fn(p, page); an entry that is no page is reported and left out.
+template <typename Fn>
+__device__ __forceinline__ void each_page(const tpb_kv_cache &c, int id, int p0, int p1, uint32_t *status, Fn fn) {
+#pragma unroll 4
+    for (int p = p0 + (int)(threadIdx.x & 31); p < p1; p += 32) {
+        const int page = __ldcg(c.table + (size_t)id * c.max_pages + p);
+        if (page < 0 || page >= c.n_pages) report(status, kBadPage);
+        else fn(p, page);
+    }
+}
+
 __global__ void __launch_bounds__(kThreads)
-kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new_lens, int n) {
+kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new_lens, int n, uint32_t *status) {
     __shared__ long long buf[kWarps];
+    __shared__ uint32_t bits[kMarkBits / 32];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
     const Scratch sc = scratch_of(c);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    bool ok = distinct(c, seqs, n, sc.marks);
-    const auto new_len = [&](int i) { return new_lens ? __ldcg(new_lens + i) : 0; };
-    if (ok) {
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int len = __ldcg(c.lens + __ldcg(seqs + i)), to = new_len(i);
+    const Listed ids(seqs, n), cuts(new_lens, n);
+    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
+    marks.clear(seqs, n, c.max_seqs);
+    __syncthreads();
+    bool ok = true;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int id = ids.at(i);
+        if (id < 0 || id >= c.max_seqs || marks.set(id)) {
+            ok = false;
+        } else {
+            const int len = __ldcg(c.lens + id), to = cuts.at(i);
             if (len < 0 || to < 0 || to > len || (long long)len > (long long)c.max_pages * c.page_tokens) ok = false;
         }
-        for (int i = warp; i < n && ok; i += kWarps) {        // every page that a listed sequence holds is one of the pool's
-            const int id = __ldcg(seqs + i), len = __ldcg(c.lens + id);
-            if (len < 0 || (long long)len > (long long)c.max_pages * c.page_tokens) continue;
-            for (int p = lane; p < pages_of(c, len); p += 32) {
-                const int page = __ldcg(c.table + (size_t)id * c.max_pages + p);
-                if (page < 0 || page >= c.n_pages) ok = false;
-            }
-        }
-        ok = __syncthreads_and(ok);
     }
+    ok = __syncthreads_and(ok);
     long long before = 0;
+    Refs refs;
     if (!ok) {
-        const long long free_pages = count_pages(c, buf, before, kOutside, is_free);
+        load_refs(c, refs);
+        const long long free_pages = count_pages(c, refs, buf, before, is_free);
         if (threadIdx.x == 0) sc.head[0] = 0;
         set_result(c, TPB_ERR_INVALID_ARG, free_pages, 0, 0);
         return;
     }
-    // give back the pages behind the cuts; `by` = 1 takes it back
-    const auto drop = [&](int by) {
+    const auto new_len = [&](int i) { return new_lens ? __ldcg(new_lens + i) : 0; };
+    // give back the pages behind the cuts; `by` = 1 takes it back.  Where nothing can stop the operation any more, the rows are cleared at once.
+    const auto drop = [&](int by, bool clear) {
         for (int i = warp; i < n; i += kWarps) {
             const int id = __ldcg(seqs + i), p1 = pages_of(c, __ldcg(c.lens + id));
-            for (int p = pages_of(c, new_len(i)) + lane; p < p1; p += 32)
-                atomicAdd(c.refs + __ldcg(c.table + (size_t)id * c.max_pages + p), by);
+            each_page(c, id, pages_of(c, new_len(i)), p1, status, [&](int p, int page) {
+                atomicAdd(c.refs + page, by);
+                if (clear) c.table[(size_t)id * c.max_pages + p] = -1;
+            });
+            __syncwarp();
+            if (clear && lane == 0) {
+                c.lens[id] = 0;
+                c.tail[id] = 0;
+            }
         }
         __syncthreads();
     };
-    drop(-1);
+    if (!new_lens) {              // freed: no cut inside a page
+        drop(-1, true);
+        load_refs(c, refs);
+        const long long free_pages = count_pages(c, refs, buf, before, is_free);
+        set_result(c, TPB_OK, free_pages, 0, 0);
+        return;
+    }
+    drop(-1, false);
     // a cut inside a page that somebody else holds too: the sequence gets a page of its own for what it keeps of it
+    load_refs(c, refs);
     long long need = 0;
     for (int i0 = 0; i0 < n; i0 += kThreads) {
         const int i = i0 + threadIdx.x;
         bool cut = false;
         if (i < n) {
-            const int to = new_len(i);
-            if (to % c.page_tokens != 0)
-                cut = __ldcg(c.refs + __ldcg(c.table + (size_t)__ldcg(seqs + i) * c.max_pages + to / c.page_tokens)) > 1;
+            const int to = cuts.at(i);
+            if (to % c.page_tokens != 0) {
+                const int page = __ldcg(c.table + (size_t)ids.at(i) * c.max_pages + to / c.page_tokens);
+                if (page < 0 || page >= c.n_pages) report(status, kBadPage);
+                else cut = __ldcg(c.refs + page) > 1;
+            }
         }
         long long total;
         const long long at = block_scan(cut ? 1 : 0, buf, total);
         if (i < n) sc.offsets[i] = cut ? (int)(need + at) : -1;
         need += total;
     }
-    const long long free_pages = count_pages(c, buf, before, kOutside, is_free);
+    const long long free_pages = count_pages(c, refs, buf, before, is_free);
     if (need > free_pages) {
-        __syncthreads();
-        drop(1);
-        const long long left = count_pages(c, buf, before, kOutside, is_free);
+        drop(1, false);
+        load_refs(c, refs);
+        const long long left = count_pages(c, refs, buf, before, is_free);
         if (threadIdx.x == 0) sc.head[0] = 0;
         set_result(c, TPB_ERR_OOM, left, 0, need);
         return;
     }
-    list_pages(c, sc.list_b, before, need, kOutside, is_free);
+    list_pages(c, refs, sc.list_b, before, need, is_free);
     __syncthreads();
     for (int i = warp; i < n; i += kWarps) {
-        const int id = __ldcg(seqs + i), p0 = pages_of(c, new_len(i)), p1 = pages_of(c, __ldcg(c.lens + id));
+        const int id = __ldcg(seqs + i), to = new_len(i), p0 = pages_of(c, to), p1 = pages_of(c, __ldcg(c.lens + id));
         int32_t *row = c.table + (size_t)id * c.max_pages;
         for (int p = p0 + lane; p < p1; p += 32) row[p] = -1;
         __syncwarp();
         if (lane == 0) {
-            c.lens[id] = new_len(i);
+            c.lens[id] = to;
             c.tail[id] = 0;
             const int at = sc.offsets[i];
             if (at >= 0) {
-                const int from = __ldcg(row + p0 - 1), to = sc.list_b[at];
+                const int from = __ldcg(row + p0 - 1), fresh = sc.list_b[at];
                 sc.list_a[at] = from;
                 atomicAdd(c.refs + from, -1);
-                c.refs[to] = 1;
-                row[p0 - 1] = to;
+                c.refs[fresh] = 1;
+                row[p0 - 1] = fresh;
             }
         }
     }
     if (threadIdx.x == 0) sc.head[0] = (int)need;
     __syncthreads();
     // a shared page of which every holder has taken a copy is free now: count again where pages were copied
-    const long long left = need > 0 ? count_pages(c, buf, before, kOutside, is_free) : free_pages;
+    long long left = free_pages;
+    if (need > 0) {
+        load_refs(c, refs);
+        left = count_pages(c, refs, buf, before, is_free);
+    }
     set_result(c, TPB_OK, left, need, need);
 }
 
 __global__ void __launch_bounds__(kThreads)
-kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int n, int share) {
+kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int n, int share, uint32_t *status) {
     __shared__ long long buf[kWarps];
+    __shared__ uint32_t bits[kMarkBits / 32];
+    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList];
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
     const Scratch sc = scratch_of(c);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Listed srcs(src, n), dsts(dst, n);
+    Refs refs;
+    load_refs(c, refs);
+    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
+    int32_t *offsets = n <= kSmallList ? small_offsets : sc.offsets;
     // sources may repeat, destinations may not, and no sequence is both
+    marks.clear(src, n, c.max_seqs);
+    marks.clear(dst, n, c.max_seqs);
+    __syncthreads();
     bool ok = true;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int id = __ldcg(src + i);
-        if (id < 0 || id >= c.max_seqs) ok = false;
-        else sc.marks[id] = 0;
+        const int from = srcs.at(i), to = dsts.at(i);
+        if (from < 0 || from >= c.max_seqs || to < 0 || to >= c.max_seqs || marks.set(to)) ok = false;
     }
-    ok = __syncthreads_and(ok) && distinct(c, dst, n, sc.marks);
+    long long before = 0;
+    const long long free_pages = count_pages(c, refs, buf, before, is_free);
+    ok = __syncthreads_and(ok);
     long long need = 0;
     if (ok) {
         const long long most = (long long)c.max_pages * c.page_tokens;
@@ -312,55 +394,51 @@ kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int
             const int i = i0 + threadIdx.x;
             int want = 0;
             if (i < n) {
-                const int from = __ldcg(src + i), len = __ldcg(c.lens + from);
-                if (__ldcg(sc.marks + from) != 0 || len < 0 || len > most || __ldcg(c.lens + __ldcg(dst + i)) != 0) ok = false;
+                const int from = srcs.at(i), len = __ldcg(c.lens + from), taken = __ldcg(c.lens + dsts.at(i));
+                if (marks.test(from) || len < 0 || len > most || taken != 0) ok = false;
                 else want = share ? (len % c.page_tokens != 0) : pages_of(c, len);
             }
             long long total;
             const long long at = block_scan(want, buf, total);
-            if (i < n) sc.offsets[i] = (int)min(need + at, (long long)INT32_MAX);
+            if (i < n) offsets[i] = (int)min(need + at, (long long)INT32_MAX);
             need += total;
-        }
-        for (int i = warp; i < n && ok; i += kWarps) {
-            const int id = __ldcg(src + i), len = __ldcg(c.lens + id);
-            if (len < 0 || len > most) continue;
-            for (int p = lane; p < pages_of(c, len); p += 32) {
-                const int page = __ldcg(c.table + (size_t)id * c.max_pages + p);
-                if (page < 0 || page >= c.n_pages) ok = false;
-            }
         }
         ok = __syncthreads_and(ok);
     }
-    long long before = 0;
-    const long long free_pages = count_pages(c, buf, before, kOutside, is_free);
     if (!ok || need > free_pages) {
         if (threadIdx.x == 0) sc.head[0] = 0;
         set_result(c, ok ? TPB_ERR_OOM : TPB_ERR_INVALID_ARG, free_pages, 0, ok ? need : 0);
         return;
     }
-    list_pages(c, sc.list_b, before, need, kOutside, is_free);
+    int32_t *list = need <= kSmallList ? small_list : sc.list_b;
+    list_pages(c, refs, list, before, need, is_free);
+    if (threadIdx.x == 0) sc.head[0] = (int)need;
     __syncthreads();
     for (int i = warp; i < n; i += kWarps) {
-        const int from = __ldcg(src + i), to = __ldcg(dst + i), len = __ldcg(c.lens + from), at = sc.offsets[i];
+        const int from = __ldcg(src + i), to = __ldcg(dst + i), len = __ldcg(c.lens + from), at = offsets[i];
         const int kept = share ? len / c.page_tokens : 0;           // pages that both hold
-        for (int p = lane; p < pages_of(c, len); p += 32) {
-            int page = __ldcg(c.table + (size_t)from * c.max_pages + p);
+        for (int p = kept + lane; p < pages_of(c, len); p += 32) {  // copies: until the source is known to be a page, of the copy itself
+            const int fresh = list[at + p - kept];
+            sc.list_a[at + p - kept] = fresh;
+            sc.list_b[at + p - kept] = fresh;
+            c.refs[fresh] = 1;
+            c.table[(size_t)to * c.max_pages + p] = fresh;
+        }
+        __syncwarp();
+        each_page(c, from, 0, pages_of(c, len), status, [&](int p, int page) {
             if (p < kept) {
                 atomicAdd(c.refs + page, 1);
+                c.table[(size_t)to * c.max_pages + p] = page;
             } else {
                 sc.list_a[at + p - kept] = page;
-                page = sc.list_b[at + p - kept];
-                c.refs[page] = 1;
             }
-            c.table[(size_t)to * c.max_pages + p] = page;
-        }
+        });
         __syncwarp();
         if (lane == 0) {
             c.lens[to] = len;
             c.tail[to] = 0;
         }
     }
-    if (threadIdx.x == 0) sc.head[0] = (int)need;
     set_result(c, TPB_OK, free_pages - need, need, need);
 }
 
@@ -369,18 +447,21 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const tpb_kv_cache
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
     const Scratch sc = scratch_of(c);
-    long long before = 0;
-    const long long live = count_pages(c, buf, before, 0, [](int, int r) { return r > 0; });
-    const auto high = [live](int p, int r) { return r > 0 && p >= live; };
+    Refs refs;
+    load_refs(c, refs);
+    long long before = 0, before_hole = 0;
+    const int n_pages = (int)c.n_pages;
+    const long long live = count_pages(c, refs, buf, before, [n_pages](int p, int r) { return r > 0 && p < n_pages; });
+    const auto high = [live, n_pages](int p, int r) { return r > 0 && p >= live && p < n_pages; };
     const auto hole = [live](int p, int r) { return r <= 0 && p < live; };
-    const long long moved = count_pages(c, buf, before, 0, high);
-    list_pages(c, sc.list_a, before, moved, 0, high);
-    count_pages(c, buf, before, kOutside, hole);                  // as many: `live` places below `live`, and `live` pages
-    list_pages(c, sc.list_b, before, moved, kOutside, hole);
+    const long long moved = count_pages(c, refs, buf, before, high);
+    count_pages(c, refs, buf, before_hole, hole);                 // as many: `live` places below `live`, and `live` pages
+    list_pages(c, refs, sc.list_a, before, moved, high);
+    list_pages(c, refs, sc.list_b, before_hole, moved, hole);
     __syncthreads();
     for (long long i = threadIdx.x; i < moved; i += kThreads) {
         const int from = sc.list_a[i], to = sc.list_b[i];
-        c.refs[to] = c.refs[from];
+        c.refs[to] = __ldcg(c.refs + from);
         c.refs[from] = 0;
     }
     if (threadIdx.x == 0) {
@@ -516,7 +597,7 @@ int tpb_kv_truncate(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, 
     if (rc != TPB_OK) return rc;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
-    TPB_CUDA(h, tpb_launch_pdl(kv_truncate_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, *c, seqs, new_lens, n));
+    TPB_CUDA(h, tpb_launch_pdl(kv_truncate_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, *c, seqs, new_lens, n, h->d_status));
     // sequences that are freed are not cut inside a page: nothing to copy
     if (new_lens)
         TPB_CUDA(h, tpb_launch_pdl(kv_copy_pages_kernel<false>, dim3(copy_blocks(h)), dim3(256), 0, (cudaStream_t)stream, *c));
@@ -529,7 +610,7 @@ int tpb_kv_fork(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, cons
     if (rc != TPB_OK) return rc;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
-    TPB_CUDA(h, tpb_launch_pdl(kv_fork_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, *c, src, dst, n, share));
+    TPB_CUDA(h, tpb_launch_pdl(kv_fork_kernel, dim3(1), dim3(kThreads), 0, (cudaStream_t)stream, *c, src, dst, n, share, h->d_status));
     TPB_CUDA(h, tpb_launch_pdl(kv_copy_pages_kernel<false>, dim3(copy_blocks(h)), dim3(256), 0, (cudaStream_t)stream, *c));
     return TPB_OK;
 }
