@@ -228,14 +228,6 @@ __device__ __forceinline__ uint32_t s8_pair_raw(uint32_t w) {
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(b) : "r"(w), "r"(0x00ff00ffu), "r"(0x00800080u));
     return b;
 }
-// the two e4m3 values of the low or high half of a word -> f16
-template <int HALF>
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
-    uint32_t d;
-    if (HALF == 0) asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(w));
-    else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(w));
-    return d;
-}
 // Four consecutive bytes of K as the two registers of a k step, times kPerUnitOfK: bytes (0, 2), (1, 3) of s8, (0, 1), (2, 3) of e4m3.
 template <int FORMAT>
 __device__ __forceinline__ void k_regs(uint32_t w, uint32_t &b0, uint32_t &b1) {

@@ -2,6 +2,8 @@
 //
 // A block -- the tokens of one page, one head -- has one scale, a power of two, so that the quotients value / scale and old scale / new scale are exact
 // in f32: quantising is one rounding (to int8, or to e4m3), and a block whose scale has to grow is rounded again by a shift.
+#include <algorithm>
+
 #include "kv_common.cuh"
 
 using namespace tpb_kv;
@@ -20,184 +22,224 @@ __device__ __forceinline__ float pow2_scale(float amax) {
     return __uint_as_float((uint32_t)(min(max(e, -100), 127 - p) + 127) << 23);
 }
 
-// One CTA per (sequence, page it touches), head, and keys or values: 128 threads with up to CHUNKS pieces of 16 values each in registers, as
-// they were loaded, between the maximum and the rounding, so that the input is read once.  Bound by HBM for prompts; for a
-// decode step by its chain of loads: offsets and id, length and tail, page and new values, old scale and old values -- what a step of it
-// brings is asked for before anything is decided.
+template <int FORMAT>
+constexpr float kLimit = FORMAT == TPB_KV_S8 ? 127.0f : 448.0f;
+
+// One CTA per (sequence, page it touches) and some of the page's blocks (a head's keys or values): a group of 128 threads takes a block at a time, with up
+// to CHUNKS pieces of 16 values a thread in registers, as they were loaded, between the maximum and the rounding, so that the input is read
+// once.  Bound by HBM for prompts; for a decode step by its chain of loads -- offsets and id, length and tail, page, new values and old ones, 0.4 us
+// each -- which is why one warp a CTA looks the sequence up, why a CTA of a prompt goes over several blocks behind one look-up, and why
+// what a step of the chain brings is asked for before anything is decided.
 //
 // Grid x: sequence i has at least as many places as it can touch pages from cu[i] / page_tokens + 2 i on, so that a CTA finds its
 // sequence by a search and the launch needs no lengths on the host.
+template <int CHUNKS>
+constexpr int kAppendGroups = CHUNKS <= 1 ? 8 : CHUNKS == 2 ? 4 : 2;
 template <typename T, int FORMAT, int HD, int CHUNKS>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128 * kAppendGroups<CHUNKS>)
 kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, const T *v, int64_t ld_v, const int32_t *seqs, const int32_t *cu,
                  int n_seqs, int rows, uint32_t *status) {
-    __shared__ float s_max[4];
-    __shared__ int s_bad[4];
+    constexpr int GROUPS = kAppendGroups<CHUNKS>;
+    __shared__ float s_max[2][4 * GROUPS];
+    __shared__ int s_found[5];              // i, cu[i], new tokens, id, length; length -1: nothing to do
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    const int pt = c.page_tokens, shift = __ffs(pt) - 1, x = (int)blockIdx.x, head = (int)blockIdx.y, t = (int)threadIdx.x;
-    const bool is_v = blockIdx.z != 0;
-    const Found b = find_sequence(cu, seqs, n_seqs, rows, x, [&](int j, int r) { return (r >> shift) + 2 * j; });
-    const int n_new = b.r1 - b.r0;
-    if (n_new <= 0) return;
-    if (b.seq < 0 || b.seq >= c.max_seqs) {
-        report(status, kBadSeq);
-        return;
+    const int pt = c.page_tokens, shift = __ffs(pt) - 1, x = (int)blockIdx.x, t = (int)threadIdx.x & 127, group = (int)threadIdx.x >> 7;
+    if (threadIdx.x < 32) {
+        const Found b = find_sequence(cu, seqs, n_seqs, rows, x, [&](int j, int r) { return (r >> shift) + 2 * j; });
+        const int n_new = b.r1 - b.r0;
+        int len = -1;
+        if (n_new > 0) {
+            if (b.seq < 0 || b.seq >= c.max_seqs) {
+                report(status, kBadSeq);
+            } else {
+                len = __ldcg(c.lens + b.seq);
+                const int tail = __ldcg(c.tail + b.seq);
+                if (len < n_new || (long long)len > (long long)c.max_pages * pt) {
+                    report(status, kBadLen);
+                    len = -1;
+                } else if (tail != n_new) {
+                    report(status, kBadTail);
+                    len = -1;
+                }
+            }
+        }
+        if (threadIdx.x == 0) {
+            s_found[0] = b.i;
+            s_found[1] = b.r0;
+            s_found[2] = n_new;
+            s_found[3] = b.seq;
+            s_found[4] = len;
+        }
     }
-    const int len = __ldcg(c.lens + b.seq), tail = __ldcg(c.tail + b.seq);
-    if (len < n_new || (long long)len > (long long)c.max_pages * pt) {
-        report(status, kBadLen);
-        return;
-    }
-    if (tail != n_new) {
-        report(status, kBadTail);
-        return;
-    }
+    __syncthreads();
+    const int r0 = s_found[1], n_new = s_found[2], seq = s_found[3], len = s_found[4];
+    if (len < 0) return;
     const int first = len - n_new;
-    const long long pg = (long long)(first >> shift) + (x - ((b.r0 >> shift) + 2 * b.i));
+    const long long pg = (long long)(first >> shift) + (x - ((r0 >> shift) + 2 * s_found[0]));
     if (pg * pt >= len) return;
-    const int page = __ldcg(c.table + (size_t)b.seq * c.max_pages + pg);
+    const int page = __ldcg(c.table + (size_t)seq * c.max_pages + pg);
     const int p0 = (int)pg * pt;                                // position of the page's first slot
     const int held = max(first - p0, 0), fill = min(len - p0, pt);   // slots [0, held) hold earlier tokens, [held, fill) are written
-    const int64_t ld = is_v ? ld_v : ld_k;
-    const T *src = (is_v ? v : k) + (int64_t)(b.r0 + p0 - first) * ld + (int64_t)head * HD;   // + slot * ld
-    Raw16<T> raw[CHUNKS];
+    const int blocks = 2 * c.kv_heads, stride = (int)gridDim.y * (int)(blockDim.x >> 7);
+    int flip = 0;
+    for (int b0 = (int)blockIdx.y * (int)(blockDim.x >> 7); b0 < blocks; b0 += stride, flip ^= 1) {
+        const int bi = b0 + group;
+        const bool there = bi < blocks, is_v = bi >= c.kv_heads;
+        const int head = there ? (is_v ? bi - c.kv_heads : bi) : 0;
+        const int64_t ld = is_v ? ld_v : ld_k;
+        const T *src = (is_v ? v : k) + (int64_t)(r0 + p0 - first) * ld + (int64_t)head * HD;   // + slot * ld
+        Raw16<T> raw[CHUNKS];
 #pragma unroll
-    for (int j = 0; j < CHUNKS; j++) {
-        const int slot = (j * 128 + t) / (HD / 16), d = (j * 128 + t) % (HD / 16) * 16;
-        if (slot >= held && slot < fill) load_raw(src + (int64_t)slot * ld + d, raw[j]);
-    }
-    if (page < 0 || page >= c.n_pages) {
-        report(status, kBadPage);
-        return;
-    }
-    const size_t block = ((size_t)layer * c.n_pages + page) * c.kv_heads + head;
-    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(is_v ? c.v : c.k) + block * (size_t)(pt * HD));
-    float *scale_at = (is_v ? c.v_scale : c.k_scale) + block;
-    const float old = held > 0 ? __ldcg(scale_at) : 0.0f;
-    uint4 before[CHUNKS];
-#pragma unroll
-    for (int j = 0; j < CHUNKS; j++)
-        if ((j * 128 + t) / (HD / 16) < held) before[j] = __ldcg(dst + j * 128 + t);
-    float amax = 0.0f;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < CHUNKS; j++) {
-        const int slot = (j * 128 + t) / (HD / 16);
-        if (slot >= held && slot < fill) {
-            float f[16];
-            values_of(raw[j], f);
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                amax = fmaxf(amax, fabsf(f[e]));
-                bad |= !(fabsf(f[e]) <= 3.402823466e38f);
-            }
+        for (int j = 0; j < CHUNKS; j++) {
+            const int slot = (j * 128 + t) / (HD / 16), d = (j * 128 + t) % (HD / 16) * 16;
+            if (there && slot >= held && slot < fill) load_raw(src + (int64_t)slot * ld + d, raw[j]);
         }
-    }
-    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));       // non-negative floats order like their bits
-    bad = __any_sync(0xffffffffu, bad);
-    if ((t & 31) == 0) {
-        s_max[t >> 5] = amax;
-        s_bad[t >> 5] = bad;
-    }
-    __syncthreads();                                            // also: everybody has the old scale before it is replaced
-    amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] | !(old >= 0.0f && old <= 3.402823466e38f);
-    const float scale = bad ? __uint_as_float(0x7fc00000u) : fmaxf(old, pow2_scale<FORMAT>(amax));
-    if (t == 0) *scale_at = scale;
-    // the quotient by a power of two is the product with its inverse; an old scale of the caller's own need not be one
-    const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
-    const float inv = pow2 ? 1.0f / scale : 0.0f, ratio = old / scale;
-#pragma unroll
-    for (int j = 0; j < CHUNKS; j++) {
-        const int slot = (j * 128 + t) / (HD / 16);
-        if (slot < held) {
-            if (scale == old || bad) continue;
-            uint32_t u[4] = {before[j].x, before[j].y, before[j].z, before[j].w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float f[4];
-                unpack4<FORMAT>(u[e], f);
-#pragma unroll
-                for (int q = 0; q < 4; q++) f[q] *= ratio;
-                u[e] = pack4<FORMAT>(f);
-            }
-            dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
-        } else if (slot < fill) {
-            uint32_t u[4] = {0u, 0u, 0u, 0u};
-            if (!bad) {
-                float f[16];
-                values_of(raw[j], f);
-#pragma unroll
-                for (int e = 0; e < 16; e++) f[e] = pow2 ? f[e] * inv : f[e] / scale;
-#pragma unroll
-                for (int e = 0; e < 4; e++) u[e] = pack4<FORMAT>(&f[4 * e]);
-            }
-            dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-    }
-}
-
-// A warp per row: finds its sequence and page, then 16 values a lane and step, keys and values, four steps' loads in flight.
-template <typename T, int FORMAT, int HD>
-__global__ void __launch_bounds__(256)
-kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_t ld_v, const int32_t *seqs, const int32_t *start,
-               const int32_t *cu, int n_seqs, int rows, uint32_t *status) {
-    tpb_grid_dep_launch();
-    tpb_grid_dep_wait();
-    const int lane = threadIdx.x & 31;
-    const int r = (int)(blockIdx.x * 8 + (threadIdx.x >> 5));
-    if (r >= rows) return;
-    const Found b = find_sequence(cu, seqs, n_seqs, rows, r, [&](int, int r0) { return r0; });
-    if (r < b.r0 || r >= b.r1) return;          // a row of no sequence
-    if (b.seq < 0 || b.seq >= c.max_seqs) {
-        report(status, kBadSeq);
-        return;
-    }
-    const int from = start ? __ldcg(start + b.i) : 0, len = __ldcg(c.lens + b.seq), shift = __ffs(c.page_tokens) - 1;
-    const long long pos = (long long)from + (r - b.r0);
-    const bool inside = from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens;
-    int page = 0, slot = 0;
-    if (inside) {
-        page = __ldcg(c.table + (size_t)b.seq * c.max_pages + (pos >> shift));
-        slot = (int)(pos & (c.page_tokens - 1));
         if (page < 0 || page >= c.n_pages) {
             report(status, kBadPage);
             return;
         }
+        const size_t block = ((size_t)layer * c.n_pages + page) * c.kv_heads + head;
+        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(is_v ? c.v : c.k) + block * (size_t)(pt * HD));
+        float *scale_at = (is_v ? c.v_scale : c.k_scale) + block;
+        const float old = there && held > 0 ? __ldcg(scale_at) : 0.0f;
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < CHUNKS; j++) {
+            const int slot = (j * 128 + t) / (HD / 16);
+            if (there && slot >= held && slot < fill) asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(amax_of(raw[j])));
+        }
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));       // non-negative floats order like their bits, NaN last
+        if ((t & 31) == 0) s_max[flip][threadIdx.x >> 5] = amax;
+        __syncthreads();                                        // also: everybody has the old scale before it is replaced
+        if (!there) continue;
+        const uint32_t *m = reinterpret_cast<const uint32_t *>(&s_max[flip][4 * group]);
+        amax = __uint_as_float(max(max(m[0], m[1]), max(m[2], m[3])));
+        const bool bad = !(amax <= 3.402823466e38f && old >= 0.0f && old <= 3.402823466e38f);
+        const float scale = bad ? __uint_as_float(0x7fc00000u) : fmaxf(old, pow2_scale<FORMAT>(amax));
+        if (t == 0) *scale_at = scale;
+        // the quotient by a power of two is the product with its inverse; an old scale of the caller's own need not be one
+        const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
+        const float inv = pow2 ? 1.0f / scale : 0.0f, ratio = old / scale;
+        const bool over = amax > kLimit<FORMAT> * scale;        // the largest f32 values saturate
+#pragma unroll
+        for (int j = 0; j < CHUNKS; j++) {
+            const int slot = (j * 128 + t) / (HD / 16);
+            if (slot < held) {
+                if (scale == old || bad) continue;
+                const uint4 before = __ldcg(dst + j * 128 + t);
+                uint32_t u[4] = {before.x, before.y, before.z, before.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float f[4];
+                    unpack4<FORMAT>(u[e], f);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) f[q] *= ratio;
+                    u[e] = pack4<FORMAT>(f);
+                }
+                dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
+            } else if (slot < fill) {
+                uint32_t u[4] = {0u, 0u, 0u, 0u};
+                if (!bad) {
+                    float f[16];
+                    values_of(raw[j], f);
+                    if (pow2) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) f[e] *= inv;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) f[e] = __fdiv_rn(f[e], scale);
+                    }
+                    if (over) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) f[e] = fminf(fmaxf(f[e], -kLimit<FORMAT>), kLimit<FORMAT>);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) u[e] = pack4<FORMAT>(&f[4 * e]);
+                }
+                dst[j * 128 + t] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
     }
-    const size_t block0 = ((size_t)layer * c.n_pages + page) * c.kv_heads;
+}
+
+// A warp has `per_warp` consecutive rows: looks up the sequence of the first, asks for the pages of all, and then goes over them with 16 values a lane and
+// step, keys and values, four steps' loads in flight.  More rows a warp spare the look-ups (8500 rows at one a warp: 8500 warps in line at the same few
+// words of L2), fewer keep more of them under way.
+template <typename T, int FORMAT, int HD>
+__global__ void __launch_bounds__(256)
+kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_t ld_v, const int32_t *seqs, const int32_t *start,
+               const int32_t *cu, int n_seqs, int rows, int per_warp, uint32_t *status) {
+    tpb_grid_dep_launch();
+    tpb_grid_dep_wait();
+    const int lane = threadIdx.x & 31, shift = __ffs(c.page_tokens) - 1;
+    const int first = ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) * per_warp, end = min(first + per_warp, rows);
     const int pieces = c.kv_heads * (HD / 16);
-    constexpr int kAhead = 4;
-    for (int p0 = lane; p0 < 2 * pieces; p0 += 32 * kAhead) {
-        uint4 w[kAhead];
-        float scale[kAhead];
-#pragma unroll
-        for (int e = 0; e < kAhead; e++) {
-            const int p = p0 + 32 * e;
-            if (inside && p < 2 * pieces) {
-                const bool is_v = p >= pieces;
-                const int q = is_v ? p - pieces : p, head = q / (HD / 16), d = q % (HD / 16) * 16;
-                scale[e] = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
-                w[e] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(is_v ? c.v : c.k) + ((block0 + head) * c.page_tokens + slot) * HD + d));
+    for (int r = first; r < end;) {
+        const Found b = find_sequence(cu, seqs, n_seqs, rows, r, [&](int, int r0) { return r0; });
+        const int stop = b.r0 > r ? min(b.r0, end) : b.r1 > r ? min(b.r1, end) : end;     // rows r .. stop - 1 share the answer
+        if (b.r0 > r || b.r1 <= r) {                                                     // rows of no sequence
+            r = stop;
+            continue;
+        }
+        if (b.seq < 0 || b.seq >= c.max_seqs) {
+            report(status, kBadSeq);
+            r = stop;
+            continue;
+        }
+        const int from = start ? __ldcg(start + b.i) : 0, len = __ldcg(c.lens + b.seq);
+        // the pages of the rows, a lane a row: -1 = behind the end (zeros), -2 = not a page (left as it is)
+        int page_of_lane = -1;
+        if (r + lane < stop) {
+            const long long pos = (long long)from + (r + lane - b.r0);
+            if (from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens) {
+                page_of_lane = __ldcg(c.table + (size_t)b.seq * c.max_pages + (pos >> shift));
+                if (page_of_lane < 0 || page_of_lane >= c.n_pages) {
+                    report(status, kBadPage);
+                    page_of_lane = -2;
+                }
             }
         }
+        for (int e = r; e < stop; e++) {
+            const int page = __shfl_sync(0xffffffffu, page_of_lane, e - r);
+            if (page == -2) continue;
+            const bool inside = page >= 0;
+            const int slot = (from + (e - b.r0)) & (c.page_tokens - 1);
+            const size_t block0 = ((size_t)layer * c.n_pages + max(page, 0)) * c.kv_heads;
+            constexpr int kAhead = 4;
+            for (int p0 = lane; p0 < 2 * pieces; p0 += 32 * kAhead) {
+                uint4 w[kAhead];
+                float scale[kAhead];
 #pragma unroll
-        for (int e = 0; e < kAhead; e++) {
-            const int p = p0 + 32 * e;
-            if (p >= 2 * pieces) break;
-            const bool is_v = p >= pieces;
-            const int q = is_v ? p - pieces : p;
-            float f[16] = {};
-            if (inside) {
-                const uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+                for (int a = 0; a < kAhead; a++) {
+                    const int p = p0 + 32 * a;
+                    if (inside && p < 2 * pieces) {
+                        const bool is_v = p >= pieces;
+                        const int q = is_v ? p - pieces : p, head = q / (HD / 16), d = q % (HD / 16) * 16;
+                        scale[a] = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
+                        w[a] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(is_v ? c.v : c.k) +
+                                                                      ((block0 + head) * c.page_tokens + slot) * HD + d));
+                    }
+                }
 #pragma unroll
-                for (int i = 0; i < 4; i++) unpack4<FORMAT>(u[i], &f[4 * i]);
+                for (int a = 0; a < kAhead; a++) {
+                    const int p = p0 + 32 * a;
+                    if (p >= 2 * pieces) break;
+                    const bool is_v = p >= pieces;
+                    const int q = is_v ? p - pieces : p;
+                    float f[16] = {};
+                    if (inside) {
+                        const uint32_t u[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
 #pragma unroll
-                for (int i = 0; i < 16; i++) f[i] *= scale[e];
+                        for (int i = 0; i < 4; i++) unpack4<FORMAT>(u[i], &f[4 * i]);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) f[i] *= scale[a];
+                    }
+                    store16((is_v ? v + (int64_t)e * ld_v : k + (int64_t)e * ld_k) + (int64_t)q * 16, f);
+                }
             }
-            store16((is_v ? v + (int64_t)r * ld_v : k + (int64_t)r * ld_k) + (int64_t)q * 16, f);
         }
+        r = stop;
     }
 }
 
@@ -233,22 +275,25 @@ int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, in
     if (rc != TPB_OK || n_seqs == 0 || rows == 0) return rc;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
-    const dim3 grid((unsigned)(rows / c->page_tokens + 2 * (int64_t)n_seqs), (unsigned)c->kv_heads, 2u);
     const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        const auto launch = [&](auto kern) {
-            return tpb_launch_pdl(kern, grid, dim3(128), 0, (cudaStream_t)stream, *c, layer, (const T *)k, ld_k, (const T *)v, ld_v, seqs, cu, n_seqs,
-                                  (int)rows, h->d_status);
+        const auto launch = [&](auto kern, int groups) {
+            // as many CTAs a page as two rounds of two an SM have room for: with more, each waits through a look-up of its own
+            const int64_t items = rows / c->page_tokens + 2 * (int64_t)n_seqs;
+            const int rounds = (2 * c->kv_heads + groups - 1) / groups;
+            const int64_t y = std::max<int64_t>(1, std::min<int64_t>(rounds, 4 * (int64_t)h->sm_count / items));
+            return tpb_launch_pdl(kern, dim3((unsigned)items, (unsigned)y), dim3(128u * (unsigned)groups), 0, (cudaStream_t)stream, *c, layer, (const T *)k,
+                                  ld_k, (const T *)v, ld_v, seqs, cu, n_seqs, (int)rows, h->d_status);
         };
-        const int chunks = c->page_tokens * c->head_dim / 2048;             // 0 (half the threads have a piece) .. 4
-        if (c->format == TPB_KV_S8) {
-            if (c->head_dim == 64) return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_S8, 64, 1>) : launch(kv_append_kernel<T, TPB_KV_S8, 64, 2>);
-            return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_S8, 128, 1>)
-                               : chunks <= 2 ? launch(kv_append_kernel<T, TPB_KV_S8, 128, 2>) : launch(kv_append_kernel<T, TPB_KV_S8, 128, 4>);
-        }
-        if (c->head_dim == 64) return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 64, 1>) : launch(kv_append_kernel<T, TPB_KV_E4M3, 64, 2>);
-        return chunks <= 1 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 1>)
-                           : chunks <= 2 ? launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 2>) : launch(kv_append_kernel<T, TPB_KV_E4M3, 128, 4>);
+        const auto by_chunks = [&](auto fmt) {
+            constexpr int F = decltype(fmt)::value;
+            const int chunks = c->page_tokens * c->head_dim / 2048;             // 0 (half the threads have a piece) .. 4
+            if (c->head_dim == 64)
+                return chunks <= 1 ? launch(kv_append_kernel<T, F, 64, 1>, kAppendGroups<1>) : launch(kv_append_kernel<T, F, 64, 2>, kAppendGroups<2>);
+            return chunks <= 1 ? launch(kv_append_kernel<T, F, 128, 1>, kAppendGroups<1>)
+                               : chunks <= 2 ? launch(kv_append_kernel<T, F, 128, 2>, kAppendGroups<2>) : launch(kv_append_kernel<T, F, 128, 4>, kAppendGroups<4>);
+        };
+        return c->format == TPB_KV_S8 ? by_chunks(std::integral_constant<int, TPB_KV_S8>{}) : by_chunks(std::integral_constant<int, TPB_KV_E4M3>{});
     });
     TPB_CUDA(h, e);
     return TPB_OK;
@@ -266,8 +311,9 @@ int tpb_kv_read(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int 
     const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         const auto launch = [&](auto kern) {
-            return tpb_launch_pdl(kern, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, *c, layer, (T *)k, ld_k, (T *)v, ld_v, seqs,
-                                  start, cu, n_seqs, (int)rows, h->d_status);
+            const int per_warp = rows > 32 * (int64_t)h->sm_count ? 2 : 1;
+            return tpb_launch_pdl(kern, dim3((unsigned)((rows + 8 * per_warp - 1) / (8 * per_warp))), dim3(256), 0, (cudaStream_t)stream, *c, layer, (T *)k, ld_k,
+                                  (T *)v, ld_v, seqs, start, cu, n_seqs, (int)rows, per_warp, h->d_status);
         };
         if (c->format == TPB_KV_S8) return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_S8, 64>) : launch(kv_read_kernel<T, TPB_KV_S8, 128>);
         return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_E4M3, 64>) : launch(kv_read_kernel<T, TPB_KV_E4M3, 128>);

@@ -3,7 +3,6 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include <cstdint>
 #include <type_traits>
@@ -133,34 +132,80 @@ __device__ __forceinline__ void store16(T *p, const float (&v)[16]) {
     }
 }
 
-// One 32-bit word of four cached values.
+// The largest magnitude among sixteen values; NaN if one of them is.
+template <typename T>
+__device__ __forceinline__ float amax_of(const Raw16<T> &r) {
+    if constexpr (sizeof(T) == 4) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(__uint_as_float(w[e]))));
+        }
+        return m;
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[e] & 0x7fff7fffu));
+                else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[e] & 0x7fff7fffu));
+            }
+        }
+        float lo, hi, f;
+        if constexpr (std::is_same<T, __half>::value) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&m));
+            lo = x.x; hi = x.y;
+        } else {
+            lo = __uint_as_float(m << 16); hi = __uint_as_float(m & 0xffff0000u);
+        }
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(f) : "f"(lo), "f"(hi));
+        return f;
+    }
+}
+
+// the two e4m3 values of the low or high half of a word -> f16
+template <int HALF>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+    uint32_t d;
+    if (HALF == 0) asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(w));
+    else asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(w));
+    return d;
+}
+// One 32-bit word of four cached values.  int8: 2^23 + 128 + x has x ^ 0x80 in its lowest byte.
 template <int FORMAT>
 __device__ __forceinline__ void unpack4(uint32_t w, float *v) {
     if constexpr (FORMAT == TPB_KV_S8) {
+        const uint32_t u = w ^ 0x80808080u;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (float)(int8_t)(w >> (8 * i));
+        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | i)) - 8388736.0f;
     } else {
+        const uint32_t h[2] = {e4m3_pair<0>(w), e4m3_pair<1>(w)};
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
-            const float2 f = __half22float2(__half2(h));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
             v[2 * i] = f.x; v[2 * i + 1] = f.y;
         }
     }
 }
-// Four quotients (value / scale) rounded to nearest even, saturated at the format's limit.
+// Four quotients (value / scale) rounded to nearest even; at most the format's limit (e4m3 saturates there).  int8: adding 1.5 * 2^23
+// rounds to a whole number, whose low byte the sum's low byte is.
 template <int FORMAT>
 __device__ __forceinline__ uint32_t pack4(const float *v) {
-    uint32_t w = 0;
     if constexpr (FORMAT == TPB_KV_S8) {
+        uint32_t m[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w |= ((uint32_t)max(-127, min(127, __float2int_rn(v[i]))) & 0xffu) << (8 * i);
+        for (int i = 0; i < 4; i++) m[i] = __float_as_uint(v[i] + 12582912.0f);
+        return __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
     } else {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            w |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3) << (16 * i);
+        uint32_t d;
+        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+            : "=r"(d) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+        return d;
     }
-    return w;
 }
 #endif
 

@@ -27,12 +27,15 @@ __device__ __forceinline__ long long block_scan(long long v, long long *buf, lon
     __syncthreads();
     if (lane == 31) buf[warp] = inc;
     __syncthreads();
-    long long base = 0;
-    total = 0;
-    for (int w = 0; w < kWarps; w++) {
-        if (w < warp) base += buf[w];
-        total += buf[w];
+    long long sums = buf[lane];                 // every warp scans the warps' sums: a loop over them costs each caller 0.5 us
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, sums, o);
+        if (lane >= o) sums += t;
     }
+    total = __shfl_sync(0xffffffffu, sums, 31);
+    const long long up_to = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
+    const long long base = warp > 0 ? up_to : 0;
     return base + inc - v;
 }
 
@@ -479,8 +482,11 @@ template <bool COMPACT>
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const tpb_kv_cache c) {
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
+    __shared__ int s_head[2];
     const Scratch sc = scratch_of(c);
-    const int count = __ldcg(sc.head);
+    if (threadIdx.x < 2) s_head[threadIdx.x] = __ldcg(sc.head + threadIdx.x);        // once a CTA: thousands of warps at one word wait in line
+    __syncthreads();
+    const int count = s_head[0];
     if (count <= 0) return;
     const int lane = threadIdx.x & 31;
     const long long page_bytes = (long long)c.kv_heads * c.page_tokens * c.head_dim;
@@ -512,7 +518,7 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const tpb_kv_cache c
         }
     }
     if (COMPACT) {
-        const int live = __ldcg(sc.head + 1);
+        const int live = s_head[1];
         const long long entries = (long long)c.max_seqs * c.max_pages, threads = (long long)gridDim.x * blockDim.x;
         for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < entries; e += threads) {
             const int page = __ldcg(c.table + e);
