@@ -528,7 +528,9 @@ int tpb_kv_compact(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c);
  *          q and the probabilities are split in two f16 terms; bf16 rows: one f16 term each (q's is exact).  The cache's values are exact; an
  *          e4m3 byte that a row of the batch sees must not be NaN (append writes none).
  *          max_len: an upper bound of the lengths that the host knows (0 = none): a hint that saves a launch for short sequences.
- *          workspace: tpb_kv_attention_workspace_bytes(h, head_dim) bytes, 16-byte aligned, of this call alone while it runs. */
+ *          workspace: tpb_kv_attention_workspace_bytes(h, head_dim) bytes, 16-byte aligned, of this call alone while it runs; with
+ *          0 < max_len <= TPB_KV_SHORT none is used (it may be NULL). */
+#define TPB_KV_SHORT 256
 int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, const void *k, int64_t ld_k, const void *v,
                   int64_t ld_v, int dtype, const int32_t *seqs, const int32_t *cu, int n_seqs, int64_t rows);
 int tpb_kv_read(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int layer, void *k, int64_t ld_k, void *v, int64_t ld_v,

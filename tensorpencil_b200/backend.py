@@ -301,33 +301,39 @@ class Backend:
         device).  q [tokens][heads*hd], k / v [tokens][kv_heads*hd], all bf16 or all f16, contiguous within a row (parts of a fused
         projection's output may be passed as they are); head_dim 64 or 128.  The result has q's type; rows in no sequence are not
         written."""
-        tokens = q.shape[0]
-        if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        dtype, tokens, index = q.dtype, q.shape[0], self._index
+        if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
             raise TypeError("attentionPacked: q, k and v must all be bfloat16 or all float16")
-        if cu.dtype != torch.int32:
+        if cu.dtype is not torch.int32:
             raise TypeError(f"attentionPacked: cu must be int32 (got {cu.dtype})")
-        if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous() or cu.device != self.device:
+        if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous() or cu.get_device() != index:
             raise ValueError(f"attentionPacked: cu must be a contiguous vector on {self.device}")
-        if out is None:
-            out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
-        elif out.dtype != q.dtype:
+        if out is not None and out.dtype is not dtype:
             raise TypeError("attentionPacked: the output must have q's dtype")
-        ld = []
-        for name, t, h in (("q", q, heads), ("k", k, kv_heads), ("v", v, kv_heads), ("out", out, heads)):
-            s = t.shape
-            if t.device != self.device or s[0] != tokens or not (
-                    (len(s) == 2 and s[1] == h * head_dim and t.stride(1) == 1) or
-                    (len(s) == 3 and s[1] == h and s[2] == head_dim and t.stride(2) == 1 and (t.stride(1) == head_dim or h == 1))):
-                raise ValueError(f"attentionPacked: {name} must be [{tokens}][{h * head_dim}] on {self.device}, contiguous within a row "
-                                 f"(got {tuple(s)}, strides {t.stride()})")
-            ld.append(max(t.stride(0), h * head_dim) if tokens <= 1 else t.stride(0))
-        rc = self._attn_calls.tpb_attention_packed(self._hv, self._stream(), out.data_ptr(), ld[3], q.data_ptr(), ld[0], k.data_ptr(), ld[1],
-                                              v.data_ptr(), ld[2], _TORCH_TO_TPB[q.dtype], cu.data_ptr(), cu.shape[0] - 1, tokens, heads,
-                                              kv_heads, head_dim, float(scale) if scale is not None else head_dim ** -0.5)
+        ld_q, ld_k = self._packed_ld("q", q, tokens, heads, head_dim), self._packed_ld("k", k, tokens, kv_heads, head_dim)
+        ld_v = self._packed_ld("v", v, tokens, kv_heads, head_dim)
+        if out is None:
+            out = q.new_empty((tokens, heads * head_dim))
+            ld_out = heads * head_dim
+        else:
+            ld_out = self._packed_ld("out", out, tokens, heads, head_dim)
+        rc = self._attn_calls.tpb_attention_packed(self._hv, self._stream(), out.data_ptr(), ld_out, q.data_ptr(), ld_q, k.data_ptr(), ld_k,
+                                                   v.data_ptr(), ld_v, _TORCH_TO_TPB[dtype], cu.data_ptr(), cu.shape[0] - 1, tokens, heads,
+                                                   kv_heads, head_dim, float(scale) if scale is not None else head_dim ** -0.5)
         if rc != TPB_OK:
             self._check(rc)
         self.launches += 1
         return out
+
+    def _packed_ld(self, name: str, t: torch.Tensor, tokens: int, heads: int, head_dim: int) -> int:
+        """Elements from one row to the next of [tokens][heads * head_dim] or [tokens][heads][head_dim]; columns are contiguous."""
+        s, st, width = t.shape, t.stride(), heads * head_dim
+        flat = len(s) == 2 and s[1] == width and st[1] == 1
+        if not ((flat or (len(s) == 3 and s[1] == heads and s[2] == head_dim and st[2] == 1 and (st[1] == head_dim or heads == 1)))
+                and s[0] == tokens and t.get_device() == self._index):
+            raise ValueError(f"attentionPacked: {name} must be [{tokens}][{width}] on {self.device}, contiguous within a row "
+                             f"(got {tuple(s)}, strides {st})")
+        return st[0] if tokens > 1 else max(st[0], width)
 
     def _gemm(self, y: torch.Tensor, w_bytes: np.ndarray, weight_scale: np.ndarray, rows: int,
               w_bits: int, ldy: Optional[int] = None):

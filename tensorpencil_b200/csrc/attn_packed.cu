@@ -175,7 +175,6 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const auto o_done = [&](int x) { return bars + 8u * (18 + x); };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBar + 192);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + L::kBar + 200);
-    volatile int *any_bad = reinterpret_cast<volatile int *>(gen + L::kBar + 204);
     int *bad = reinterpret_cast<int *>(gen + L::kBad);
 
     const int warp = threadIdx.x >> 5;
@@ -214,7 +213,6 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             mbar_init(o_done(s), 1);
         }
         *abort_flag = 0;
-        *any_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     for (int i = threadIdx.x; i < 3 * HD; i += kThreads) bad[i] = INT_MAX;
@@ -323,7 +321,10 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 tc_fence_after();
                 const float inv_l = 1.0f / l_run;
                 T *dst = static_cast<T *>(p.out) + (long long)(start + pos) * p.ld_out + (long long)(head * p.group + hq) * HD;
-                const bool fix = *any_bad != 0;
+                // Did V have a NaN or an infinity where somebody does not look?  (Every lane asks for every 32nd column.)
+                bool fix = false;
+                for (int i = lane; i < 3 * HD; i += 32) fix |= bad[i] != INT_MAX;
+                fix = __any_sync(0xffffffffu, fix);
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t v[32];
@@ -476,7 +477,6 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                                     if (key < len) {
                                         const int kind = (h & ~(ex | 0x8000u) & 0xffffu) != 0 ? 0 : (h & 0x8000u) ? 2 : 1;
                                         atomicMin(bad + kind * HD + col0 + e, key);
-                                        *any_bad = 1;
                                     }
                                     u[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
                                 }

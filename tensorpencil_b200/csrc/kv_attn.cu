@@ -32,7 +32,7 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kPiece = 16;           // tokens with one page and scale
-constexpr int kMinTokens = 256;      // a CTA takes at least so many: shorter runs cost more in joining than they gain
+constexpr int kMinTokens = TPB_KV_SHORT;      // a CTA takes at least so many: shorter runs cost more in joining than they gain
 constexpr int kRing = 16384;         // bytes of a warp's ring
 constexpr float kLazy = 6.0f, kUp = 6.0f;      // w < 2^(kLazy + kUp + 1) fits f16
 
@@ -961,13 +961,14 @@ int tpb_kv_attention(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c,
     TPB_CHECK_ARG(h, rows * (heads / c->kv_heads) < ((int64_t)1 << 30), "kv_attention: rows * heads / kv_heads must be below 2^30");
     TPB_CHECK_ARG(h, scale >= 0.0f && scale <= 3.4e38f, "kv_attention: scale must be finite and not negative");
     if (n_seqs == 0 || rows == 0) return TPB_OK;
-    TPB_CHECK_ARG(h, out && q && seqs && cu && workspace, "kv_attention: null pointer");
+    const bool whole = max_len > 0 && max_len <= kMinTokens;
+    TPB_CHECK_ARG(h, out && q && seqs && cu && (workspace || whole), "kv_attention: null pointer");
     const int64_t width = (int64_t)heads * c->head_dim, mult = dtype == TPB_F32 ? 4 : 8;
     TPB_CHECK_ARG(h, ld_q >= width && ld_out >= width && ld_q % mult == 0 && ld_out % mult == 0,
                   "kv_attention: ld_q and ld_out must be at least heads * head_dim and multiples of %lld", (long long)mult);
     TPB_CHECK_ARG(h, tpb_aligned16(out) && tpb_aligned16(q) && tpb_aligned16(workspace), "kv_attention: out, q and workspace must be 16-byte aligned");
     TPB_CHECK_ARG(h, ((reinterpret_cast<uintptr_t>(seqs) | reinterpret_cast<uintptr_t>(cu)) & 3u) == 0, "kv_attention: seqs and cu must be 4-byte aligned");
-    TPB_CHECK_ARG(h, workspace_bytes >= tpb_kv_attention_workspace_bytes(h, c->head_dim), "kv_attention: the workspace holds %zu bytes, %zu are needed",
+    TPB_CHECK_ARG(h, whole || workspace_bytes >= tpb_kv_attention_workspace_bytes(h, c->head_dim), "kv_attention: the workspace holds %zu bytes, %zu are needed",
                   workspace_bytes, tpb_kv_attention_workspace_bytes(h, c->head_dim));
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
@@ -990,7 +991,7 @@ int tpb_kv_attention(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c,
     p.notes = p.ws + (size_t)h->sm_count * kMaxCtas * 2 * slot_floats(c->head_dim);
     p.status = h->d_status;
     // sequences known to be short stay whole, which saves the second launch (a longer one that comes all the same is one CTA's work)
-    p.whole = max_len > 0 && max_len <= kMinTokens;
+    p.whole = whole;
     cudaStream_t st = (cudaStream_t)stream;
     if (c->head_dim == 64) return c->format == TPB_KV_S8 ? by_type<64, TPB_KV_S8>(h, st, p) : by_type<64, TPB_KV_E4M3>(h, st, p);
     return c->format == TPB_KV_S8 ? by_type<128, TPB_KV_S8>(h, st, p) : by_type<128, TPB_KV_E4M3>(h, st, p);

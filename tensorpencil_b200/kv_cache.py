@@ -84,6 +84,8 @@ class KvCache:
         if nbytes == 0:
             raise ValueError(f"a cache of {n_pages} pages and {max_seqs} sequences is out of range")
         self._scratch = torch.empty(nbytes, dtype=torch.uint8, device=backend.device)
+        self._calls, self._index, self._scale = backend._attn_calls, k.get_device(), head_dim ** -0.5
+        self._no_workspace = _lib.KV_SHORT
         self._workspace_bytes = int(backend.lib.tpb_kv_attention_workspace_bytes(backend.h, head_dim))
         d = _lib.KvCacheDesc(k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), table=table.data_ptr(),
                              lens=lens.data_ptr(), tail=tail.data_ptr(), refs=refs.data_ptr(), result=self.result.data_ptr(),
@@ -92,35 +94,43 @@ class KvCache:
         self._desc, self._d = d, C.addressof(d)
 
     # -- arguments -------------------------------------------------------------------
-    def _ints(self, name: str, t: torch.Tensor, n: Optional[int] = None) -> int:
+    # A decode step makes two of these calls a layer, each about as long as its kernel: the checks ask every tensor for as little as they can.
+    def _ints(self, name: str, t: torch.Tensor, n: int) -> int:
+        if t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.get_device() == self._index:
+            return t.data_ptr()
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32 (got {t.dtype})")
-        if t.device != self.be.device or not t.is_contiguous() or t.dim() != 1 or (n is not None and t.shape[0] != n):
-            raise ValueError(f"{name} must be a contiguous vector{'' if n is None else f' of {n}'} on {self.be.device}")
-        return t.data_ptr()
+        raise ValueError(f"{name} must be a contiguous vector of {n} on {self.be.device} (got {tuple(t.shape)} on {t.device})")
 
     def _rows(self, name: str, t: torch.Tensor, rows: int, heads: int, dtype: torch.dtype) -> int:
         """Elements from one row to the next of [rows][heads * head_dim] or [rows][heads][head_dim]; columns are contiguous."""
         width = heads * self.head_dim
+        s, st = t.shape, t.stride()
+        if t.dtype is dtype and len(s) == 2 and s[1] == width and st[1] == 1 and s[0] == rows and t.get_device() == self._index:
+            return st[0] if rows > 1 else max(st[0], width)
         if t.dtype != dtype or dtype not in _ROWS:
             raise TypeError(f"{name} must be float32, bfloat16 or float16, like its partners (got {t.dtype})")
-        s = t.shape
-        if t.device != self.be.device or s[0] != rows or not (
-                (len(s) == 2 and s[1] == width and (t.stride(1) == 1)) or
-                (len(s) == 3 and s[1] == heads and s[2] == self.head_dim and t.stride(2) == 1 and (t.stride(1) == self.head_dim or heads == 1))):
-            raise ValueError(f"{name} must be [{rows}][{width}] on {self.be.device}, contiguous within a row (got {tuple(s)}, strides {t.stride()})")
-        return max(t.stride(0), width) if rows <= 1 else t.stride(0)
+        if t.get_device() != self._index or s[0] != rows or not (
+                len(s) == 3 and s[1] == heads and s[2] == self.head_dim and st[2] == 1 and (st[1] == self.head_dim or heads == 1)):
+            raise ValueError(f"{name} must be [{rows}][{width}] on {self.be.device}, contiguous within a row (got {tuple(s)}, strides {st})")
+        return st[0] if rows > 1 else max(st[0], width)
+
+    @staticmethod
+    def _dtype(name: str, t: torch.Tensor) -> int:
+        try:
+            return _ROWS[t.dtype]
+        except KeyError:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})") from None
 
     # -- tokens ----------------------------------------------------------------------
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, cu: torch.Tensor):
         """Quantises k and v ([rows][kv_heads * head_dim], f32, bf16 or f16) into the last cu[i + 1] - cu[i] places of each sequence: the
         tokens of its last ``extend``."""
-        rows = k.shape[0]
+        be, dtype = self.be, self._dtype("k", k)
+        rows, n = k.shape[0], seqs.shape[0]
         ld_k, ld_v = self._rows("k", k, rows, self.kv_heads, k.dtype), self._rows("v", v, rows, self.kv_heads, k.dtype)
-        n = seqs.shape[0]
-        be = self.be
-        rc = be._attn_calls.tpb_kv_append(be._hv, be._stream(), self._d, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _ROWS[k.dtype],
-                                     self._ints("seqs", seqs), self._ints("cu", cu, n + 1), n, rows)
+        ids, at = self._ints("seqs", seqs, n), self._ints("cu", cu, n + 1)
+        rc = self._calls.tpb_kv_append(be._hv, be._stream(), self._d, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, dtype, ids, at, n, rows)
         if rc != TPB_OK:
             be._check(rc)
         be.launches += 1
@@ -129,15 +139,16 @@ class KvCache:
              dtype: torch.dtype = torch.float32, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values of tokens start[i] .. start[i] + cu[i + 1] - cu[i] - 1 of each sequence (from 0 without ``start``), packed into ``rows``
         rows; zero behind a sequence's end.  Rows of no sequence are not written."""
+        be, n, width = self.be, seqs.shape[0], self.kv_heads * self.head_dim
+        ids, at = self._ints("seqs", seqs, n), self._ints("cu", cu, n + 1)
         if out is None:
-            out = tuple(torch.empty((rows, self.kv_heads * self.head_dim), dtype=dtype, device=self.be.device) for _ in range(2))
-        k, v = out
-        ld_k, ld_v = self._rows("k", k, rows, self.kv_heads, k.dtype), self._rows("v", v, rows, self.kv_heads, k.dtype)
-        n = seqs.shape[0]
-        be = self.be
-        rc = be._attn_calls.tpb_kv_read(be._hv, be._stream(), self._d, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _ROWS[k.dtype],
-                                   self._ints("seqs", seqs), None if start is None else self._ints("start", start, n),
-                                   self._ints("cu", cu, n + 1), n, rows)
+            k, v = torch.empty((2, rows, width), dtype=dtype, device=be.device).unbind(0)
+            ld_k = ld_v = width
+        else:
+            k, v = out
+            ld_k, ld_v = self._rows("k", k, rows, self.kv_heads, k.dtype), self._rows("v", v, rows, self.kv_heads, k.dtype)
+        rc = self._calls.tpb_kv_read(be._hv, be._stream(), self._d, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, self._dtype("k", k), ids,
+                                     None if start is None else self._ints("start", start, n), at, n, rows)
         if rc != TPB_OK:
             be._check(rc)
         be.launches += 1
@@ -147,18 +158,20 @@ class KvCache:
                   max_len: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of each sequence's last cu[i + 1] - cu[i] tokens, whose queries are q's rows ([rows][heads * head_dim], f32, bf16 or
         f16), over the sequence's cache; the result has q's type.  ``max_len``: an upper bound of the lengths, where the host knows one."""
+        be, dtype = self.be, self._dtype("q", q)
         rows, n = q.shape[0], seqs.shape[0]
         ld_q = self._rows("q", q, rows, heads, q.dtype)
-        be = self.be
         if out is None:
-            out = torch.empty((rows, heads * self.head_dim), dtype=q.dtype, device=q.device)
-        ld_out = self._rows("out", out, rows, heads, q.dtype)
-        # of this call alone: another stream's call, or a captured one's replay, may run beside it
-        work = torch.empty(self._workspace_bytes, dtype=torch.uint8, device=q.device)
-        rc = be._attn_calls.tpb_kv_attention(be._hv, be._stream(), self._d, layer, out.data_ptr(), ld_out, q.data_ptr(), ld_q, _ROWS[q.dtype],
-                                        self._ints("seqs", seqs), self._ints("cu", cu, n + 1), n, rows, heads,
-                                        float(scale) if scale is not None else self.head_dim ** -0.5, max_len, work.data_ptr(),
-                                        self._workspace_bytes)
+            out = q.new_empty((rows, heads * self.head_dim))
+            ld_out = heads * self.head_dim
+        else:
+            ld_out = self._rows("out", out, rows, heads, q.dtype)
+        # of this call alone: another stream's call, or a captured one's replay, may run beside it.  Short sequences need none.
+        work = None if 0 < max_len <= self._no_workspace else torch.empty(self._workspace_bytes, dtype=torch.uint8, device=be.device)
+        ids, at = self._ints("seqs", seqs, n), self._ints("cu", cu, n + 1)
+        rc = self._calls.tpb_kv_attention(be._hv, be._stream(), self._d, layer, out.data_ptr(), ld_out, q.data_ptr(), ld_q, dtype, ids, at, n, rows,
+                                          heads, self._scale if scale is None else float(scale), max_len,
+                                          None if work is None else work.data_ptr(), 0 if work is None else self._workspace_bytes)
         if rc != TPB_OK:
             be._check(rc)
         be.launches += 1
@@ -168,14 +181,14 @@ class KvCache:
     def extend(self, seqs: torch.Tensor, n_new: torch.Tensor):
         """Room for n_new[i] more tokens in sequence seqs[i]; lens counts them from here on."""
         n = seqs.shape[0]
-        self.be._check(self.be.lib.tpb_kv_extend(self.be._hv, self.be._stream(), self._d, self._ints("seqs", seqs),
+        self.be._check(self.be.lib.tpb_kv_extend(self.be._hv, self.be._stream(), self._d, self._ints("seqs", seqs, n),
                                                  self._ints("n_new", n_new, n), n))
         self.be.launches += 1
 
     def truncate(self, seqs: torch.Tensor, lens: Optional[torch.Tensor] = None):
         """Cuts sequence seqs[i] to lens[i] tokens; without ``lens`` frees it."""
         n = seqs.shape[0]
-        self.be._check(self.be.lib.tpb_kv_truncate(self.be._hv, self.be._stream(), self._d, self._ints("seqs", seqs),
+        self.be._check(self.be.lib.tpb_kv_truncate(self.be._hv, self.be._stream(), self._d, self._ints("seqs", seqs, n),
                                                    None if lens is None else self._ints("lens", lens, n), n))
         self.be.launches += 1 if lens is None else 2
 
@@ -183,7 +196,7 @@ class KvCache:
         """Makes the free sequence dst[i] a copy of src[i]: holding src's full pages and a copy of the part-filled one, or, with ``share``
         false, a copy of every page."""
         n = src.shape[0]
-        self.be._check(self.be.lib.tpb_kv_fork(self.be._hv, self.be._stream(), self._d, self._ints("src", src), self._ints("dst", dst, n), n,
+        self.be._check(self.be.lib.tpb_kv_fork(self.be._hv, self.be._stream(), self._d, self._ints("src", src, n), self._ints("dst", dst, n), n,
                                                int(share)))
         self.be.launches += 2
 

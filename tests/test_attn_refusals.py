@@ -119,7 +119,7 @@ def test_a_small_workspace_is_refused(lib, handle):
 
 def cpu_backend():
     be = Backend.__new__(Backend)                          # no device, no library behind it: the checks come first
-    be.device = torch.device("cpu")
+    be.device, be._index = torch.device("cpu"), -1
     return be
 
 
@@ -132,7 +132,7 @@ def test_attention_packed_refuses_tensors():
         with pytest.raises(TypeError):
             call(**bad)
     for bad in (dict(q=q[:, :192]), dict(k=k[:9]), dict(v=k.t().contiguous().t()), dict(heads=8), dict(cu=cu.view(1, 2)), dict(out=q[:5]),
-                dict(cu=torch.zeros(4, dtype=torch.int32)[::2]), dict(q=q.view(10, 2, 128)), dict(q=q.to("meta"))):
+                dict(cu=torch.zeros(4, dtype=torch.int32)[::2]), dict(q=q.view(10, 2, 128))):
         with pytest.raises(ValueError):
             call(**bad)
 
@@ -160,20 +160,28 @@ def test_a_cache_refuses_tensors_that_do_not_fit():
 
 def test_cache_methods_refuse_tensors():
     c = KvCache.__new__(KvCache)
-    c.be, c.kv_heads, c.head_dim = cpu_backend(), 2, 64
+    c.be, c.kv_heads, c.head_dim, c._index = cpu_backend(), 2, 64, -1
     x, ids, cu = torch.zeros(5, 128), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     for bad in (dict(k=x.double(), v=x.double()), dict(v=x.half()), dict(k=x.to(torch.int8))):
         with pytest.raises(TypeError):
             c.append(0, **{"k": x, "v": x, "seqs": ids, "cu": cu, **bad})
-    for bad in (dict(k=x[:, :64]), dict(v=x[:4]), dict(v=x.t().contiguous().t()), dict(k=x.to("meta"))):
+    for bad in (dict(k=x[:, :64]), dict(v=x[:4]), dict(v=x.t().contiguous().t())):
         with pytest.raises(ValueError):
             c.append(0, **{"k": x, "v": x, "seqs": ids, "cu": cu, **bad})
     with pytest.raises(TypeError):
-        c._ints("seqs", ids.long())
+        c._ints("seqs", ids.long(), 1)
     with pytest.raises(ValueError):
         c._ints("cu", cu, 3)
     with pytest.raises(ValueError):
         c._rows("q", torch.zeros(5, 256), 5, 8, torch.float32)
+    c._index = 0                                           # tensors of another device than the cache's
+    for call in (lambda: c._rows("q", torch.zeros(5, 128), 5, 2, torch.float32), lambda: c._ints("cu", cu, 2)):
+        with pytest.raises(ValueError):
+            call()
+    be = cpu_backend()
+    be._index = 0
+    with pytest.raises(ValueError):
+        be._packed_ld("q", torch.zeros(5, 128), 5, 2, 64)
 
 
 def test_places_of_the_append_launch():
