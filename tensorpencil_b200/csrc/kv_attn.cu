@@ -49,10 +49,11 @@ struct Cfg {
     static constexpr bool kQRegs = NT * kTerms <= 2 && HD * NT * kTerms <= 256;      // q's fragments in registers
     static constexpr int kQf = kQRegs ? 0 : NT * kSteps * kTerms * 32 * 8;           // or in shared memory
     static constexpr int kMergeLd = HD + 4;
-    static constexpr int kMerge = kRows * kMergeLd * 4;                  // where the warps' sums are added up
+    static constexpr int kMerge = 2 * kRows * kMergeLd * 4;              // where the warps' sums are added up, in pairs
     static constexpr int kSmem = kWarps * kRing + kMerge + kQf;
     static constexpr int kCtas = NT == 1 ? 3 : 2;                        // per SM
     static_assert(kRows <= 32, "rows fit a slot");
+    static_assert(kCtas * (kSmem + 2816 + 1024) <= 228 * 1024 || NT > 1, "three CTAs fit an SM (2816: the static shared memory)");
 };
 constexpr int kMaxCtas = 3, kMaxRows = 32;
 
@@ -85,25 +86,28 @@ struct AttnParams {
 };
 
 // ---- the line of units ------------------------------------------------------------------------
-// Chunk of kThreads sequences of the batch in shared memory: first unit, length, rows.
+// Chunk of kSeqs sequences of the batch in shared memory: first unit, length, rows.  (With 128 of them a third CTA would not fit an SM.)
+constexpr int kSeqs = 96;
 struct Chunk {
-    long long start[kThreads + 1];
-    int len[kThreads], row0[kThreads], n_q[kThreads], seq[kThreads];
-    long long warp_sum[kThreads / 32];
+    long long start[kSeqs + 1];
+    int len[kSeqs], row0[kSeqs], n_q[kSeqs], seq[kSeqs];
+    long long warp_sum[kSeqs / 32];
 };
-// A run costs about a unit of time more than its tokens do (48 sequences of 1 to 16000 tokens, 8 kv heads: CTAs that drew the short ones were
-// the last to end), so its units begin with one that has no tokens.
+// A run takes about as long again as kRunUnits of its tokens' units do -- its chain of loads, q, the merging -- so its units begin with that many
+// which have no tokens.  (48 sequences of 1 to 16000 tokens, 8 kv heads, a unit 1.9 us: without them half the CTAs ended at 60 us and those that
+// drew the short sequences at 140, with one 100.)
+constexpr int kRunUnits = 3;
 template <int UNIT>
-__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : 1 + (len + UNIT - 1) / UNIT; }
+__device__ __forceinline__ int tiles_of(const AttnParams &p, int len) { return p.whole ? 1 : kRunUnits + (len + UNIT - 1) / UNIT; }
 
-// Loads sequences base .. base + kThreads - 1, the first of which begins at unit `cum`; returns the unit behind the last.  `tell`: report ids and
+// Loads sequences base .. base + kSeqs - 1, the first of which begins at unit `cum`; returns the unit behind the last.  `tell`: report ids and
 // lengths out of range (such a sequence has no units: its rows are not written).
 template <int RT, int UNIT>
 __device__ long long load_chunk(const AttnParams &p, Chunk &ck, int base, long long cum, bool tell) {
     const int i = base + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long units = 0;
     int len = 0, row0 = 0, n_q = 0, seq = -1;
-    if (i < p.n_seqs && threadIdx.x < kThreads) {
+    if (i < p.n_seqs && threadIdx.x < kSeqs) {
         seq = __ldcg(p.seqs + i);
         row0 = row_offset(p.cu, i, p.rows);
         n_q = row_offset(p.cu, i + 1, p.rows) - row0;
@@ -127,27 +131,27 @@ __device__ long long load_chunk(const AttnParams &p, Chunk &ck, int base, long l
         if (lane >= o) inc += t;
     }
     __syncthreads();                     // the last user of the chunk is done
-    if (warp < kThreads / 32 && lane == 31) ck.warp_sum[warp] = inc;
+    if (warp < kSeqs / 32 && lane == 31) ck.warp_sum[warp] = inc;
     __syncthreads();
     long long at = cum, total = cum;
-    for (int w = 0; w < kThreads / 32; w++) {
+    for (int w = 0; w < kSeqs / 32; w++) {
         if (w < warp) at += ck.warp_sum[w];
         total += ck.warp_sum[w];
     }
-    if (threadIdx.x < kThreads) {
+    if (threadIdx.x < kSeqs) {
         ck.start[threadIdx.x] = at + inc - units;
         ck.len[threadIdx.x] = len;
         ck.row0[threadIdx.x] = row0;
         ck.n_q[threadIdx.x] = n_q;
         ck.seq[threadIdx.x] = seq;
-        if (threadIdx.x == kThreads - 1) ck.start[kThreads] = total;
+        if (threadIdx.x == kSeqs - 1) ck.start[kSeqs] = total;
     }
     __syncthreads();
     return total;
 }
-// The sequence of the loaded chunk that holds unit u, start[0] <= u < start[kThreads].
+// The sequence of the loaded chunk that holds unit u, start[0] <= u < start[kSeqs].
 __device__ __forceinline__ int find_in_chunk(const Chunk &ck, long long u) {
-    int lo = 0, hi = kThreads;           // start[lo] <= u < start[hi]
+    int lo = 0, hi = kSeqs;           // start[lo] <= u < start[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (ck.start[mid] <= u) lo = mid;
@@ -178,7 +182,7 @@ __device__ __forceinline__ Segment segment_at(const AttnParams &p, const Chunk &
 }
 template <int UNIT>
 __device__ __forceinline__ long long units_per_cta(const AttnParams &p, long long total, int ctas) {
-    return max((total + ctas - 1) / ctas, (long long)(p.whole ? 1 : kMinTokens / UNIT));
+    return max((total + ctas - 1) / ctas, (long long)(p.whole ? 1 : kRunUnits + kMinTokens / UNIT));
 }
 
 // ---- arithmetic -------------------------------------------------------------------------------
@@ -351,17 +355,17 @@ kv_attention_kernel(const AttnParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
 
     long long total = 0;
-    for (int base = 0; base < p.n_seqs; base += kThreads) total = load_chunk<RT, UNIT>(p, ck, base, total, blockIdx.x == 0);
+    for (int base = 0; base < p.n_seqs; base += kSeqs) total = load_chunk<RT, UNIT>(p, ck, base, total, blockIdx.x == 0);
     const long long per = units_per_cta<UNIT>(p, total, (int)gridDim.x);
     long long u = per * blockIdx.x;
     const long long u_end = min(u + per, total);
     JoinNote note = {};
     if (u < u_end) {
         int base = 0;
-        if (p.n_seqs > kThreads) {
+        if (p.n_seqs > kSeqs) {
             long long behind = load_chunk<RT, UNIT>(p, ck, 0, 0, false);
             while (u >= behind) {
-                base += kThreads;
+                base += kSeqs;
                 behind = load_chunk<RT, UNIT>(p, ck, base, behind, false);
             }
         }
@@ -436,17 +440,17 @@ kv_attention_kernel(const AttnParams p) {
         };
         // Makes the run that begins at unit u the one at hand and sets its first steps on their way.
         const auto begin = [&]() {
-            while (u >= ck.start[kThreads]) {
-                base += kThreads;
-                load_chunk<RT, UNIT>(p, ck, base, ck.start[kThreads], false);
+            while (u >= ck.start[kSeqs]) {
+                base += kSeqs;
+                load_chunk<RT, UNIT>(p, ck, base, ck.start[kSeqs], false);
             }
             s = segment_at<RT, UNIT>(p, ck, u, u_end);
             len = ck.len[s.idx];
             n_q = ck.n_q[s.idx];
             row0 = ck.row0[s.idx];
             row = p.c.table + (size_t)ck.seq[s.idx] * p.c.max_pages;
-            tok1 = p.whole ? len : min((s.t1 - 1) * UNIT, len);
-            mine0 = max(s.t0 - 1, 0) * UNIT + warp * C::kStep;
+            tok1 = p.whole ? len : min(max(s.t1 - kRunUnits, 0) * UNIT, len);
+            mine0 = max(s.t0 - kRunUnits, 0) * UNIT + warp * C::kStep;
             n_steps = tok1 > mine0 ? (tok1 - mine0 + UNIT - 1) / UNIT : 0;
             now0 = 0;
             now = look(0);
@@ -738,16 +742,18 @@ kv_attention_kernel(const AttnParams p) {
                         o[nt][m][2 + e] *= f2;
                     }
                 }
+            // (warp 0 + warp 1) + (warp 2 + warp 3), the halves at the same time
+            float *half = merge + (warp >> 1) * (RT * C::kMergeLd);
 #pragma unroll 1
-            for (int w = 0; w < kWarps; w++) {
-                if (warp == w) {
+            for (int w = 0; w < 2; w++) {
+                if ((warp & 1) == w) {
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 2; e++)
 #pragma unroll
                             for (int i4 = 0; i4 < HD / 32; i4++) {
-                                float4 *dst = reinterpret_cast<float4 *>(merge + (nt * 8 + 2 * t + e) * C::kMergeLd + 32 * i4 + 4 * g);
+                                float4 *dst = reinterpret_cast<float4 *>(half + (nt * 8 + 2 * t + e) * C::kMergeLd + 32 * i4 + 4 * g);
                                 float4 x = make_float4(o[nt][2 * i4][e], o[nt][2 * i4][2 + e], o[nt][2 * i4 + 1][e], o[nt][2 * i4 + 1][2 + e]);
                                 if (w > 0) {
                                     const float4 y = *dst;
@@ -770,7 +776,9 @@ kv_attention_kernel(const AttnParams p) {
                 }
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) sum += s_l[w][r] * part_factor(s_ms[w][r], big_s);
-                const float4 a = *reinterpret_cast<const float4 *>(merge + r * C::kMergeLd + d);
+                const float4 a0 = *reinterpret_cast<const float4 *>(merge + r * C::kMergeLd + d);
+                const float4 a1 = *reinterpret_cast<const float4 *>(merge + (RT + r) * C::kMergeLd + d);
+                const float4 a = make_float4(a0.x + a1.x, a0.y + a1.y, a0.z + a1.z, a0.w + a1.w);
                 if (whole) {
                     float second;
                     const float f = finish_scale(big_s, sum, big_w, second);
