@@ -230,7 +230,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         // ---------------- softmax + output: a thread per row ----------------
         const int x = warp >> 2;
         const int r = (warp & 3) * 32 + lane;
-        const int tok = r / p.group, hq = r - tok * p.group;
+        const int tok = r / p.group;
         const int pos = pos0 + x * p.tile_tokens + tok;
         const bool row_ok = tok < p.tile_tokens && pos < len;
         const int lim = row_ok ? pos + 1 : 0;                    // keys that the row sees
@@ -320,17 +320,19 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             if (ok) {
                 tc_fence_after();
                 const float inv_l = 1.0f / l_run;
-                T *dst = static_cast<T *>(p.out) + (long long)(start + pos) * p.ld_out + (long long)(head * p.group + hq) * HD;
                 // Did V have a NaN or an infinity where somebody does not look?  (Every lane asks for every 32nd column.)
                 bool fix = false;
                 for (int i = lane; i < 3 * HD; i += 32) fix |= bad[i] != INT_MAX;
                 fix = __any_sync(0xffffffffu, fix);
+                // A thread has a row; whole rows leave through the place of the tile's queries, which nobody reads any more: stores of 32 rows' 16
+                // bytes each took 3.6 us a CTA.  Pieces of 16 bytes are permuted within eight rows, so neither side has bank conflicts.
+                constexpr int kPieces = HD / 8;                              // of a row
+                const uint32_t mine = smem_base + L::kQ + x * L::kAtoms * kAtomBytes + (uint32_t)(warp & 3) * (32 * HD * 2);
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; c++) {
                     uint32_t v[32];
                     tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
                     tc_wait_ld_dep(v);
-                    if (!row_ok) continue;
                     if (fix) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
@@ -348,8 +350,21 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             w[e] = pack2<T>(__uint_as_float(v[8 * i + 2 * e]) * inv_l, __uint_as_float(v[8 * i + 2 * e + 1]) * inv_l);
-                        reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        st_shared_v4(mine + (uint32_t)(lane * HD * 2) + (uint32_t)(((c * 4 + i) ^ (lane & 7)) * 16), w[0], w[1], w[2], w[3]);
                     }
+                }
+                __syncwarp();
+                const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
+                constexpr int kRowsAtOnce = 32 / kPieces;
+                const int piece = lane % kPieces;
+#pragma unroll 4
+                for (int q = 0; q < 32; q += kRowsAtOnce) {
+                    const int rr = q + lane / kPieces;                       // row of the warp's 32
+                    const int tile_row = (warp & 3) * 32 + rr, tk = tile_row / p.group;
+                    const uint4 w = ld_shared_v4(mine + (uint32_t)(rr * HD * 2) + (uint32_t)((piece ^ (rr & 7)) * 16));
+                    if ((rows_ok >> rr) & 1u)
+                        st_global_v4(static_cast<T *>(p.out) + (long long)(start + pos0 + x * p.tile_tokens + tk) * p.ld_out +
+                                         (long long)(head * p.group + tile_row - tk * p.group) * HD + piece * 8, w);
                 }
             }
         }
