@@ -175,6 +175,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const auto o_done = [&](int x) { return bars + 8u * (18 + x); };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBar + 192);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + L::kBar + 200);
+    volatile int *any_bad = reinterpret_cast<volatile int *>(gen + L::kBar + 204);
     int *bad = reinterpret_cast<int *>(gen + L::kBad);
 
     const int warp = threadIdx.x >> 5;
@@ -213,9 +214,16 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             mbar_init(o_done(s), 1);
         }
         *abort_flag = 0;
+        *any_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     for (int i = threadIdx.x; i < 3 * HD; i += kThreads) bad[i] = INT_MAX;
+    // Rows of a tile of queries that hold no token (128 / group has a remainder): zeros, or an infinity left there would move their reference
+    // point tile after tile.
+    const int used_rows = p.tile_tokens * p.group;
+    for (int i = threadIdx.x; i < (kTile - used_rows) * 8 * 2 * L::kAtoms; i += kThreads)
+        st_shared_v4(smem_base + L::kQ + (i / ((kTile - used_rows) * 8)) * kAtomBytes + used_rows * 128 + (i % ((kTile - used_rows) * 8)) * 16, 0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512)
                      : "memory");
@@ -226,20 +234,24 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
+    // A softmax thread's row.  (Inside the branch below, the same lines cost nine registers too many: 8192 tokens 510 us with the spills, 487 without.)
+    const int x_of_warp = (warp >> 2) & 1;
+    const int row = (warp & 3) * 32 + lane;
+    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    const int pos = pos0 + x_of_warp * p.tile_tokens + row_tok;
+    const bool row_ok = row_tok < p.tile_tokens && pos < len;
+    const int lim = row_ok ? pos + 1 : 0;                        // keys that the row sees
+    const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_o = tmem_base + t_lane + 256u + (uint32_t)(x_of_warp * HD);
+    float l_run = 0.0f;
+    bool ok = true;
+
     if (warp < 8) {
-        // ---------------- softmax + output: a thread per row ----------------
-        const int x = warp >> 2;
-        const int r = (warp & 3) * 32 + lane;
-        const int tok = r / p.group;
-        const int pos = pos0 + x * p.tile_tokens + tok;
-        const bool row_ok = tok < p.tile_tokens && pos < len;
-        const int lim = row_ok ? pos + 1 : 0;                    // keys that the row sees
+        // ---------------- softmax: a thread per row ----------------
+        const int x = x_of_warp;
         const int my_tiles = x ? tiles_b : tiles_a;
-        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem_base + t_lane + (uint32_t)(x * 128);
-        const uint32_t t_o = tmem_base + t_lane + 256u + (uint32_t)(x * HD);
-        float m_run = -3.402823466e38f, l_run = 0.0f;
-        bool ok = true;
+        float m_run = -3.402823466e38f;
         const auto do_tile = [&](auto masked_tag, const int j) -> bool {
             constexpr bool MASKED = decltype(masked_tag)::value;
             const bool good = mbar_wait(s_full(x), (uint32_t)j & 1u, abort_flag, p.status, (14u << 24) | 1u, true);
@@ -309,64 +321,13 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             m_run = m_new;
             return true;
         };
-        // a tile of keys that every row of this tile sees as a whole needs no mask
+        // A tile of keys that the first token sees as a whole needs no mask: rows behind the last token, or behind the last whole token of the tile,
+        // come to nothing whatever they see.
         const int whole = pos0 + x * p.tile_tokens + 1;
-        const bool rows_full = end_b - pos0 >= (x + 1) * p.tile_tokens && p.tile_tokens * p.group == kTile;
-        for (int j = 0; ok && j < my_tiles; j++)
-            ok = rows_full && (j + 1) * kTile <= whole ? do_tile(std::false_type{}, j) : do_tile(std::true_type{}, j);
+        for (int j = 0; ok && j < my_tiles; j++) ok = (j + 1) * kTile <= whole ? do_tile(std::false_type{}, j) : do_tile(std::true_type{}, j);
         if (ok && my_tiles > 0) {
             ok = mbar_wait(o_done(x), 0, abort_flag, p.status, (14u << 24) | 3u, true);
             ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                tc_fence_after();
-                const float inv_l = 1.0f / l_run;
-                // Did V have a NaN or an infinity where somebody does not look?  (Every lane asks for every 32nd column.)
-                bool fix = false;
-                for (int i = lane; i < 3 * HD; i += 32) fix |= bad[i] != INT_MAX;
-                fix = __any_sync(0xffffffffu, fix);
-                // A thread has a row; whole rows leave through the place of the tile's queries, which nobody reads any more: stores of 32 rows' 16
-                // bytes each took 3.6 us a CTA.  Pieces of 16 bytes are permuted within eight rows, so neither side has bank conflicts.
-                constexpr int kPieces = HD / 8;                              // of a row
-                const uint32_t mine = smem_base + L::kQ + x * L::kAtoms * kAtomBytes + (uint32_t)(warp & 3) * (32 * HD * 2);
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    uint32_t v[32];
-                    tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
-                    tc_wait_ld_dep(v);
-                    if (fix) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            float o = __uint_as_float(v[i]);
-                            const int col = c * 32 + i;
-                            if (lim > bad[col]) o += __uint_as_float(0x7fc00000u);
-                            if (lim > bad[HD + col]) o += INFINITY;
-                            if (lim > bad[2 * HD + col]) o -= INFINITY;
-                            v[i] = __float_as_uint(o);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            w[e] = pack2<T>(__uint_as_float(v[8 * i + 2 * e]) * inv_l, __uint_as_float(v[8 * i + 2 * e + 1]) * inv_l);
-                        st_shared_v4(mine + (uint32_t)(lane * HD * 2) + (uint32_t)(((c * 4 + i) ^ (lane & 7)) * 16), w[0], w[1], w[2], w[3]);
-                    }
-                }
-                __syncwarp();
-                const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
-                constexpr int kRowsAtOnce = 32 / kPieces;
-                const int piece = lane % kPieces;
-#pragma unroll 4
-                for (int q = 0; q < 32; q += kRowsAtOnce) {
-                    const int rr = q + lane / kPieces;                       // row of the warp's 32
-                    const int tile_row = (warp & 3) * 32 + rr, tk = tile_row / p.group;
-                    const uint4 w = ld_shared_v4(mine + (uint32_t)(rr * HD * 2) + (uint32_t)((piece ^ (rr & 7)) * 16));
-                    if ((rows_ok >> rr) & 1u)
-                        st_global_v4(static_cast<T *>(p.out) + (long long)(start + pos0 + x * p.tile_tokens + tk) * p.ld_out +
-                                         (long long)(head * p.group + tile_row - tk * p.group) * HD + piece * 8, w);
-                }
-            }
         }
     } else {
         if (warp == 8) {
@@ -379,7 +340,6 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                         tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, head * p.group,
                                     start + pos0 + x * p.tile_tokens);
                 };
-                bool ok = true;
                 load_q(0);
                 for (int j = 0; ok && j < tiles; j++) {
                     const int st = j % kStages;
@@ -422,7 +382,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                                   (t > 0 || kk > 0) ? 1u : 0u);
                     }
                 };
-                bool ok = mbar_wait(q_full(0), 0, abort_flag, p.status, (13u << 24) | 1u);
+                ok = mbar_wait(q_full(0), 0, abort_flag, p.status, (13u << 24) | 1u);
                 if (ok) ok = mbar_wait(k_full(0), 0, abort_flag, p.status, (13u << 24) | 2u);
                 if (ok) {
                     tc_fence_after();
@@ -469,7 +429,6 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             // ---------------- V: warps 10 and 11, half of a tile's rows each ----------------
             constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;      // exponent all ones: NaN or infinity
             constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-            bool ok = true;
             for (int j = 0; ok && j < tiles; j++) {
                 const int st = j % kStages;
                 ok = mbar_wait(v_full(st), (uint32_t)(j / kStages) & 1u, abort_flag, p.status, (15u << 24) | 1u, true);
@@ -492,6 +451,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                                     if (key < len) {
                                         const int kind = (h & ~(ex | 0x8000u) & 0xffffu) != 0 ? 0 : (h & 0x8000u) ? 2 : 1;
                                         atomicMin(bad + kind * HD + col0 + e, key);
+                                        *any_bad = 1;
                                     }
                                     u[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
                                 }
@@ -504,6 +464,42 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_seen(st));
             }
+        }
+    }
+
+    // ---------------- output ----------------
+    if (warp < 8 && ok && (x_of_warp ? tiles_b : tiles_a) > 0) {
+        tc_fence_after();
+        const float inv_l = 1.0f / l_run;
+        T *dst = static_cast<T *>(p.out) + (long long)(start + pos) * p.ld_out + (long long)(head * p.group + row_head) * HD;
+        const bool fix = *any_bad != 0;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; c++) {
+            uint32_t v[32];
+            tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
+            tc_wait_ld_dep(v);
+            if (row_ok) {
+                if (fix) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        float o = __uint_as_float(v[i]);
+                        const int col = c * 32 + i;
+                        if (lim > bad[col]) o += __uint_as_float(0x7fc00000u);
+                        if (lim > bad[HD + col]) o += INFINITY;
+                        if (lim > bad[2 * HD + col]) o -= INFINITY;
+                        v[i] = __float_as_uint(o);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] = pack2<T>(__uint_as_float(v[8 * i + 2 * e]) * inv_l, __uint_as_float(v[8 * i + 2 * e + 1]) * inv_l);
+                    reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            __syncwarp();
         }
     }
 

@@ -131,20 +131,36 @@ __device__ __forceinline__ void set_result(const tpb_kv_cache &c, int status, lo
     c.result[3] = (int)min(needed, (long long)INT32_MAX);
 }
 
+// A list of the call's: its entry threadIdx.x is asked for at once, and the first kSmallList entries are in shared memory from then on (a null list: all
+// zero).  at() may be used behind the next barrier, by any thread; mine() at once, for i = threadIdx.x + k kThreads.
+constexpr int kSmallList = 1024;
+static_assert(kSmallList == kThreads, "a thread keeps one entry");
+struct Listed {
+    const int32_t *list;
+    int32_t *kept;
+    int first;
+    __device__ Listed(const int32_t *l, int n, int32_t *smem) : list(l), kept(smem), first(l && (int)threadIdx.x < n ? __ldcg(l + threadIdx.x) : 0) {
+        kept[threadIdx.x] = first;
+    }
+    __device__ int mine(int i) const { return i < kThreads ? first : list ? __ldcg(list + i) : 0; }
+    __device__ int at(int i) const { return i < kSmallList ? kept[i] : list ? __ldcg(list + i) : 0; }
+};
+
 // A mark a sequence: bits in shared memory for up to kMarkBits sequences, else words of the cache's scratch (marks of the ids in question only).
 constexpr int kMarkBits = 32768;
 struct Marks {
     uint32_t *bits;
     int32_t *words;
     bool small;
-    __device__ void clear(const int32_t *ids, int n, int max_seqs) const {
-        if (small) {
+    __device__ void clear_bits(int max_seqs) const {             // before anything else
+        if (small)
             for (int i = threadIdx.x; i < (max_seqs + 31) / 32; i += kThreads) bits[i] = 0;
-        } else {
-            for (int i = threadIdx.x; i < n; i += kThreads) {
-                const int id = __ldcg(ids + i);
-                if (id >= 0 && id < max_seqs) words[id] = 0;
-            }
+    }
+    __device__ void clear_words(const Listed &ids, int n, int max_seqs) const {
+        if (small) return;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const int id = ids.mine(i);
+            if (id >= 0 && id < max_seqs) words[id] = 0;
         }
     }
     __device__ bool set(int id) const {           // was it set?
@@ -154,38 +170,29 @@ struct Marks {
     __device__ bool test(int id) const { return small ? (bits[id >> 5] >> (id & 31)) & 1u : __ldcg(words + id) != 0; }
 };
 
-// The first entry of a list that a thread deals with is in a register: list[threadIdx.x].
-struct Listed {
-    const int32_t *list;
-    int mine;
-    __device__ Listed(const int32_t *l, int n) : list(l), mine(l && (int)threadIdx.x < n ? __ldcg(l + threadIdx.x) : 0) {}
-    __device__ int at(int i) const { return !list ? 0 : i == (int)threadIdx.x ? mine : __ldcg(list + i); }
-};
-
 // A CTA's bookkeeping is a chain of dependent loads and barriers, 0.3 to 0.5 us each, so what does not depend on one another is asked for
-// together (the lists, the reference counts), what a later pass needs stays in registers, and offsets and marks are in shared memory.
-// fork + truncate of 32 sequences over 1300 pages: 28 -> 17 us with the copies.
-constexpr int kSmallList = 1024;
-
+// together (the lists, the reference counts), what a later pass needs stays in registers, and lists, lengths, offsets and marks are in shared memory.
+// fork + truncate of 32 sequences over 1300 pages, with the copies: 28 -> 19 us.
 __global__ void __launch_bounds__(kThreads)
 kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new, int n) {
     __shared__ long long buf[kWarps];
     __shared__ uint32_t bits[kMarkBits / 32];
-    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList];
+    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList], small_ids[kSmallList], small_adds[kSmallList], small_lens[kSmallList];
+    const Scratch sc = scratch_of(c);
+    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
+    marks.clear_bits(c.max_seqs);
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
-    const Scratch sc = scratch_of(c);
-    const Listed ids(seqs, n), adds(n_new, n);
+    const Listed ids(seqs, n, small_ids), adds(n_new, n, small_adds);
     Refs refs;
     load_refs(c, refs);
-    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
     int32_t *offsets = n <= kSmallList ? small_offsets : sc.offsets;
     const long long most = (long long)c.max_pages * c.page_tokens;
-    marks.clear(seqs, n, c.max_seqs);
+    marks.clear_words(ids, n, c.max_seqs);
     __syncthreads();
     bool ok = true;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int id = ids.at(i);
+        const int id = ids.mine(i);
         if (id < 0 || id >= c.max_seqs || marks.set(id)) ok = false;
     }
     long long before = 0;
@@ -197,7 +204,8 @@ kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new
             const int i = i0 + threadIdx.x;
             int want = 0;
             if (i < n) {
-                const int len = __ldcg(c.lens + ids.at(i)), add = adds.at(i);
+                const int len = __ldcg(c.lens + ids.mine(i)), add = adds.mine(i);
+                if (i < kSmallList) small_lens[i] = len;
                 if (len < 0 || add < 0 || (long long)len + add > most) ok = false;
                 else want = pages_of(c, len + add) - pages_of(c, len);
             }
@@ -210,7 +218,7 @@ kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new
     }
     if (!ok || need > free_pages) {
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int id = ids.at(i);
+            const int id = ids.mine(i);
             if (id >= 0 && id < c.max_seqs) c.tail[id] = 0;
         }
         set_result(c, ok ? TPB_ERR_OOM : TPB_ERR_INVALID_ARG, free_pages, 0, ok ? need : 0);
@@ -221,7 +229,7 @@ kv_extend_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *n_new
     __syncthreads();
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < n; i += kWarps) {
-        const int id = __ldcg(seqs + i), add = __ldcg(n_new + i), len = __ldcg(c.lens + id);
+        const int id = ids.at(i), add = adds.at(i), len = i < kSmallList ? small_lens[i] : __ldcg(c.lens + id);
         const int p0 = pages_of(c, len), p1 = pages_of(c, len + add), at = offsets[i];
         for (int p = p0 + lane; p < p1; p += 32) {
             const int page = list[at + p - p0];
@@ -252,21 +260,24 @@ __global__ void __launch_bounds__(kThreads)
 kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new_lens, int n, uint32_t *status) {
     __shared__ long long buf[kWarps];
     __shared__ uint32_t bits[kMarkBits / 32];
-    tpb_grid_dep_launch();
-    tpb_grid_dep_wait();
+    __shared__ int32_t small_ids[kSmallList], small_cuts[kSmallList], small_lens[kSmallList];
     const Scratch sc = scratch_of(c);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Listed ids(seqs, n), cuts(new_lens, n);
     const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
-    marks.clear(seqs, n, c.max_seqs);
+    marks.clear_bits(c.max_seqs);
+    tpb_grid_dep_launch();
+    tpb_grid_dep_wait();
+    const Listed ids(seqs, n, small_ids), cuts(new_lens, n, small_cuts);
+    marks.clear_words(ids, n, c.max_seqs);
     __syncthreads();
     bool ok = true;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int id = ids.at(i);
+        const int id = ids.mine(i);
         if (id < 0 || id >= c.max_seqs || marks.set(id)) {
             ok = false;
         } else {
-            const int len = __ldcg(c.lens + id), to = cuts.at(i);
+            const int len = __ldcg(c.lens + id), to = cuts.mine(i);
+            if (i < kSmallList) small_lens[i] = len;
             if (len < 0 || to < 0 || to > len || (long long)len > (long long)c.max_pages * c.page_tokens) ok = false;
         }
     }
@@ -280,12 +291,12 @@ kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new
         set_result(c, TPB_ERR_INVALID_ARG, free_pages, 0, 0);
         return;
     }
-    const auto new_len = [&](int i) { return new_lens ? __ldcg(new_lens + i) : 0; };
+    const auto old_len = [&](int i) { return i < kSmallList ? small_lens[i] : __ldcg(c.lens + ids.at(i)); };
     // give back the pages behind the cuts; `by` = 1 takes it back.  Where nothing can stop the operation any more, the rows are cleared at once.
     const auto drop = [&](int by, bool clear) {
         for (int i = warp; i < n; i += kWarps) {
-            const int id = __ldcg(seqs + i), p1 = pages_of(c, __ldcg(c.lens + id));
-            each_page(c, id, pages_of(c, new_len(i)), p1, status, [&](int p, int page) {
+            const int id = ids.at(i), p1 = pages_of(c, old_len(i));
+            each_page(c, id, pages_of(c, cuts.at(i)), p1, status, [&](int p, int page) {
                 atomicAdd(c.refs + page, by);
                 if (clear) c.table[(size_t)id * c.max_pages + p] = -1;
             });
@@ -312,9 +323,9 @@ kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new
         const int i = i0 + threadIdx.x;
         bool cut = false;
         if (i < n) {
-            const int to = cuts.at(i);
+            const int to = cuts.mine(i);
             if (to % c.page_tokens != 0) {
-                const int page = __ldcg(c.table + (size_t)ids.at(i) * c.max_pages + to / c.page_tokens);
+                const int page = __ldcg(c.table + (size_t)ids.mine(i) * c.max_pages + to / c.page_tokens);
                 if (page < 0 || page >= c.n_pages) report(status, kBadPage);
                 else cut = __ldcg(c.refs + page) > 1;
             }
@@ -336,7 +347,7 @@ kv_truncate_kernel(const tpb_kv_cache c, const int32_t *seqs, const int32_t *new
     list_pages(c, refs, sc.list_b, before, need, is_free);
     __syncthreads();
     for (int i = warp; i < n; i += kWarps) {
-        const int id = __ldcg(seqs + i), to = new_len(i), p0 = pages_of(c, to), p1 = pages_of(c, __ldcg(c.lens + id));
+        const int id = ids.at(i), to = cuts.at(i), p0 = pages_of(c, to), p1 = pages_of(c, old_len(i));
         int32_t *row = c.table + (size_t)id * c.max_pages;
         for (int p = p0 + lane; p < p1; p += 32) row[p] = -1;
         __syncwarp();
@@ -368,23 +379,24 @@ __global__ void __launch_bounds__(kThreads)
 kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int n, int share, uint32_t *status) {
     __shared__ long long buf[kWarps];
     __shared__ uint32_t bits[kMarkBits / 32];
-    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList];
-    tpb_grid_dep_launch();
-    tpb_grid_dep_wait();
+    __shared__ int32_t small_offsets[kSmallList], small_list[kSmallList], small_src[kSmallList], small_dst[kSmallList], small_lens[kSmallList];
     const Scratch sc = scratch_of(c);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Listed srcs(src, n), dsts(dst, n);
+    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
+    marks.clear_bits(c.max_seqs);
+    tpb_grid_dep_launch();
+    tpb_grid_dep_wait();
+    const Listed srcs(src, n, small_src), dsts(dst, n, small_dst);
     Refs refs;
     load_refs(c, refs);
-    const Marks marks{bits, sc.marks, c.max_seqs <= kMarkBits};
     int32_t *offsets = n <= kSmallList ? small_offsets : sc.offsets;
     // sources may repeat, destinations may not, and no sequence is both
-    marks.clear(src, n, c.max_seqs);
-    marks.clear(dst, n, c.max_seqs);
+    marks.clear_words(srcs, n, c.max_seqs);
+    marks.clear_words(dsts, n, c.max_seqs);
     __syncthreads();
     bool ok = true;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int from = srcs.at(i), to = dsts.at(i);
+        const int from = srcs.mine(i), to = dsts.mine(i);
         if (from < 0 || from >= c.max_seqs || to < 0 || to >= c.max_seqs || marks.set(to)) ok = false;
     }
     long long before = 0;
@@ -397,7 +409,8 @@ kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int
             const int i = i0 + threadIdx.x;
             int want = 0;
             if (i < n) {
-                const int from = srcs.at(i), len = __ldcg(c.lens + from), taken = __ldcg(c.lens + dsts.at(i));
+                const int from = srcs.mine(i), len = __ldcg(c.lens + from), taken = __ldcg(c.lens + dsts.mine(i));
+                if (i < kSmallList) small_lens[i] = len;
                 if (marks.test(from) || len < 0 || len > most || taken != 0) ok = false;
                 else want = share ? (len % c.page_tokens != 0) : pages_of(c, len);
             }
@@ -418,7 +431,7 @@ kv_fork_kernel(const tpb_kv_cache c, const int32_t *src, const int32_t *dst, int
     if (threadIdx.x == 0) sc.head[0] = (int)need;
     __syncthreads();
     for (int i = warp; i < n; i += kWarps) {
-        const int from = __ldcg(src + i), to = __ldcg(dst + i), len = __ldcg(c.lens + from), at = offsets[i];
+        const int from = srcs.at(i), to = dsts.at(i), len = i < kSmallList ? small_lens[i] : __ldcg(c.lens + from), at = offsets[i];
         const int kept = share ? len / c.page_tokens : 0;           // pages that both hold
         for (int p = kept + lane; p < pages_of(c, len); p += 32) {  // copies: until the source is known to be a page, of the copy itself
             const int fresh = list[at + p - kept];

@@ -142,7 +142,8 @@ class KvCache:
         be, n, width = self.be, seqs.shape[0], self.kv_heads * self.head_dim
         ids, at = self._ints("seqs", seqs, n), self._ints("cu", cu, n + 1)
         if out is None:
-            k, v = torch.empty((2, rows, width), dtype=dtype, device=be.device).unbind(0)
+            k = torch.empty((rows, width), dtype=dtype, device=be.device)
+            v = k.new_empty((rows, width))
             ld_k = ld_v = width
         else:
             k, v = out

@@ -213,6 +213,33 @@ def test_a_large_pool(be):
     be.status_poll()
 
 
+def test_long_lists_over_many_sequences(be):
+    """Lists longer than a block has threads, more sequences than marks fit shared memory, and ids listed twice in them."""
+    n, max_seqs = 2500, 40000
+    c, m = both(be, n_pages=9000, max_seqs=max_seqs, max_pages=6, page=16, kv=1, hd=64)
+    rng = np.random.default_rng(7)
+    ids = [int(i) for i in rng.permutation(max_seqs)[:2 * n]]
+    src, dst = ids[:n], ids[n:]
+    lens = [int(x) for x in rng.integers(0, 50, n)]
+    c.extend(i32(src), i32(lens)), m.extend(src, lens)
+    same_tables(c, m)
+    c.fork(i32(src), i32(dst)), m.fork(src, dst, True)
+    same_tables(c, m)
+    for bad in (src[:2000] + src[700:701], src[:2000] + [max_seqs]):
+        c.truncate(i32(bad)), m.truncate(bad)
+        same_tables(c, m)
+    c.fork(i32(src[:1500] + src[:1]), i32(dst[:1501])), m.fork(src[:1500] + src[:1], dst[:1501], True)      # in use
+    same_tables(c, m)
+    to = [x // 2 for x in lens]
+    c.truncate(i32(dst), i32(to)), m.truncate(dst, to)
+    same_tables(c, m)
+    c.truncate(i32(src)), m.truncate(src)
+    same_tables(c, m)
+    c.compact(), m.compact()
+    same_tables(c, m)
+    be.status_poll()
+
+
 def test_refused_operations_change_nothing_and_say_why(be):
     from tensorpencil_b200 import _lib
     c, m = both(be, n_pages=5, max_seqs=4, max_pages=4, kv=1)
