@@ -180,6 +180,10 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
+    if (warp == 8 && lane < 3) {
+        const CUtensorMap *map = lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
 
@@ -200,7 +204,24 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int tiles = max(tiles_a, tiles_b);
     const int look_from = (pos0 + 1) / kTile;           // first tile of keys that tile A's first token does not see as a whole
 
-    if (threadIdx.x == 0) {
+    // The first loads leave before anything else is set up: they take longer than all of it.
+    const auto load_q = [&](int x) {
+        mbar_arrive_expect_tx(q_full(x), (uint32_t)(L::kAtoms * 128 * p.tile_tokens * p.group));
+        for (int a = 0; a < L::kAtoms; a++)
+            tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, head * p.group,
+                        start + pos0 + x * p.tile_tokens);
+    };
+    const auto load_k = [&](int j) {
+        mbar_arrive_expect_tx(k_full(j % kStages), L::kAtoms * kAtomBytes);
+        for (int a = 0; a < L::kAtoms; a++)
+            tma_load_3d(smem_base + L::kK + (j % kStages * L::kAtoms + a) * kAtomBytes, &map_k, k_full(j % kStages), a * 64, head, start + j * kTile);
+    };
+    const auto load_v = [&](int j) {
+        mbar_arrive_expect_tx(v_full(j % kStages), L::kAtoms * kAtomBytes);
+        for (int a = 0; a < L::kAtoms; a++)
+            tma_load_3d(smem_base + L::kV + (j % kStages * L::kAtoms + a) * kAtomBytes, &map_v, v_full(j % kStages), a * 64, head, start + j * kTile);
+    };
+    if (warp == 8 && lane == 0) {
         for (int s = 0; s < 2; s++) {
             mbar_init(q_full(s), 1);
             mbar_init(k_full(s), 1);
@@ -216,6 +237,10 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         *abort_flag = 0;
         *any_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        load_q(0);
+        load_k(0);
+        if (tiles_b > 0) load_q(1);
+        load_v(0);
     }
     for (int i = threadIdx.x; i < 3 * HD; i += kThreads) bad[i] = INT_MAX;
     // Rows of a tile of queries that hold no token (128 / group has a remainder): zeros, or an infinity left there would move their reference
@@ -333,28 +358,15 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (warp == 8) {
             // ---------------- TMA ----------------
             if (lane == 0) {
-                const uint32_t q_bytes = (uint32_t)(L::kAtoms * 128 * p.tile_tokens * p.group);
-                const auto load_q = [&](int x) {
-                    mbar_arrive_expect_tx(q_full(x), q_bytes);
-                    for (int a = 0; a < L::kAtoms; a++)
-                        tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, head * p.group,
-                                    start + pos0 + x * p.tile_tokens);
-                };
-                load_q(0);
-                for (int j = 0; ok && j < tiles; j++) {
+                for (int j = 1; ok && j < tiles; j++) {
                     const int st = j % kStages;
                     const uint32_t ph = (uint32_t)(j / kStages) & 1u;
                     ok = mbar_wait(k_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x10u | st, true);
                     if (!ok) break;
-                    mbar_arrive_expect_tx(k_full(st), L::kAtoms * kAtomBytes);
-                    for (int a = 0; a < L::kAtoms; a++)
-                        tma_load_3d(smem_base + L::kK + (st * L::kAtoms + a) * kAtomBytes, &map_k, k_full(st), a * 64, head, start + j * kTile);
-                    if (j == 0 && tiles_b > 0) load_q(1);
+                    load_k(j);
                     ok = mbar_wait(v_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x20u | st, true);
                     if (!ok) break;
-                    mbar_arrive_expect_tx(v_full(st), L::kAtoms * kAtomBytes);
-                    for (int a = 0; a < L::kAtoms; a++)
-                        tma_load_3d(smem_base + L::kV + (st * L::kAtoms + a) * kAtomBytes, &map_v, v_full(st), a * 64, head, start + j * kTile);
+                    load_v(j);
                 }
             }
         } else if (warp == 9) {
