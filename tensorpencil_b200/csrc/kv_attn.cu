@@ -8,8 +8,8 @@
 //     would of a tcgen05 tile of 128 rows.  The cached values are exact in f16.
 //   - f32 accuracy (SPLIT) for f32 and f16 rows: q = hi + lo in f16 (after scaling the row by a power of two), and the weights likewise, two
 //     products each.  bf16 queries are exact in one f16 term, and weights of one f16 term (2^-12) are below a bf16 result's half step (2^-9).
-//   - K's int8 goes into the product as it is: byte ^ 0x80 in the low byte of an f16 is the number (128 + k) 2^-24, and the sum's start value
-//     takes the 128 sum(q) off again (a fixed number a row).  V's cancels less well over a long sequence and is converted exactly.
+//   - For bf16 rows K's int8 goes into the product as it is: byte ^ 0x80 in the low byte of an f16 is the number (128 + k) 2^-24, and the
+//     sum's start value takes the 128 sum(q) off again (a fixed number a row).  V's cancels less well over a long sequence and is converted exactly.
 //   - Page scales are uniform over a piece of 16 tokens (a page holds 16, 32 or 64): ks multiplies scores, vs the weights.
 //   - A warp owns its data path: K and V of 16 or 32 tokens a step by cp.async into a ring of its own, no barrier between warps, and the next
 //     run's first step is on its way while a run's sums are merged.  Bytes lie in shared memory with their 16-byte pieces
@@ -232,19 +232,21 @@ __device__ __forceinline__ uint32_t s8_pair_raw(uint32_t w) {
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(b) : "r"(w), "r"(0x00ff00ffu), "r"(0x00800080u));
     return b;
 }
-// Four consecutive bytes of K as the two registers of a k step, times kPerUnitOfK: bytes (0, 2), (1, 3) of s8, (0, 1), (2, 3) of e4m3.
-template <int FORMAT>
+// Four consecutive bytes of K as the two registers of a k step, times kPerUnitOfK: bytes (0, 2), (1, 3) of s8, (0, 1), (2, 3) of e4m3.  RAW: as
+// 128 + k, for one instruction less a pair; the sums are then several times the scores, and f32 results lose a bit or two (16 sequences
+// of 3000 tokens, five drafted each: 1.9e-6 off instead of 1.0e-6).
+template <int FORMAT, bool RAW>
 __device__ __forceinline__ void k_regs(uint32_t w, uint32_t &b0, uint32_t &b1) {
     if constexpr (FORMAT == TPB_KV_S8) {
-        b0 = s8_pair_raw(w);
-        b1 = s8_pair_raw(w >> 8);
+        b0 = RAW ? s8_pair_raw(w) : s8_pair(w);
+        b1 = RAW ? s8_pair_raw(w >> 8) : s8_pair(w >> 8);
     } else {
         b0 = e4m3_pair<0>(w);
         b1 = e4m3_pair<1>(w);
     }
 }
-template <int FORMAT>
-constexpr float kPerUnitOfK = FORMAT == TPB_KV_S8 ? 16777216.0f : 1.0f;        // 2^24
+template <int FORMAT, bool RAW>
+constexpr float kPerUnitOfK = FORMAT == TPB_KV_S8 && RAW ? 16777216.0f : 1.0f;        // 2^24
 // Four columns of V for two tokens: v[e] = (a's byte e, b's byte e).
 template <int FORMAT>
 __device__ __forceinline__ void v_regs(uint32_t a, uint32_t b, uint32_t (&v)[4]) {
@@ -499,7 +501,7 @@ kv_attention_kernel(const AttnParams p) {
                     }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                sum *= FORMAT == TPB_KV_S8 ? -128.0f / 16777216.0f : 0.0f;
+                sum *= FORMAT == TPB_KV_S8 && !SPLIT ? -128.0f / 16777216.0f : 0.0f;
             };
             if constexpr (C::kQRegs) {
 #pragma unroll
@@ -589,7 +591,7 @@ kv_attention_kernel(const AttnParams p) {
                             uint32_t a[2][2];
 #pragma unroll
                             for (int j = 0; j < 2; j++)
-                                k_regs<FORMAT>(k4 == 0 ? w[h][j].x : k4 == 1 ? w[h][j].y : k4 == 2 ? w[h][j].z : w[h][j].w, a[j][0], a[j][1]);
+                                k_regs<FORMAT, !SPLIT>(k4 == 0 ? w[h][j].x : k4 == 1 ? w[h][j].y : k4 == 2 ? w[h][j].z : w[h][j].w, a[j][0], a[j][1]);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -620,7 +622,7 @@ kv_attention_kernel(const AttnParams p) {
                         mx[e] = mxw[e] = -INFINITY;
 #pragma unroll
                         for (int h = 0; h < H; h++) {
-                            f[e][h] = ks[h] * r_s * kPerUnitOfK<FORMAT>;
+                            f[e][h] = ks[h] * r_s * kPerUnitOfK<FORMAT, !SPLIT>;
                             if (hide) {
 #pragma unroll
                                 for (int j = 0; j < 2; j++)
