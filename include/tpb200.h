@@ -461,7 +461,7 @@ int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t
  * A cache is memory that the caller owns, described by a tpb_kv_cache (a plain struct, read during each call; the calls below
  * keep nothing of it).  All pointers are device memory:
  *   k, v              [layers][n_pages][kv_heads][page_tokens][head_dim], one byte a value, 16-byte aligned
- *   k_scale, v_scale  [layers][n_pages][kv_heads] f32: a value stands for q * scale.  A block -- the tokens of one page, one head -- has one scale
+ *   k_scale, v_scale  [layers][n_pages][kv_heads] f32: a value stands for q * scale, scale >= 0.  A block -- the tokens of one page, one head -- has one
  *   table             [max_seqs][max_pages] the pages of each sequence, in order; -1 behind them
  *   lens              [max_seqs] tokens of each sequence (0 = the sequence is free)
  *   tail              [max_seqs] tokens that the last tpb_kv_extend gave the sequence; 0 after a truncation or a fork
@@ -488,7 +488,7 @@ typedef struct tpb_kv_cache {
     int32_t kv_heads;
     int32_t page_tokens;  /* 16, 32 or 64 */
     int32_t head_dim;     /* 64 or 128 */
-    int32_t max_seqs, max_pages;  /* max_pages * page_tokens below 2^31, max_seqs * max_pages below 2^31 */
+    int32_t max_seqs, max_pages;  /* max_pages * page_tokens at most 2^30, max_seqs * max_pages below 2^31 */
     int32_t format;       /* tpb_kv_format */
 } tpb_kv_cache;
 

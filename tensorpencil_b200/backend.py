@@ -333,7 +333,7 @@ class Backend:
                 and s[0] == tokens and t.get_device() == self._index):
             raise ValueError(f"attentionPacked: {name} must be [{tokens}][{width}] on {self.device}, contiguous within a row "
                              f"(got {tuple(s)}, strides {st})")
-        return st[0] if tokens > 1 else max(st[0], width)
+        return st[0] if tokens > 1 else width
 
     def _gemm(self, y: torch.Tensor, w_bytes: np.ndarray, weight_scale: np.ndarray, rows: int,
               w_bits: int, ldy: Optional[int] = None):

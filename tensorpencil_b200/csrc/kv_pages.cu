@@ -568,8 +568,8 @@ int tpb_kv::check_cache(tpb_handle_t h, const tpb_kv_cache *c, const char *what)
                   "%s: the cache's sizes must be positive, n_pages at most 2^24 and kv_heads below 65536", what);
     // token rows of the whole cache, and its table's entries, are counted in 32 bits
     TPB_CHECK_ARG(h, (__int128)c->layers * c->n_pages * c->kv_heads * c->page_tokens < ((int64_t)1 << 31) &&
-                         (int64_t)c->max_pages * c->page_tokens < ((int64_t)1 << 31) && (int64_t)c->max_seqs * c->max_pages < ((int64_t)1 << 31),
-                  "%s: the cache exceeds 2^31 rows or table entries", what);
+                         (int64_t)c->max_pages * c->page_tokens <= ((int64_t)1 << 30) && (int64_t)c->max_seqs * c->max_pages < ((int64_t)1 << 31),
+                  "%s: the cache exceeds 2^31 rows or table entries, or a sequence 2^30 tokens", what);
     return TPB_OK;
 }
 

@@ -107,13 +107,13 @@ class KvCache:
         width = heads * self.head_dim
         s, st = t.shape, t.stride()
         if t.dtype is dtype and len(s) == 2 and s[1] == width and st[1] == 1 and s[0] == rows and t.get_device() == self._index:
-            return st[0] if rows > 1 else max(st[0], width)
+            return st[0] if rows > 1 else width
         if t.dtype != dtype or dtype not in _ROWS:
             raise TypeError(f"{name} must be float32, bfloat16 or float16, like its partners (got {t.dtype})")
         if t.get_device() != self._index or s[0] != rows or not (
                 len(s) == 3 and s[1] == heads and s[2] == self.head_dim and st[2] == 1 and (st[1] == self.head_dim or heads == 1)):
             raise ValueError(f"{name} must be [{rows}][{width}] on {self.be.device}, contiguous within a row (got {tuple(s)}, strides {st})")
-        return st[0] if rows > 1 else max(st[0], width)
+        return st[0] if rows > 1 else width
 
     @staticmethod
     def _dtype(name: str, t: torch.Tensor) -> int:
