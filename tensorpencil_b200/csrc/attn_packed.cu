@@ -12,7 +12,19 @@
 // and B, of consecutive tokens: while the tensor pipe works for one, the other's softmax runs.
 //
 // Roles: warps 0-3 / 4-7 softmax and output of tile A / B, warp 8 TMA, warp 9 MMA, warps 10 and 11 look V over.  MMAs of one thread execute in
-// issue order, which is what frees the buffers: S_x(j+1) is issued after P_x(j) V(j).  Every wait is bounded.
+// issue order, which is what frees the buffers: S_x(j+1) is issued after P_x(j) V(j).  With head_dim 64 tensor memory has room for a P beside
+// S: there S_x(j+1) is issued as soon as S_x(j) is in registers (four prompts of 259 to 3001 tokens, 14 heads over 2: 46.5 -> 43.3 us).
+// Every wait is bounded.
+//
+// A CTA that has work goes on to the pairs of CTAs that have not started, one after another, asked for when the last tile of keys of its own pair
+// is loaded: the next pair's loads and first scores run under the last products and the output of the one before, where a CTA of its own
+// would spend 4 us on starting and ending.
+//
+// What bounds it: of a step of 3400 cycles (a tile of keys against both tiles of queries, head_dim 128) the tensor pipe is busy for 2050, the
+// special-function units for 2050; the rest is the way from one to the other -- scores out of tensor memory twice, weights back, four
+// barriers.  Measured (bf16, 32 heads over 8): 8192 tokens 454 us, 1210 TFLOP/s; nine prompts of 17 to 4093 tokens 93 us.  What
+// was measured and is not here: a pair of CTAs over tcgen05 cta_group::2, 705 us for the 8192 tokens; two threads a row, 503; a quarter of
+// the exponentials by a polynomial on the FMA pipe, 489; a grid of CTAs of one pair each, 467.
 //
 // What a row must not see.  Scores of later tokens, other sequences and rows past the end are replaced before the maximum and
 // their weights set to zero, so K's values there do not matter.  V's do, 0 * NaN being NaN: in the tiles that some row sees only a part of,
@@ -34,17 +46,20 @@ constexpr int kTile = 128;
 constexpr int kAtomBytes = 16384;     // [128 rows][64 values of 16 bits] in the 128-byte swizzle layout
 constexpr int kThreads = 384;
 constexpr int kStages = 2;
+constexpr int kPlaces = 256;          // places without rows that a CTA passes over at most, 1 to 2 us each
 constexpr float kLazy = 8.0f;         // the reference point moves when the maximum has grown by more than 2^8
 
 template <int HD>
 struct Layout {
     static constexpr int kAtoms = HD / 64;
+    static constexpr bool kApart = HD == 64;                              // P has columns of its own in tensor memory
     static constexpr int kQ = 0;                                          // tiles A, B
     static constexpr int kK = kQ + 2 * kAtoms * kAtomBytes;
     static constexpr int kV = kK + kStages * kAtoms * kAtomBytes;
     static constexpr int kBar = kV + kStages * kAtoms * kAtomBytes;
-    static constexpr int kBad = kBar + 256;                               // [3][HD] first NaN, +inf, -inf of a column
-    static constexpr int kBytes = kBad + 3 * HD * 4 + 1024;
+    static constexpr int kPair = kBar + 256;                              // two Pairs, then the answer to the request for another one
+    static constexpr int kBad = kPair + 128;                              // [2][3][HD] first NaN, +inf, -inf of a column, of every other pair
+    static constexpr int kBytes = kBad + 2 * 3 * HD * 4 + 1024;
 };
 
 struct PackedParams {
@@ -54,6 +69,7 @@ struct PackedParams {
     int n_seqs, tokens;
     int group, kv_heads, tile_tokens;      // query heads a kv head, 128 / group
     unsigned slots;
+    int take_more;                // there are more CTAs than SMs
     float scale_log2;
     uint32_t *status;
 };
@@ -82,19 +98,35 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     return r;
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
         : "memory");
+}
+__device__ __forceinline__ void tc_commit_one(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one)
+        : "memory");
+}
+// 1 in one lane of a warp.  The MMA warp stays together and only its instructions are that lane's: descriptors and addresses are then the same for
+// the whole warp and are kept where tcgen05.mma takes them from.  (A branch for lane 0 around all of it: 8192 tokens 481 us instead of 467.)
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
 }
 __device__ __forceinline__ void tc_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -154,6 +186,29 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
+// A pair of tiles of one kv head: what a CTA works on at a time.
+struct Pair {
+    int head, start, len, pos0;          // start < 0: there is no more
+};
+// Asks for a CTA of the grid that has not started yet; 16 bytes at `answer` say which (or that there is none) once `bar` has counted them.
+__device__ __forceinline__ void ask_next(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool read_next(uint32_t answer, uint32_t &block) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.b32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(ok), "=r"(block)
+        : "r"(answer)
+        : "memory");
+    return ok != 0;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -164,21 +219,29 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint8_t *gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t bars = smem_base + L::kBar;
     const auto q_full = [&](int x) { return bars + 8u * x; };
-    const auto k_full = [&](int s) { return bars + 8u * (2 + s); };
-    const auto k_empty = [&](int s) { return bars + 8u * (4 + s); };
-    const auto v_full = [&](int s) { return bars + 8u * (6 + s); };
-    const auto v_empty = [&](int s) { return bars + 8u * (8 + s); };
-    const auto v_seen = [&](int s) { return bars + 8u * (10 + s); };     // looked over
-    const auto s_full = [&](int x) { return bars + 8u * (12 + x); };
-    const auto p_half = [&](int x) { return bars + 8u * (14 + x); };     // the first 64 keys' weights
-    const auto p_full = [&](int x) { return bars + 8u * (16 + x); };
-    const auto o_done = [&](int x) { return bars + 8u * (18 + x); };
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBar + 192);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + L::kBar + 200);
-    volatile int *any_bad = reinterpret_cast<volatile int *>(gen + L::kBar + 204);
+    const auto q_empty = [&](int x) { return bars + 8u * (2 + x); };
+    const auto k_full = [&](int s) { return bars + 8u * (4 + s); };
+    const auto k_empty = [&](int s) { return bars + 8u * (6 + s); };
+    const auto v_full = [&](int s) { return bars + 8u * (8 + s); };
+    const auto v_empty = [&](int s) { return bars + 8u * (10 + s); };
+    const auto v_seen = [&](int s) { return bars + 8u * (12 + s); };     // looked over
+    const auto s_full = [&](int x) { return bars + 8u * (14 + x); };
+    const auto p_half = [&](int x) { return bars + 8u * (16 + x); };     // the first 64 keys' weights
+    const auto p_full = [&](int x) { return bars + 8u * (18 + x); };
+    const auto o_done = [&](int x) { return bars + 8u * (20 + x); };
+    const auto pair_full = [&](int i) { return bars + 8u * (22 + (i & 1)); };
+    const auto pair_empty = [&](int i) { return bars + 8u * (24 + (i & 1)); };
+    const uint32_t answered = bars + 8u * 26;
+    const auto s_read = [&](int x) { return smem_base + L::kPair + 64u + 8u * x; };     // kApart: the scores are in registers
+    const auto pv_done = [&](int x) { return smem_base + L::kPair + 80u + 8u * x; };    // kApart: the products of a tile of keys are in O
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBar + 232);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + L::kBar + 236);
+    volatile int *any_bad = reinterpret_cast<volatile int *>(gen + L::kBar + 240);      // [2]
+    const uint32_t answer = smem_base + L::kPair + 32;
+    Pair *pairs = reinterpret_cast<Pair *>(gen + L::kPair);
     int *bad = reinterpret_cast<int *>(gen + L::kBad);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);          // alike in a warp, and known to be
     const int lane = threadIdx.x & 31;
     if (warp == 8 && lane < 3) {
         const CUtensorMap *map = lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v;
@@ -187,43 +250,45 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
 
-    // Which rows.  Sequence s has at least as many places as it has pairs of tiles from cu[s] / (2 tile_tokens) + s on; the last tiles of a sequence,
-    // which see the most keys, come first.
-    const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
-    const int slot = (int)(p.slots - 1u - blockIdx.x / (unsigned)p.kv_heads);
+    // Which rows stand behind a block index.  Sequence s has at least as many places as it has pairs of tiles from cu[s] / (2 tile_tokens) + s on; the
+    // last tiles of a sequence, which see the most keys, come first.  start < 0: none.  A whole warp calls it.
     const int pair_tokens = 2 * p.tile_tokens;
-    const Found b = find_sequence(p.cu, nullptr, p.n_seqs, p.tokens, slot, [&](int i, int r) { return r / pair_tokens + i; });
-    const int seq = b.i, start = b.r0, len = b.r1 - b.r0;
-    const long long first = (long long)(slot - (start / pair_tokens + seq)) * pair_tokens;      // position of tile A's first token
-    if (first < 0 || first >= len) return;
-    const int pos0 = (int)first;
-    // keys that a tile's last token sees, and the tiles of keys they take; B may have no tokens at all
-    const int end_a = min(pos0 + p.tile_tokens, len), end_b = min(pos0 + pair_tokens, len);
-    const int tiles_a = (end_a + kTile - 1) / kTile;
-    const int tiles_b = end_b > end_a ? (end_b + kTile - 1) / kTile : 0;
-    const int tiles = max(tiles_a, tiles_b);
-    const int look_from = (pos0 + 1) / kTile;           // first tile of keys that tile A's first token does not see as a whole
+    const auto find_pair = [&](uint32_t block) {
+        const int slot = (int)(p.slots - 1u - block / (unsigned)p.kv_heads);
+        const Found b = find_sequence(p.cu, nullptr, p.n_seqs, p.tokens, slot, [&](int i, int r) { return r / pair_tokens + i; });
+        const long long first = (long long)(slot - (b.r0 / pair_tokens + b.i)) * pair_tokens;      // position of tile A's first token
+        const bool there = first >= 0 && first < b.r1 - b.r0;
+        return Pair{(int)(block % (unsigned)p.kv_heads), there ? b.r0 : -1, b.r1 - b.r0, there ? (int)first : 0};
+    };
+    // The tiles of keys that tile x's last token sees the end of; 0: x has no tokens.
+    const auto key_tiles = [&](const Pair &w, int x) {
+        const int from = w.pos0 + x * p.tile_tokens, end = min(from + p.tile_tokens, w.len);
+        return end > from ? (end + kTile - 1) / kTile : 0;
+    };
+    Pair now = find_pair(blockIdx.x);
+    if (now.start < 0) return;
 
-    // The first loads leave before anything else is set up: they take longer than all of it.
-    const auto load_q = [&](int x) {
+    // The first loads leave before anything else is set up: they take longer than all of it.  k and v stages are counted over all pairs.
+    const auto load_q = [&](const Pair &w, int x) {
         mbar_arrive_expect_tx(q_full(x), (uint32_t)(L::kAtoms * 128 * p.tile_tokens * p.group));
         for (int a = 0; a < L::kAtoms; a++)
-            tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, head * p.group,
-                        start + pos0 + x * p.tile_tokens);
+            tma_load_3d(smem_base + L::kQ + (x * L::kAtoms + a) * kAtomBytes, &map_q, q_full(x), a * 64, w.head * p.group,
+                        w.start + w.pos0 + x * p.tile_tokens);
     };
-    const auto load_k = [&](int j) {
-        mbar_arrive_expect_tx(k_full(j % kStages), L::kAtoms * kAtomBytes);
+    const auto load_k = [&](const Pair &w, int j, int st) {
+        mbar_arrive_expect_tx(k_full(st), L::kAtoms * kAtomBytes);
         for (int a = 0; a < L::kAtoms; a++)
-            tma_load_3d(smem_base + L::kK + (j % kStages * L::kAtoms + a) * kAtomBytes, &map_k, k_full(j % kStages), a * 64, head, start + j * kTile);
+            tma_load_3d(smem_base + L::kK + (st * L::kAtoms + a) * kAtomBytes, &map_k, k_full(st), a * 64, w.head, w.start + j * kTile);
     };
-    const auto load_v = [&](int j) {
-        mbar_arrive_expect_tx(v_full(j % kStages), L::kAtoms * kAtomBytes);
+    const auto load_v = [&](const Pair &w, int j, int st) {
+        mbar_arrive_expect_tx(v_full(st), L::kAtoms * kAtomBytes);
         for (int a = 0; a < L::kAtoms; a++)
-            tma_load_3d(smem_base + L::kV + (j % kStages * L::kAtoms + a) * kAtomBytes, &map_v, v_full(j % kStages), a * 64, head, start + j * kTile);
+            tma_load_3d(smem_base + L::kV + (st * L::kAtoms + a) * kAtomBytes, &map_v, v_full(st), a * 64, w.head, w.start + j * kTile);
     };
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < 2; s++) {
             mbar_init(q_full(s), 1);
+            mbar_init(q_empty(s), 1);
             mbar_init(k_full(s), 1);
             mbar_init(k_empty(s), 1);
             mbar_init(v_full(s), 1);
@@ -233,16 +298,25 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             mbar_init(p_half(s), 4);
             mbar_init(p_full(s), 4);
             mbar_init(o_done(s), 1);
+            if (L::kApart) {
+                mbar_init(s_read(s), 4);
+                mbar_init(pv_done(s), 1);
+            }
+            mbar_init(pair_full(s), 1);
+            mbar_init(pair_empty(s), 11);        // the softmax warps, the MMA warp, the two that look V over
+            any_bad[s] = 0;
         }
+        mbar_init(answered, 1);
         *abort_flag = 0;
-        *any_bad = 0;
+        pairs[0] = now;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        load_q(0);
-        load_k(0);
-        if (tiles_b > 0) load_q(1);
-        load_v(0);
+        mbar_arrive(pair_full(0));
+        load_q(now, 0);
+        load_k(now, 0, 0);
+        if (key_tiles(now, 1) > 0) load_q(now, 1);
+        load_v(now, 0, 0);
     }
-    for (int i = threadIdx.x; i < 3 * HD; i += kThreads) bad[i] = INT_MAX;
+    for (int i = threadIdx.x; i < 2 * 3 * HD; i += kThreads) bad[i] = INT_MAX;
     // Rows of a tile of queries that hold no token (128 / group has a remainder): zeros, or an infinity left there would move their reference
     // point tile after tile.
     const int used_rows = p.tile_tokens * p.group;
@@ -257,217 +331,366 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    // A softmax thread's row.  (Inside the branch below, the same lines cost nine registers too many: 8192 tokens 510 us with the spills, 487 without.)
-    const int x_of_warp = (warp >> 2) & 1;
-    const int row = (warp & 3) * 32 + lane;
-    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
-    const int pos = pos0 + x_of_warp * p.tile_tokens + row_tok;
-    const bool row_ok = row_tok < p.tile_tokens && pos < len;
-    const int lim = row_ok ? pos + 1 : 0;                        // keys that the row sees
-    const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_o = tmem_base + t_lane + 256u + (uint32_t)(x_of_warp * HD);
-    float l_run = 0.0f;
+    // Every role goes through the same pairs: the first is known, warp 8 tells of the others.
     bool ok = true;
+    const auto next_pair = [&](int i) {              // pair i > 0, for a warp of the other roles; false: no more
+        if (!p.take_more) return false;
+        ok = ok && mbar_wait(pair_full(i), (uint32_t)(i >> 1) & 1u, abort_flag, p.status, (16u << 24) | 1u, true);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return false;
+        now = pairs[i & 1];
+        return now.start >= 0;
+    };
+    const auto pair_over = [&](int i) {              // this warp is done with pair i
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair_empty(i));
+    };
 
     if (warp < 8) {
-        // ---------------- softmax: a thread per row ----------------
-        const int x = x_of_warp;
-        const int my_tiles = x ? tiles_b : tiles_a;
+        // ---------------- softmax and output: a thread per row ----------------
+        const int x = warp >> 2;
+        const int row = (warp & 3) * 32 + lane;
+        const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem_base + t_lane + (uint32_t)(x * 128);
-        float m_run = -3.402823466e38f;
-        const auto do_tile = [&](auto masked_tag, const int j) -> bool {
-            constexpr bool MASKED = decltype(masked_tag)::value;
-            const bool good = mbar_wait(s_full(x), (uint32_t)j & 1u, abort_flag, p.status, (14u << 24) | 1u, true);
-            if (!__all_sync(0xffffffffu, good)) return false;
-            tc_fence_after();
-            const int left = lim - j * kTile;                    // columns >= left are hidden
-            // The scores are read out of tensor memory twice, 32 columns ahead of their use: once for the maximum, once for the weights.
-            uint32_t v[2][32];
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tc_ld_32x32(t_s, v[0]);
+        const uint32_t t_o = tmem_base + t_lane + 256u + (uint32_t)(x * HD);
+        uint32_t phases = 0;                         // bit 0: of s_full, bit 1: of o_done
+        for (int i = 0; i == 0 || next_pair(i); i++) {
+            const int my_tiles = key_tiles(now, x);
+            // position of the row's token; of the warp's pair only this and the tiles stay in registers
+            const int pos = now.pos0 + x * p.tile_tokens + row_tok;
+            const int lim = row_tok < p.tile_tokens && pos < now.len ? pos + 1 : 0;        // keys that the row sees
+            float m_run = -3.402823466e38f, l_run = 0.0f;
+            const auto do_tile = [&](auto masked_tag, const int j) -> bool {
+                constexpr bool MASKED = decltype(masked_tag)::value;
+                const bool good = mbar_wait(s_full(x), phases & 1u, abort_flag, p.status, (14u << 24) | 1u, true);
+                phases ^= 1u;
+                if (!__all_sync(0xffffffffu, good)) return false;
+                tc_fence_after();
+                const int left = lim - j * kTile;                    // columns >= left are hidden
+                // The scores are read out of tensor memory twice, 32 columns ahead of their use: once for the maximum, once for the weights.
+                uint32_t v[2][32];
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tc_ld_32x32(t_s, v[0]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tc_wait_ld_dep(v[c & 1]);
-                tc_ld_32x32(t_s + (uint32_t)(((c + 1) & 3) * 32), v[(c + 1) & 1]);
+                for (int c = 0; c < 4; c++) {
+                    tc_wait_ld_dep(v[c & 1]);
+                    tc_ld_32x32(t_s + (uint32_t)(((c + 1) & 3) * 32), v[(c + 1) & 1]);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float a = !MASKED || c * 32 + i < left ? __uint_as_float(v[c & 1][i]) : -INFINITY;
-                    const float b = !MASKED || c * 32 + i + 1 < left ? __uint_as_float(v[c & 1][i + 1]) : -INFINITY;
-                    m4[(i >> 1) & 3] = fmaxf(fmaxf(m4[(i >> 1) & 3], a), b);
-                }
-            }
-            const float m_cand = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-            const float m_new = (m_cand > m_run + kLazy) ? m_cand : m_run;
-            const float alpha = ex2(m_run - m_new);
-            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                // O holds the products up to tile j - 1: s_full of tile j was committed behind them
-#pragma unroll 1
-                for (int c = 0; c < HD / 16; c++) {
-                    uint32_t o[16];
-                    tc_ld_16(t_o + (uint32_t)(c * 16), o);
-                    tc_wait_ld_16(o);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                    tc_st_16(t_o + (uint32_t)(c * 16), o);
-                }
-            }
-            const uint64_t c2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-m_new, -m_new);
-            uint64_t sum2[2] = {0ull, 0ull};
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t pk[16];
-                tc_wait_ld_dep(v[c & 1]);
-                if (c < 3) tc_ld_32x32(t_s + (uint32_t)((c + 1) * 32), v[(c + 1) & 1]);
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float a0, a1;
-                    unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), c2, nm2), a0, a1);
-                    float e0 = ex2(a0), e1 = ex2(a1);
-                    if (MASKED) {
-                        if (c * 32 + 2 * i >= left) e0 = 0.0f;
-                        if (c * 32 + 2 * i + 1 >= left) e1 = 0.0f;
+                    for (int e = 0; e < 32; e += 2) {
+                        const float a = !MASKED || c * 32 + e < left ? __uint_as_float(v[c & 1][e]) : -INFINITY;
+                        const float b = !MASKED || c * 32 + e + 1 < left ? __uint_as_float(v[c & 1][e + 1]) : -INFINITY;
+                        m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], a), b);
                     }
-                    sum2[i & 1] = add_f2(sum2[i & 1], pack_f2(e0, e1));
-                    pk[i] = pack2<T>(e0, e1);
                 }
-                tc_st_16(t_s + (uint32_t)(c * 16), pk);
-                if (c & 1) {
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(c == 1 ? p_half(x) : p_full(x));
+                const float m_cand = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+                const float m_new = (m_cand > m_run + kLazy) ? m_cand : m_run;
+                const float alpha = ex2(m_run - m_new);
+                // O holds the products up to tile j - 1, and their weights may be written over: s_full of tile j was committed behind them, or they
+                // are waited for
+                if (L::kApart && j > 0) {
+                    const bool there = mbar_wait(pv_done(x), phases & 1u, abort_flag, p.status, (14u << 24) | 2u, true);
+                    if (!__all_sync(0xffffffffu, there)) return false;
+                    tc_fence_after();
                 }
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; c++) {
+                        uint32_t o[16];
+                        tc_ld_16(t_o + (uint32_t)(c * 16), o);
+                        tc_wait_ld_16(o);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tc_st_16(t_o + (uint32_t)(c * 16), o);
+                    }
+                }
+                const uint64_t c2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-m_new, -m_new);
+                uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t pk[16];
+                    tc_wait_ld_dep(v[c & 1]);
+                    if (c < 3) tc_ld_32x32(t_s + (uint32_t)((c + 1) * 32), v[(c + 1) & 1]);
+                    if (L::kApart && c == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_read(x));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        float a0, a1;
+                        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c & 1][2 * e]), __uint_as_float(v[c & 1][2 * e + 1])), c2, nm2), a0, a1);
+                        float e0 = ex2(a0), e1 = ex2(a1);
+                        if (MASKED) {
+                            if (c * 32 + 2 * e >= left) e0 = 0.0f;
+                            if (c * 32 + 2 * e + 1 >= left) e1 = 0.0f;
+                        }
+                        sum2[e & 1] = add_f2(sum2[e & 1], pack_f2(e0, e1));
+                        pk[e] = pack2<T>(e0, e1);
+                    }
+                    tc_st_16(L::kApart ? tmem_base + t_lane + (uint32_t)(384 + x * 64 + c * 16) : t_s + (uint32_t)(c * 16), pk);
+                    if (c & 1) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(c == 1 ? p_half(x) : p_full(x));
+                    }
+                }
+                float s0, s1;
+                unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
+                l_run = l_run * alpha + (s0 + s1);
+                m_run = m_new;
+                return true;
+            };
+            // A tile of keys that the first token sees as a whole needs no mask: rows behind the last token, or behind the last whole token of the
+            // tile, come to nothing whatever they see.
+            const int whole = pos - row_tok + 1;
+            for (int j = 0; ok && j < my_tiles; j++) ok = (j + 1) * kTile <= whole ? do_tile(std::false_type{}, j) : do_tile(std::true_type{}, j);
+            if (ok && my_tiles > 0) {
+                ok = mbar_wait(o_done(x), phases >> 1, abort_flag, p.status, (14u << 24) | 3u, true);
+                phases ^= 2u;
+                ok = __all_sync(0xffffffffu, ok);
             }
-            float s0, s1;
-            unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
-            l_run = l_run * alpha + (s0 + s1);
-            m_run = m_new;
-            return true;
-        };
-        // A tile of keys that the first token sees as a whole needs no mask: rows behind the last token, or behind the last whole token of the tile,
-        // come to nothing whatever they see.
-        const int whole = pos0 + x * p.tile_tokens + 1;
-        for (int j = 0; ok && j < my_tiles; j++) ok = (j + 1) * kTile <= whole ? do_tile(std::false_type{}, j) : do_tile(std::true_type{}, j);
-        if (ok && my_tiles > 0) {
-            ok = mbar_wait(o_done(x), 0, abort_flag, p.status, (14u << 24) | 3u, true);
-            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (my_tiles > 0) {
+                tc_fence_after();
+                const float inv_l = 1.0f / l_run;
+                const Pair w = pairs[i & 1];
+                T *dst = static_cast<T *>(p.out) + (long long)(w.start + lim - 1) * p.ld_out + (long long)(w.head * p.group + row_head) * HD;
+                const bool fix = any_bad[i & 1] != 0;
+                const int *first_bad = bad + (i & 1) * 3 * HD;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t v[32];
+                    tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
+                    tc_wait_ld_dep(v);
+                    if (lim > 0) {
+                        if (fix) {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                float o = __uint_as_float(v[e]);
+                                const int col = c * 32 + e;
+                                if (lim > first_bad[col]) o += __uint_as_float(0x7fc00000u);
+                                if (lim > first_bad[HD + col]) o += INFINITY;
+                                if (lim > first_bad[2 * HD + col]) o -= INFINITY;
+                                v[e] = __float_as_uint(o);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int h = 0; h < 4; h++)
+                                o[h] = pack2<T>(__uint_as_float(v[8 * e + 2 * h]) * inv_l, __uint_as_float(v[8 * e + 2 * h + 1]) * inv_l);
+                            reinterpret_cast<uint4 *>(dst + c * 32)[e] = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();          // O is read: the next pair's first weights, which this warp hands over later, let it be overwritten
+            }
+            pair_over(i);
         }
-    } else {
-        if (warp == 8) {
-            // ---------------- TMA ----------------
+    } else if (warp == 8) {
+        // ---------------- TMA, and which pair comes next ----------------
+        uint32_t n_kv = 0, q_phase = 3u, n_asked = 0;         // bit x of q_phase: of q_empty
+        const auto ask = [&] {
+            mbar_arrive_expect_tx(answered, 16);
+            ask_next(answer, answered);
+        };
+        for (int i = 0; ok; i++) {
             if (lane == 0) {
-                for (int j = 1; ok && j < tiles; j++) {
-                    const int st = j % kStages;
-                    const uint32_t ph = (uint32_t)(j / kStages) & 1u;
+                for (int x = 0; ok && x < 2; x++) {
+                    if (key_tiles(now, x) == 0) continue;
+                    if (i > 0) {
+                        ok = mbar_wait(q_empty(x), (q_phase >> x) & 1u, abort_flag, p.status, (12u << 24) | 0x30u | x, true);
+                        if (ok) load_q(now, x);
+                    }
+                    q_phase ^= 1u << x;
+                }
+                const int tiles = max(key_tiles(now, 0), key_tiles(now, 1));
+                for (int j = 0; ok && j < tiles; j++, n_kv++) {
+                    // asked for no earlier than its loads need: a pair taken early waits here while another CTA has nothing to do
+                    if (p.take_more && j + 1 == tiles) ask();
+                    if (n_kv == 0) continue;                                       // left above
+                    const int st = (int)(n_kv % kStages);
+                    const uint32_t ph = (n_kv / kStages) & 1u;
                     ok = mbar_wait(k_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x10u | st, true);
                     if (!ok) break;
-                    load_k(j);
+                    load_k(now, j, st);
                     ok = mbar_wait(v_empty(st), ph ^ 1u, abort_flag, p.status, (12u << 24) | 0x20u | st, true);
                     if (!ok) break;
-                    load_v(j);
+                    load_v(now, j, st);
                 }
             }
-        } else if (warp == 9) {
-            // ---------------- MMA ----------------
-            if (lane == 0) {
-                const uint32_t idesc_qk = make_idesc<T>(kTile, false), idesc_pv = make_idesc<T>(HD, true);
-                const auto issue_qk = [&](int x, int t) {
-                    const uint32_t ka = smem_base + L::kK + (t % kStages) * L::kAtoms * kAtomBytes;
-                    const uint32_t qa = smem_base + L::kQ + x * L::kAtoms * kAtomBytes;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok || !p.take_more) break;
+            for (int places = 0;; places++) {
+                ok = mbar_wait(answered, n_asked++ & 1u, abort_flag, p.status, (12u << 24) | 0x40u, true);
+                ok = __all_sync(0xffffffffu, ok);
+                uint32_t block = 0;
+                const bool there = ok && read_next(answer, block);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // read before the next answer is written
+                now = {0, -1, 0, 0};
+                if (!there) break;
+                now = find_pair(block);
+                // A place without rows is passed over.  After many the CTA ends, and those that are left start as CTAs: nobody waits for long.
+                if (now.start >= 0 || places == kPlaces) break;
+                __syncwarp();
+                if (lane == 0) ask();
+                __syncwarp();
+            }
+            if (ok && i > 0) ok = mbar_wait(pair_empty(i + 1), (uint32_t)((i - 1) >> 1) & 1u, abort_flag, p.status, (12u << 24) | 0x50u, true);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int b = (i + 1) & 1;
+            if (any_bad[b]) {
+                for (int c = lane; c < 3 * HD; c += 32) bad[b * 3 * HD + c] = INT_MAX;
+                __syncwarp();
+                if (lane == 0) any_bad[b] = 0;
+            }
+            if (lane == 0) pairs[b] = now;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair_full(i + 1));
+            if (now.start < 0) break;
+        }
+    } else if (warp == 9) {
+        // ---------------- MMA ----------------
+        uint32_t n_kv = 0, x_phase = 0, q_phase = 0;             // tiles of keys so far; bit x: of p_half and p_full, of q_full
+        const uint32_t one = elect_one();
+        for (int i = 0; i == 0 || next_pair(i); i++) {
+            const auto wait = [&](uint32_t bar, uint32_t phase, uint32_t code) -> bool {
+                const bool good = mbar_wait(bar, phase, abort_flag, p.status, (13u << 24) | code);
+                return __all_sync(0xffffffffu, good);
+            };
+            const uint32_t idesc_qk = make_idesc<T>(kTile, false), idesc_pv = make_idesc<T>(HD, true);
+            const int tiles_a = __shfl_sync(0xffffffffu, key_tiles(now, 0), 0), tiles_b = __shfl_sync(0xffffffffu, key_tiles(now, 1), 0);
+            const int tiles = max(tiles_a, tiles_b);
+            const auto issue_qk = [&](int x, uint32_t n, bool last) {
+                const uint32_t ka = smem_base + L::kK + (n % kStages) * L::kAtoms * kAtomBytes;
+                const uint32_t qa = smem_base + L::kQ + x * L::kAtoms * kAtomBytes;
 #pragma unroll
-                    for (int a = 0; a < L::kAtoms; a++) {
-                        const uint64_t qd = make_kmajor_sw128_desc(qa + a * kAtomBytes), kd = make_kmajor_sw128_desc(ka + a * kAtomBytes);
+                for (int a = 0; a < L::kAtoms; a++) {
+                    const uint64_t qd = make_kmajor_sw128_desc(qa + a * kAtomBytes), kd = make_kmajor_sw128_desc(ka + a * kAtomBytes);
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++)
-                            tc_mma_ss(tmem_base + (uint32_t)(x * 128), qd + 2u * kk, kd + 2u * kk, idesc_qk, (a | kk) ? 1u : 0u);
-                    }
-                    tc_commit(s_full(x));
-                };
-                const auto issue_pv = [&](int x, int t, int part) {
-                    const uint64_t vd = make_mn_major_desc(smem_base + L::kV + (t % kStages) * L::kAtoms * kAtomBytes);
-#pragma unroll
-                    for (int k2 = 0; k2 < 4; k2++) {
-                        const int kk = 4 * part + k2;           // 16 keys: 8 columns of P, 2048 bytes of V
-                        tc_mma_ts(tmem_base + 256u + (uint32_t)(x * HD), tmem_base + (uint32_t)(x * 128 + 8 * kk), vd + 128u * kk, idesc_pv,
-                                  (t > 0 || kk > 0) ? 1u : 0u);
-                    }
-                };
-                ok = mbar_wait(q_full(0), 0, abort_flag, p.status, (13u << 24) | 1u);
-                if (ok) ok = mbar_wait(k_full(0), 0, abort_flag, p.status, (13u << 24) | 2u);
-                if (ok) {
-                    tc_fence_after();
-                    issue_qk(0, 0);
-                    if (tiles_b > 0) {
-                        ok = mbar_wait(q_full(1), 0, abort_flag, p.status, (13u << 24) | 9u);
-                        if (ok) issue_qk(1, 0);
-                    }
-                    tc_commit(k_empty(0));
+                    for (int kk = 0; kk < 4; kk++)
+                        tc_mma_ss(one, tmem_base + (uint32_t)(x * 128), qd + 2u * kk, kd + 2u * kk, idesc_qk, (a | kk) ? 1u : 0u);
                 }
-                for (int j = 0; ok && j < tiles; j++) {
-                    const int st = j % kStages;
-                    const bool more = j + 1 < tiles;
-                    ok = mbar_wait(v_seen(st), (uint32_t)(j / kStages) & 1u, abort_flag, p.status, (13u << 24) | 3u);
-                    bool k_there = false;
-                    for (int x = 0; ok && x < 2; x++) {
-                        const int mine = x ? tiles_b : tiles_a;
-                        if (j < mine) {
-                            ok = mbar_wait(p_half(x), (uint32_t)j & 1u, abort_flag, p.status, (13u << 24) | 4u);
+                tc_commit_one(one, s_full(x));
+                if (last) tc_commit_one(one, q_empty(x));
+            };
+            const auto issue_pv = [&](int x, int j, int part) {
+                const uint64_t vd = make_mn_major_desc(smem_base + L::kV + ((n_kv + j) % kStages) * L::kAtoms * kAtomBytes);
+#pragma unroll
+                for (int k2 = 0; k2 < 4; k2++) {
+                    const int kk = 4 * part + k2;           // 16 keys: 8 columns of P, 2048 bytes of V
+                    tc_mma_ts(one, tmem_base + 256u + (uint32_t)(x * HD), tmem_base + (uint32_t)((L::kApart ? 384 + x * 64 : x * 128) + 8 * kk),
+                              vd + 128u * kk, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                }
+            };
+            ok = ok && wait(q_full(0), q_phase & 1u, 1u);
+            q_phase ^= 1u;
+            if (ok) ok = wait(k_full(n_kv % kStages), (n_kv / kStages) & 1u, 2u);
+            if (ok) {
+                tc_fence_after();
+                issue_qk(0, n_kv, tiles_a == 1);
+                if (tiles_b > 0) {
+                    ok = wait(q_full(1), q_phase >> 1, 9u);
+                    q_phase ^= 2u;
+                    if (ok) issue_qk(1, n_kv, tiles_b == 1);
+                }
+                tc_commit_one(one, k_empty(n_kv % kStages));
+            }
+            for (int j = 0; ok && j < tiles; j++) {
+                const uint32_t n = n_kv + j, st = n % kStages, st1 = (n + 1) % kStages;
+                const bool more = j + 1 < tiles;
+                ok = wait(v_seen(st), (n / kStages) & 1u, 3u);
+                bool k_there = false;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    if (!ok) break;
+                    const int mine = x ? tiles_b : tiles_a;
+                    if (j < mine) {
+                        ok = wait(p_half(x), (x_phase >> x) & 1u, 4u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(x, j, 0);
+                        if (L::kApart && j + 1 < mine) {
+                            ok = wait(s_read(x), (x_phase >> x) & 1u, 7u);
                             if (!ok) break;
                             tc_fence_after();
-                            issue_pv(x, j, 0);
-                            ok = mbar_wait(p_full(x), (uint32_t)j & 1u, abort_flag, p.status, (13u << 24) | 5u);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_pv(x, j, 1);
-                            if (j + 1 == mine) tc_commit(o_done(x));
-                        }
-                        if (x == 1) tc_commit(v_empty(st));
-                        if (j + 1 < mine) {
                             if (!k_there) {
-                                ok = mbar_wait(k_full((j + 1) % kStages), (uint32_t)((j + 1) / kStages) & 1u, abort_flag, p.status, (13u << 24) | 6u);
+                                ok = wait(k_full(st1), ((n + 1) / kStages) & 1u, 6u);
                                 if (!ok) break;
                                 tc_fence_after();
                                 k_there = true;
                             }
-                            issue_qk(x, j + 1);
+                            issue_qk(x, n + 1, j + 2 == mine);
                         }
+                        ok = wait(p_full(x), (x_phase >> x) & 1u, 5u);
+                        x_phase ^= 1u << x;
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_pv(x, j, 1);
+                        if (L::kApart) tc_commit_one(one, pv_done(x));
+                        if (j + 1 == mine) tc_commit_one(one, o_done(x));
                     }
-                    if (ok && more) tc_commit(k_empty((j + 1) % kStages));
+                    if (x == 1) tc_commit_one(one, v_empty(st));
+                    if (!L::kApart && j + 1 < mine) {
+                        if (!k_there) {
+                            ok = wait(k_full(st1), ((n + 1) / kStages) & 1u, 6u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            k_there = true;
+                        }
+                        issue_qk(x, n + 1, j + 2 == mine);
+                    }
                 }
+                if (ok && more) tc_commit_one(one, k_empty(st1));
             }
-        } else {
-            // ---------------- V: warps 10 and 11, half of a tile's rows each ----------------
-            constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;      // exponent all ones: NaN or infinity
-            constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-            for (int j = 0; ok && j < tiles; j++) {
-                const int st = j % kStages;
-                ok = mbar_wait(v_full(st), (uint32_t)(j / kStages) & 1u, abort_flag, p.status, (15u << 24) | 1u, true);
+            n_kv += tiles;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            pair_over(i);
+        }
+    } else {
+        // ---------------- V: warps 10 and 11, half of a tile's rows each ----------------
+        constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;      // exponent all ones: NaN or infinity
+        constexpr uint32_t kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+        uint32_t n_kv = 0;
+        for (int i = 0; i == 0 || next_pair(i); i++) {
+            const int tiles = max(key_tiles(now, 0), key_tiles(now, 1));
+            const int look_from = (now.pos0 + 1) / kTile;           // first tile of keys that tile A's first token does not see as a whole
+            int *first_bad = bad + (i & 1) * 3 * HD;
+            for (int j = 0; ok && j < tiles; j++, n_kv++) {
+                const int st = (int)(n_kv % kStages);
+                ok = mbar_wait(v_full(st), (n_kv / kStages) & 1u, abort_flag, p.status, (15u << 24) | 1u, true);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (j >= look_from) {
                     for (int a = 0; a < L::kAtoms; a++) {
                         const uint32_t base = smem_base + L::kV + (st * L::kAtoms + a) * kAtomBytes + (uint32_t)(warp - 10) * (kAtomBytes / 2);
 #pragma unroll 4
-                        for (int i = lane; i < kAtomBytes / 32; i += 32) {
-                            const uint4 w = ld_shared_v4(base + 16u * i);
+                        for (int c = lane; c < kAtomBytes / 32; c += 32) {
+                            const uint4 w = ld_shared_v4(base + 16u * c);
                             const uint32_t hit = (((w.x & kExp) + kOne) | ((w.y & kExp) + kOne) | ((w.z & kExp) + kOne) | ((w.w & kExp) + kOne)) & 0x80008000u;
                             if (hit) {
-                                const int row = (warp - 10) * 64 + i / 8, key = j * kTile + row;
-                                const int col0 = a * 64 + ((i & 7) ^ (row & 7)) * 8;
+                                const int row = (warp - 10) * 64 + c / 8, key = j * kTile + row;
+                                const int col0 = a * 64 + ((c & 7) ^ (row & 7)) * 8;
                                 uint32_t u[4] = {w.x, w.y, w.z, w.w};
                                 for (int e = 0; e < 8; e++) {
                                     const uint32_t h = (u[e >> 1] >> (16 * (e & 1))) & 0xffffu, ex = kExp & 0xffffu;
                                     if ((h & ex) != ex) continue;
-                                    if (key < len) {
+                                    if (key < now.len) {
                                         const int kind = (h & ~(ex | 0x8000u) & 0xffffu) != 0 ? 0 : (h & 0x8000u) ? 2 : 1;
-                                        atomicMin(bad + kind * HD + col0 + e, key);
-                                        *any_bad = 1;
+                                        atomicMin(first_bad + kind * HD + col0 + e, key);
+                                        any_bad[i & 1] = 1;
                                     }
                                     u[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
                                 }
-                                st_shared_v4(base + 16u * i, u[0], u[1], u[2], u[3]);
+                                st_shared_v4(base + 16u * c, u[0], u[1], u[2], u[3]);
                             }
                         }
                     }
@@ -476,42 +699,8 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_seen(st));
             }
-        }
-    }
-
-    // ---------------- output ----------------
-    if (warp < 8 && ok && (x_of_warp ? tiles_b : tiles_a) > 0) {
-        tc_fence_after();
-        const float inv_l = 1.0f / l_run;
-        T *dst = static_cast<T *>(p.out) + (long long)(start + pos) * p.ld_out + (long long)(head * p.group + row_head) * HD;
-        const bool fix = *any_bad != 0;
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; c++) {
-            uint32_t v[32];
-            tc_ld_32x32(t_o + (uint32_t)(c * 32), v);
-            tc_wait_ld_dep(v);
-            if (row_ok) {
-                if (fix) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        float o = __uint_as_float(v[i]);
-                        const int col = c * 32 + i;
-                        if (lim > bad[col]) o += __uint_as_float(0x7fc00000u);
-                        if (lim > bad[HD + col]) o += INFINITY;
-                        if (lim > bad[2 * HD + col]) o -= INFINITY;
-                        v[i] = __float_as_uint(o);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        w[e] = pack2<T>(__uint_as_float(v[8 * i + 2 * e]) * inv_l, __uint_as_float(v[8 * i + 2 * e + 1]) * inv_l);
-                    reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-            __syncwarp();
+            if (!ok) break;
+            pair_over(i);
         }
     }
 
@@ -588,6 +777,7 @@ int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t
     const int64_t slots = tokens / (2 * p.tile_tokens) + n_seqs;
     TPB_CHECK_ARG(h, slots * kv_heads < INT32_MAX, "attention_packed: tokens * heads exceeds the grid");
     p.slots = (unsigned)slots;
+    p.take_more = slots * kv_heads > h->sm_count;
     tpb_device_guard guard(h->device);
     TPB_CUDA(h, guard.err);
     CUtensorMap mq, mk, mv;

@@ -192,3 +192,34 @@ def test_no_tokens_and_no_sequences(be):
     out = torch.full((5, 256), 2.0, dtype=torch.bfloat16).cuda()
     be.attentionPacked(q, k, v, offsets([]), 4, 2, 64, out=out)
     assert (out == 2.0).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_more_pairs_of_tiles_than_the_gpu_has_sms(be, hd):
+    """Pairs of tiles that follow one another in one block: each sequence's rows come out as they do alone, with and without NaN and infinities that
+    some of its rows see, whatever the pair before it saw."""
+    rng = np.random.default_rng(hd)
+    heads, kv = 16, 8
+    lens = [int(n) for n in rng.choice([1, 60, 129, 300, 411], 90)]
+    q, k, v = make(sum(lens), heads, kv, hd, "bf16", 21)
+    starts = np.cumsum([0] + lens)
+    for i in range(0, 90, 3):
+        v[starts[i] + int(rng.integers(0, lens[i])), int(rng.integers(0, kv * hd))] = (float("nan"), float("inf"), -float("inf"))[i // 3 % 3]
+    out = be.attentionPacked(q, k, v, offsets(lens), heads, kv, hd)
+    be.status_poll()
+    for i, n in enumerate(lens):
+        rows = slice(int(starts[i]), int(starts[i]) + n)
+        alone = be.attentionPacked(q[rows], k[rows], v[rows], offsets([n]), heads, kv, hd)
+        assert torch.equal(torch.isnan(out[rows]), torch.isnan(alone))
+        assert torch.equal(torch.nan_to_num(out[rows]), torch.nan_to_num(alone)), (i, n)
+    assert torch.isnan(out).any() and torch.isinf(out).any()
+
+
+def test_tens_of_thousands_of_sequences_without_tokens(be):
+    """More of them than a block passes over on its way to work."""
+    heads, kv, hd = 8, 8, 64
+    lens = [150] + [0] * 30000 + [70] + [0] * 30000 + [129, 300]
+    q, k, v = make(sum(lens), heads, kv, hd, "f16", 22)
+    out = be.attentionPacked(q, k, v, offsets(lens), heads, kv, hd)
+    be.status_poll()
+    check(out, q, k, v, [n for n in lens if n], heads, kv, hd, "f16", rows_at_most=30)
