@@ -112,7 +112,7 @@ int tpb_status_poll(tpb_handle_t h, tpb_stream_t stream, uint32_t *detail) {
     if (detail) *detail = word;
     if (word != 0) {
         TPB_CUDA(h, cudaMemsetAsync(h->d_status, 0, 4, st));
-        if ((word >> 24) >= 32u)
+        if ((word >> 24) == 32u)
             return tpb_fail(h, TPB_ERR_STATE, "a key / value cache does not fit the call: %s (status 0x%08x)",
                             (word & 15u) == 1 ? "sequence id out of range" : (word & 15u) == 2 ? "page out of range"
                             : (word & 15u) == 3 ? "length out of range" : "rows are not those of the last extension", word);
