@@ -18,6 +18,9 @@
 //   - The work of all (sequence, kv head, row tile)s is one line of units of tokens, cut into equal pieces, one a CTA.  A CTA that has
 //     not all of a sequence's tokens leaves a partial result; a second kernel joins them in the order of the tokens, so the
 //     result is the same from run to run.
+// Measured (32 heads over 8 of 128): 131000 tokens, int8, bf16 rows 55 us (the cache's 268 MB at the rate of a plain copy: 41.5), 48 sequences of 1 to 16000
+// tokens, e4m3, 75 us (62), one of 200 tokens 7.5 us; five drafted tokens of 16 sequences, 16 heads over 4 of 64, f32 rows: 25 us, a chain of about five
+// steps a warp.  Steps of 16 tokens with four CTAs an SM took 132 us where 32 with three took 102 (the 48 sequences), rings of 24 KB with two 131.
 //
 // Softmax.  Per row two running references, both whole numbers in log2 units so that every rescaling is exact: ms >= max s - kLazy for the sum
 // l = sum 2^(s - ms), and mw for the weights w = 2^(s + log2 vs - mw + kUp), whose size depends on the page's scale as well.
@@ -812,7 +815,7 @@ kv_attention_kernel(const AttnParams p) {
 
 // Joins the partial results of the run that CTA blockIdx.x of the kernel above began and did not end.  Its time is a chain of loads behind the end of
 // that kernel (starting it costs 1 us, a note 0.8), so a thread asks for references, sums and its share of the weighted values all
-// at once, before anything is known of their factors: 131000 tokens 10 us with one dependent load behind another, 5 drafted tokens 25.
+// at once, before anything is known of their factors: 131000 tokens 6 us, five drafted tokens 6; with one dependent load behind another 10 and 25.
 constexpr int kJoinThreads = 512;
 constexpr int kJoinAhead = 8;        // parts of which a thread holds four dimensions
 constexpr int kJoinFactors = 2048;   // (part, row) pairs of a pass

@@ -31,12 +31,17 @@ constexpr float kLimit = FORMAT == TPB_KV_S8 ? 127.0f : 448.0f;
 // each -- which is why one warp a CTA looks the sequence up, why a CTA of a prompt goes over several blocks behind one look-up, and why
 // what a step of the chain brings is asked for before anything is decided.
 //
+// DENSE: 64 registers a thread, 1024 threads an SM whatever the block's size, for more CTAs than the SMs hold at 72 (two pieces, one CTA) or 96 (four pieces,
+// three).  Measured with the rows read back: 8384 tokens in four prompts, 8 heads of 128, bf16 to e4m3, pages of 64 30.9 -> 27.7 us; 1541 tokens, which need
+// no second round, 11.5, and 12.4 with it.  One piece a thread (pages of 16): a CTA of eight groups, or, with more pages than SMs, two of four,
+// one of which looks up while the other copies: 38.5 -> 32.7 us; f32 45.9 -> 38.9.
+//
 // Grid x: sequence i has at least as many places as it can touch pages from cu[i] / page_tokens + 2 i on, so that a CTA finds its
 // sequence by a search and the launch needs no lengths on the host.
 template <int CHUNKS>
 constexpr int kAppendGroups = CHUNKS <= 1 ? 8 : CHUNKS == 2 ? 4 : 2;
-template <typename T, int FORMAT, int HD, int CHUNKS>
-__global__ void __launch_bounds__(128 * kAppendGroups<CHUNKS>)
+template <typename T, int FORMAT, int HD, int CHUNKS, bool DENSE>
+__global__ void __launch_bounds__(128 * kAppendGroups<CHUNKS>, DENSE ? 8 / kAppendGroups<CHUNKS> : 1)
 kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, const T *v, int64_t ld_v, const int32_t *seqs, const int32_t *cu,
                  int n_seqs, int rows, uint32_t *status) {
     constexpr int GROUPS = kAppendGroups<CHUNKS>;
@@ -163,83 +168,68 @@ kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, cons
     }
 }
 
-// A warp has `per_warp` consecutive rows: looks up the sequence of the first, asks for the pages of all, and then goes over them with 16 values a lane and
-// step, keys and values, four steps' loads in flight.  More rows a warp spare the look-ups (8500 rows at one a warp: 8500 warps in line at the same few
-// words of L2), fewer keep more of them under way.
+// A warp a row: looks its sequence and page up and goes over it with 16 values a lane and step, keys and values, four steps' loads in flight.
+// Measured: 8384 rows of 8 heads of 128, e4m3 to bf16, behind the append of the same: 27.3 us for both, 16 of them bytes at a copy's rate; with four CTAs an
+// SM 28.2, with six 33 (the loads in flight no longer fit the registers); several rows a warp, one after the other: two 1 us more, four 9.
 template <typename T, int FORMAT, int HD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 kv_read_kernel(const tpb_kv_cache c, int layer, T *k, int64_t ld_k, T *v, int64_t ld_v, const int32_t *seqs, const int32_t *start,
-               const int32_t *cu, int n_seqs, int rows, int per_warp, uint32_t *status) {
+               const int32_t *cu, int n_seqs, int rows, uint32_t *status) {
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
     const int lane = threadIdx.x & 31, shift = __ffs(c.page_tokens) - 1;
-    const int first = ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) * per_warp, end = min(first + per_warp, rows);
-    const int pieces = c.kv_heads * (HD / 16);
-    for (int r = first; r < end;) {
-        const Found b = find_sequence(cu, seqs, n_seqs, rows, r, [&](int, int r0) { return r0; });
-        const int stop = b.r0 > r ? min(b.r0, end) : b.r1 > r ? min(b.r1, end) : end;     // rows r .. stop - 1 share the answer
-        if (b.r0 > r || b.r1 <= r) {                                                     // rows of no sequence
-            r = stop;
-            continue;
+    const int r = (int)blockIdx.x * 8 + (int)(threadIdx.x >> 5);
+    if (r >= rows) return;
+    const Found b = find_sequence(cu, seqs, n_seqs, rows, r, [&](int, int r0) { return r0; });
+    if (b.r0 > r || b.r1 <= r) return;                       // a row of no sequence
+    if (b.seq < 0 || b.seq >= c.max_seqs) {
+        report(status, kBadSeq);
+        return;
+    }
+    const int from = start ? __ldcg(start + b.i) : 0, len = __ldcg(c.lens + b.seq);
+    const long long pos = (long long)from + (r - b.r0);
+    const bool inside = from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens;       // behind the end: zeros
+    int page = 0;
+    if (inside) {
+        page = __ldcg(c.table + (size_t)b.seq * c.max_pages + (pos >> shift));
+        if (page < 0 || page >= c.n_pages) {
+            report(status, kBadPage);
+            return;
         }
-        if (b.seq < 0 || b.seq >= c.max_seqs) {
-            report(status, kBadSeq);
-            r = stop;
-            continue;
-        }
-        const int from = start ? __ldcg(start + b.i) : 0, len = __ldcg(c.lens + b.seq);
-        // the pages of the rows, a lane a row: -1 = behind the end (zeros), -2 = not a page (left as it is)
-        int page_of_lane = -1;
-        if (r + lane < stop) {
-            const long long pos = (long long)from + (r + lane - b.r0);
-            if (from >= 0 && pos < len && pos < (long long)c.max_pages * c.page_tokens) {
-                page_of_lane = __ldcg(c.table + (size_t)b.seq * c.max_pages + (pos >> shift));
-                if (page_of_lane < 0 || page_of_lane >= c.n_pages) {
-                    report(status, kBadPage);
-                    page_of_lane = -2;
-                }
+    }
+    const int pieces = c.kv_heads * (HD / 16), slot = (int)pos & (c.page_tokens - 1);
+    const size_t block0 = ((size_t)layer * c.n_pages + page) * c.kv_heads;
+    constexpr int kAhead = 4;
+    for (int p0 = lane; p0 < 2 * pieces; p0 += 32 * kAhead) {
+        uint4 w[kAhead];
+        float scale[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            const int p = p0 + 32 * a;
+            if (inside && p < 2 * pieces) {
+                const bool is_v = p >= pieces;
+                const int q = is_v ? p - pieces : p, head = q / (HD / 16), d = q % (HD / 16) * 16;
+                scale[a] = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
+                w[a] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(is_v ? c.v : c.k) +
+                                                              ((block0 + head) * c.page_tokens + slot) * HD + d));
             }
         }
-        for (int e = r; e < stop; e++) {
-            const int page = __shfl_sync(0xffffffffu, page_of_lane, e - r);
-            if (page == -2) continue;
-            const bool inside = page >= 0;
-            const int slot = (from + (e - b.r0)) & (c.page_tokens - 1);
-            const size_t block0 = ((size_t)layer * c.n_pages + max(page, 0)) * c.kv_heads;
-            constexpr int kAhead = 4;
-            for (int p0 = lane; p0 < 2 * pieces; p0 += 32 * kAhead) {
-                uint4 w[kAhead];
-                float scale[kAhead];
 #pragma unroll
-                for (int a = 0; a < kAhead; a++) {
-                    const int p = p0 + 32 * a;
-                    if (inside && p < 2 * pieces) {
-                        const bool is_v = p >= pieces;
-                        const int q = is_v ? p - pieces : p, head = q / (HD / 16), d = q % (HD / 16) * 16;
-                        scale[a] = __ldcg((is_v ? c.v_scale : c.k_scale) + block0 + head);
-                        w[a] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(is_v ? c.v : c.k) +
-                                                                      ((block0 + head) * c.page_tokens + slot) * HD + d));
-                    }
-                }
+        for (int a = 0; a < kAhead; a++) {
+            const int p = p0 + 32 * a;
+            if (p >= 2 * pieces) break;
+            const bool is_v = p >= pieces;
+            const int q = is_v ? p - pieces : p;
+            float f[16] = {};
+            if (inside) {
+                const uint32_t u[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
 #pragma unroll
-                for (int a = 0; a < kAhead; a++) {
-                    const int p = p0 + 32 * a;
-                    if (p >= 2 * pieces) break;
-                    const bool is_v = p >= pieces;
-                    const int q = is_v ? p - pieces : p;
-                    float f[16] = {};
-                    if (inside) {
-                        const uint32_t u[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
+                for (int i = 0; i < 4; i++) unpack4<FORMAT>(u[i], &f[4 * i]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) unpack4<FORMAT>(u[i], &f[4 * i]);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) f[i] *= scale[a];
-                    }
-                    store16((is_v ? v + (int64_t)e * ld_v : k + (int64_t)e * ld_k) + (int64_t)q * 16, f);
-                }
+                for (int i = 0; i < 16; i++) f[i] *= scale[a];
             }
+            store16((is_v ? v + (int64_t)r * ld_v : k + (int64_t)r * ld_k) + (int64_t)q * 16, f);
         }
-        r = stop;
     }
 }
 
@@ -277,21 +267,31 @@ int tpb_kv_append(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, in
     TPB_CUDA(h, guard.err);
     const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        const auto launch = [&](auto kern, int groups) {
-            // as many CTAs a page as two rounds of two an SM have room for: with more, each waits through a look-up of its own
-            const int64_t items = rows / c->page_tokens + 2 * (int64_t)n_seqs;
+        const int64_t items = rows / c->page_tokens + 2 * (int64_t)n_seqs;
+        // as many CTAs a page as two rounds of two an SM have room for: with more, each waits through a look-up of its own
+        const auto ctas_of = [&](int groups) {
             const int rounds = (2 * c->kv_heads + groups - 1) / groups;
-            const int64_t y = std::max<int64_t>(1, std::min<int64_t>(rounds, 4 * (int64_t)h->sm_count / items));
-            return tpb_launch_pdl(kern, dim3((unsigned)items, (unsigned)y), dim3(128u * (unsigned)groups), 0, (cudaStream_t)stream, *c, layer, (const T *)k,
-                                  ld_k, (const T *)v, ld_v, seqs, cu, n_seqs, (int)rows, h->d_status);
+            return std::max<int64_t>(1, std::min<int64_t>(rounds, 4 * (int64_t)h->sm_count / items));
+        };
+        const auto launch = [&](auto kern, int groups) {
+            return tpb_launch_pdl(kern, dim3((unsigned)items, (unsigned)ctas_of(groups)), dim3(128u * (unsigned)groups), 0, (cudaStream_t)stream, *c, layer,
+                                  (const T *)k, ld_k, (const T *)v, ld_v, seqs, cu, n_seqs, (int)rows, h->d_status);
         };
         const auto by_chunks = [&](auto fmt) {
             constexpr int F = decltype(fmt)::value;
             const int chunks = c->page_tokens * c->head_dim / 2048;             // 0 (half the threads have a piece) .. 4
-            if (c->head_dim == 64)
-                return chunks <= 1 ? launch(kv_append_kernel<T, F, 64, 1>, kAppendGroups<1>) : launch(kv_append_kernel<T, F, 64, 2>, kAppendGroups<2>);
-            return chunks <= 1 ? launch(kv_append_kernel<T, F, 128, 1>, kAppendGroups<1>)
-                               : chunks <= 2 ? launch(kv_append_kernel<T, F, 128, 2>, kAppendGroups<2>) : launch(kv_append_kernel<T, F, 128, 4>, kAppendGroups<4>);
+            const auto by_load = [&](auto hd, auto n) {
+                constexpr int HD = decltype(hd)::value, N = decltype(n)::value, G = kAppendGroups<N>;
+                if constexpr (N == 1) return launch(kv_append_kernel<T, F, HD, 1, false>, items > h->sm_count ? G / 2 : G);
+                else if constexpr (sizeof(T) == 4) return launch(kv_append_kernel<T, F, HD, N, false>, G);
+                else return items * ctas_of(G) > (N == 2 ? 1 : 3) * (int64_t)h->sm_count ? launch(kv_append_kernel<T, F, HD, N, true>, G)
+                                                                                       : launch(kv_append_kernel<T, F, HD, N, false>, G);
+            };
+            const std::integral_constant<int, 1> one;
+            const std::integral_constant<int, 2> two;
+            if (c->head_dim == 64) return chunks <= 1 ? by_load(std::integral_constant<int, 64>{}, one) : by_load(std::integral_constant<int, 64>{}, two);
+            const std::integral_constant<int, 128> hd;
+            return chunks <= 1 ? by_load(hd, one) : chunks <= 2 ? by_load(hd, two) : by_load(hd, std::integral_constant<int, 4>{});
         };
         return c->format == TPB_KV_S8 ? by_chunks(std::integral_constant<int, TPB_KV_S8>{}) : by_chunks(std::integral_constant<int, TPB_KV_E4M3>{});
     });
@@ -311,9 +311,8 @@ int tpb_kv_read(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, int 
     const cudaError_t e = by_dtype(dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         const auto launch = [&](auto kern) {
-            const int per_warp = rows > 32 * (int64_t)h->sm_count ? 2 : 1;
-            return tpb_launch_pdl(kern, dim3((unsigned)((rows + 8 * per_warp - 1) / (8 * per_warp))), dim3(256), 0, (cudaStream_t)stream, *c, layer, (T *)k, ld_k,
-                                  (T *)v, ld_v, seqs, start, cu, n_seqs, (int)rows, per_warp, h->d_status);
+            return tpb_launch_pdl(kern, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, *c, layer, (T *)k, ld_k, (T *)v, ld_v, seqs, start,
+                                  cu, n_seqs, (int)rows, h->d_status);
         };
         if (c->format == TPB_KV_S8) return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_S8, 64>) : launch(kv_read_kernel<T, TPB_KV_S8, 128>);
         return c->head_dim == 64 ? launch(kv_read_kernel<T, TPB_KV_E4M3, 64>) : launch(kv_read_kernel<T, TPB_KV_E4M3, 128>);
