@@ -566,3 +566,38 @@ def test_a_captured_step_replays_while_the_lengths_grow(be):
         same_tables(c, m)
         same_values(c, m)
         check_attention(c, m, out, q, [2, 0], [1, 1], heads, "f32")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("page,hd,total", [(16, 128, 4100), (16, 64, 4100), (32, 128, 3100), (64, 128, 8300), (64, 64, 4100)])
+def test_long_prompts_are_cached_as_short_ones_are(be, page, hd, total, dt):
+    """More pages than the GPU takes at once: the bytes and scales of a batch are those of its sequences one at a time, a page or two a call."""
+    from tensorpencil_b200.kv_cache import KvCache
+    kv, lens = 8, [total // 2, 5, total // 3, total - total // 2 - total // 3 - 5]
+    rng = np.random.default_rng(total + hd)
+    k, v = (values(rng, total, kv, hd, dt) for _ in "kv")
+    seqs, cu = i32(range(4)), offsets(lens)
+    made = []
+    for whole in (True, False):
+        c = KvCache(be, 1, total // page + 8, kv, hd, 4, total // page + 4, page, "s8")
+        c.extend(seqs, i32([3, 1, 0, 7]))                  # the prompts begin inside a page
+        c.append(0, k[:11], v[:11], seqs, offsets([3, 1, 0, 7]))
+        if whole:
+            c.extend(seqs, i32(lens))
+            c.append(0, k, v, seqs, cu)
+        else:
+            at = 0
+            for s, n in enumerate(lens):
+                done, held = 0, [3, 1, 0, 7][s]
+                while done < n:                            # up to the end of the page, so that every block is rounded the same number of times
+                    part = min(n - done, 2 * page - (held + done) % page)
+                    c.extend(i32([s]), i32([part]))
+                    c.append(0, k[at + done:at + done + part], v[at + done:at + done + part], i32([s]), i32([0, part]))
+                    done += part
+                at += n
+        c.check()
+        made.append(c.read(0, seqs, offsets([a + b for a, b in zip(lens, [3, 1, 0, 7])]), total + 11, dtype=torch.float32))
+    assert torch.equal(made[0][0], made[1][0]) and torch.equal(made[0][1], made[1][1])
+    # the last to come to a block were rounded once: off by half a step, and a step is at most 2 amax / 127 (the first page's tokens before them are k's too)
+    got, want = made[0][0].view(-1, kv, hd)[3:3 + lens[0]], k[:lens[0]].float()
+    assert ((got - want).abs() <= want.abs().max() / 127 * 1.000001).all()
