@@ -9,7 +9,7 @@
 //
 // Rows.  A tile's 128 rows are (token, query head of the group) pairs of one kv head: 128 / g tokens x g heads.  All of a group's heads
 // share the K and V tiles, and short prompts fill a tile g times sooner than with one head a tile.  A CTA has two such tiles, A
-// and B, of consecutive tokens: while the tensor pipe works for one, the other's softmax runs.
+// and B, of consecutive tokens: while the tensor pipe works for one, the other's softmax runs.  (Or one, in a small batch.)
 //
 // Roles: warps 0-3 / 4-7 softmax and output of tile A / B, warp 8 TMA, warp 9 MMA, warps 10 and 11 look V over.  MMAs of one thread execute in
 // issue order, which is what frees the buffers: S_x(j+1) is issued after P_x(j) V(j).  With head_dim 64 tensor memory has room for a P beside
@@ -69,6 +69,7 @@ struct PackedParams {
     int n_seqs, tokens;
     int group, kv_heads, tile_tokens;      // query heads a kv head, 128 / group
     unsigned slots;
+    int tiles;                    // of queries that a CTA has: 2 (A, B), or only A
     int take_more;                // there are more CTAs than SMs
     float scale_log2;
     uint32_t *status;
@@ -250,9 +251,9 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     tpb_grid_dep_launch();
     tpb_grid_dep_wait();
 
-    // Which rows stand behind a block index.  Sequence s has at least as many places as it has pairs of tiles from cu[s] / (2 tile_tokens) + s on; the
+    // Which rows stand behind a block index.  Sequence s has at least as many places as it has pairs of tiles from cu[s] / pair_tokens + s on; the
     // last tiles of a sequence, which see the most keys, come first.  start < 0: none.  A whole warp calls it.
-    const int pair_tokens = 2 * p.tile_tokens;
+    const int pair_tokens = p.tiles * p.tile_tokens;
     const auto find_pair = [&](uint32_t block) {
         const int slot = (int)(p.slots - 1u - block / (unsigned)p.kv_heads);
         const Found b = find_sequence(p.cu, nullptr, p.n_seqs, p.tokens, slot, [&](int i, int r) { return r / pair_tokens + i; });
@@ -263,7 +264,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // The tiles of keys that tile x's last token sees the end of; 0: x has no tokens.
     const auto key_tiles = [&](const Pair &w, int x) {
         const int from = w.pos0 + x * p.tile_tokens, end = min(from + p.tile_tokens, w.len);
-        return end > from ? (end + kTile - 1) / kTile : 0;
+        return end > from && x < p.tiles ? (end + kTile - 1) / kTile : 0;
     };
     Pair now = find_pair(blockIdx.x);
     if (now.start < 0) return;
@@ -774,7 +775,13 @@ int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t
     p.tile_tokens = kTile / p.group;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = h->d_status;
-    const int64_t slots = tokens / (2 * p.tile_tokens) + n_seqs;
+    // Two tiles share a CTA, whose steps are longer for it, where there is work for all SMs.  Where the SMs have room for all tiles at once, each has a
+    // CTA of its own; also up to two a SM if the sequences are long, since the early tiles are soon done with.  Measured (two tiles / one; head_dim 128,
+    // bf16): 1595 tokens, 8 heads over 1 29.5 / 24.7 us; 2048 tokens, 16 over 2 36.8 / 31.4; 1024 tokens, 32 over 4 22.4 / 21.9; twice 400 tokens, 32 over 8
+    // 13.3 / 14.7.
+    const int64_t alone = tokens / p.tile_tokens + n_seqs;
+    p.tiles = alone * kv_heads <= (tokens >= 1024 * (int64_t)n_seqs ? 2 : 1) * h->sm_count ? 1 : 2;
+    const int64_t slots = p.tiles == 1 ? alone : tokens / (2 * p.tile_tokens) + n_seqs;
     TPB_CHECK_ARG(h, slots * kv_heads < INT32_MAX, "attention_packed: tokens * heads exceeds the grid");
     p.slots = (unsigned)slots;
     p.take_more = slots * kv_heads > h->sm_count;

@@ -223,3 +223,19 @@ def test_tens_of_thousands_of_sequences_without_tokens(be):
     out = be.attentionPacked(q, k, v, offsets(lens), heads, kv, hd)
     be.status_poll()
     check(out, q, k, v, [n for n in lens if n], heads, kv, hd, "f16", rows_at_most=30)
+
+
+@pytest.mark.parametrize("lens,heads,kv,hd,dt", [([900, 129, 1, 0, 255, 700, 64], 16, 8, 128, "f16"), ([333, 700, 18, 19, 512], 14, 2, 64, "f16"),
+                                                ([1500, 2, 1030], 12, 4, 128, "bf16"), ([260] * 9, 33, 3, 64, "bf16"), ([130] * 12, 8, 8, 64, "f16")])
+def test_large_batches_give_the_bits_of_small_ones(be, lens, heads, kv, hd, dt):
+    """Two tiles of queries a block, or one where the batch is small: the same rows either way, and the formula's."""
+    times = 6
+    q, k, v = make(sum(lens) * times, heads, kv, hd, dt, sum(lens))
+    out = be.attentionPacked(q, k, v, offsets(lens * times), heads, kv, hd)
+    be.status_poll()
+    at = 0
+    for n in lens * times:
+        rows = slice(at, at + n)
+        assert torch.equal(out[rows], be.attentionPacked(q[rows], k[rows], v[rows], offsets([n]), heads, kv, hd)), n
+        at += n
+    check(out, q, k, v, lens, heads, kv, hd, dt, rows_at_most=20)
