@@ -816,6 +816,8 @@ kv_attention_kernel(const AttnParams p) {
 // Joins the partial results of the run that CTA blockIdx.x of the kernel above began and did not end.  Its time is a chain of loads behind the end of
 // that kernel (starting it costs 1 us, a note 0.8), so a thread asks for references, sums and its share of the weighted values all
 // at once, before anything is known of their factors: 131000 tokens 6 us, five drafted tokens 6; with one dependent load behind another 10 and 25.
+// Grid y: from 16 rows of 128 on two CTAs share the rows (20000 tokens, 16 rows a kv head 26.2 -> 23.5 us for both kernels, 32 rows 46.6 -> 38.3); with fewer
+// values the second CTA costs more than it takes over (five drafted tokens, 20 rows of 64, 25.6 -> 26.7).
 constexpr int kJoinThreads = 512;
 constexpr int kJoinAhead = 8;        // parts of which a thread holds four dimensions
 constexpr int kJoinFactors = 2048;   // (part, row) pairs of a pass
@@ -831,11 +833,12 @@ __global__ void __launch_bounds__(kJoinThreads, 2) kv_attention_join_kernel(cons
     const JoinNote *from = reinterpret_cast<const JoinNote *>(p.notes) + c0;
     const int rows = __ldcg(&from->rows), n = __ldcg(&from->last_cta) - c0 + 1, row_tile = __ldcg(&from->row_tile), head = __ldcg(&from->head);
     const long long out_row = __ldcg(&from->out_row);
-    // few rows: four threads share a row's dimensions, each with every fourth part
-    const int shares = rows * 4 <= kGroups ? 4 : 1;
-    const int rows_at_once = min(min(kGroups / shares, 32), max(kJoinFactors / max(n, 1), 1));
+    // few rows: four threads (or two) share a row's dimensions, each with every fourth part
+    const int each = (rows + (int)gridDim.y - 1) / (int)gridDim.y;
+    const int shares = each * 4 <= kGroups ? 4 : each * 2 <= kGroups ? 2 : 1;
+    const int rows_at_once = min(min(min(kGroups / shares, 32), max(each, 1)), max(kJoinFactors / max(n, 1), 1));
     const int lane4 = threadIdx.x % kLanes, group = threadIdx.x / kLanes, share = group % shares, rl = group / shares;
-    for (int r0 = 0; r0 < rows; r0 += rows_at_once) {
+    for (int r0 = (int)blockIdx.y * rows_at_once; r0 < rows; r0 += (int)gridDim.y * rows_at_once) {
         const int rg = min(rows_at_once, rows - r0);
         const bool mine = rl < rg;
         const auto load_o = [&](int c) {
@@ -935,7 +938,7 @@ int launch_attention(tpb_handle_t h, cudaStream_t st, const AttnParams &p) {
     const int ctas = h->sm_count * C::kCtas;
     TPB_CUDA(h, tpb_launch_pdl(kv_attention_kernel<HD, FORMAT, SPLIT, NT>, dim3((unsigned)ctas), dim3(kThreads), (size_t)C::kSmem, st, p));
     if (!p.whole)
-        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)ctas), dim3(kJoinThreads), 0, st, p));
+        TPB_CUDA(h, tpb_launch_pdl(kv_attention_join_kernel<HD, C::kRows>, dim3((unsigned)ctas, HD == 128 && NT >= 2 ? 2 : 1), dim3(kJoinThreads), 0, st, p));
     return TPB_OK;
 }
 

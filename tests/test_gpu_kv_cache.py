@@ -601,3 +601,10 @@ def test_long_prompts_are_cached_as_short_ones_are(be, page, hd, total, dt):
     # the last to come to a block were rounded once: off by half a step, and a step is at most 2 amax / 127 (the first page's tokens before them are k's too)
     got, want = made[0][0].view(-1, kv, hd)[3:3 + lens[0]], k[:lens[0]].float()
     assert ((got - want).abs() <= want.abs().max() / 127 * 1.000001).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("new,heads,kv", [(4, 4, 1), (6, 8, 2), (8, 4, 1)])
+def test_many_rows_over_a_long_cache(be, new, heads, kv, dt):
+    """16 to 32 rows a kv head, joined from parts by two blocks."""
+    test_attention_matches_the_formula(be, [5000, 700], new, heads, kv, 128, 64, dt, "s8")
