@@ -511,7 +511,7 @@ int tpb_kv_fork(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c, cons
 int tpb_kv_compact(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c);
 
 /* A batch names sequences (seqs[i], each at most once) and rows of a packed tensor: sequence seqs[i] owns the rows cu[i] .. cu[i+1] - 1 (cu:
- * n_seqs + 1 ascending offsets).  dtype: TPB_F32, TPB_BF16 or TPB_F16; rows ld elements apart, 16-byte aligned.
+ * n_seqs + 1 ascending offsets; rows ahead of cu[0] and from cu[n_seqs] on are nobody's).  dtype: TPB_F32, TPB_BF16 or TPB_F16; rows ld elements apart, 16-byte aligned.
  *
  * append   quantises the rows of k and v into the last cu[i+1] - cu[i] places of the sequence, which must be as many as its tail.  A block's
  *          scale is the smallest power of two, at least 2^-100, with amax <= limit * scale (limit: s8 127, e4m3 448) over the values that

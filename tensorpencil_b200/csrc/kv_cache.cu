@@ -81,10 +81,10 @@ kv_append_kernel(const tpb_kv_cache c, int layer, const T *k, int64_t ld_k, cons
     const int r0 = s_found[1], n_new = s_found[2], seq = s_found[3], len = s_found[4];
     if (len < 0) return;
     const int first = len - n_new;
-    const long long pg = (long long)(first >> shift) + (x - ((r0 >> shift) + 2 * s_found[0]));
-    if (pg * pt >= len) return;
+    const int pg = page_at_place(x, s_found[0], r0, first, len, shift);
+    if (pg < 0) return;
     const int page = __ldcg(c.table + (size_t)seq * c.max_pages + pg);
-    const int p0 = (int)pg * pt;                                // position of the page's first slot
+    const int p0 = pg * pt;                                // position of the page's first slot
     const int held = max(first - p0, 0), fill = min(len - p0, pt);   // slots [0, held) hold earlier tokens, [held, fill) are written
     const int blocks = 2 * c.kv_heads, stride = (int)gridDim.y * (int)(blockDim.x >> 7);
     int flip = 0;

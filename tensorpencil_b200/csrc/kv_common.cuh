@@ -29,6 +29,15 @@ __host__ __device__ inline Scratch scratch_of(const tpb_kv_cache &c) {
     return s;
 }
 
+// The page of its sequence's row of the table that place x of an append's launch stands for, where the search gave sequence i: rows from r0 on, tokens
+// first .. len - 1 new.  Its places begin at r0 / page_tokens + 2 i; -1: a place in front of them (rows ahead of the batch's first sequence: the search
+// knows no earlier one) or behind its last page.
+__host__ __device__ inline int page_at_place(int x, int i, int r0, int first, int len, int shift) {
+    const int at = x - ((r0 >> shift) + 2 * i);
+    const long long pg = (long long)(first >> shift) + at;
+    return at >= 0 && (pg << shift) < len ? (int)pg : -1;
+}
+
 // codes of the handle's status word (tpb_status_poll): role 32 = a cache that does not fit the call
 constexpr uint32_t kBadSeq = (32u << 24) | 1u, kBadPage = (32u << 24) | 2u, kBadLen = (32u << 24) | 3u, kBadTail = (32u << 24) | 4u;
 

@@ -2,7 +2,10 @@
 points get a zeroed stand-in for a handle, which they only write their message to, and the Python methods CPU tensors.  Also the index
 arithmetic that the kernels' launches rely on."""
 import ctypes as C
+import os
 import random
+import shutil
+import subprocess
 
 import pytest
 
@@ -205,3 +208,49 @@ def test_tables_of_a_scratch_hold_every_list():
     lib = _lib.load()
     for pages, seqs in ((1, 1), (17, 3), (70001, 1300)):
         assert lib.tpb_kv_scratch_bytes(pages, seqs) // 4 == 8 + seqs + seqs + pages + pages
+
+
+@pytest.fixture(scope="module")
+def page_at_place(tmp_path_factory):
+    """The kernel's own arithmetic, compiled for the host."""
+    gxx, cuda = shutil.which("g++"), "/usr/local/cuda/include"
+    if gxx is None or not os.path.isdir(cuda):
+        pytest.skip("no g++ / CUDA headers")
+    root, at = os.path.dirname(os.path.dirname(os.path.abspath(__file__))), tmp_path_factory.mktemp("places")
+    src, out = at / "places.cpp", at / "places.so"
+    src.write_text('#include "kv_common.cuh"\n'
+                   'extern "C" int at(int x, int i, int r0, int first, int len, int shift) { return tpb_kv::page_at_place(x, i, r0, first, len, shift); }\n')
+    r = subprocess.run([gxx, "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(root, "include"), "-I",
+                        os.path.join(root, "tensorpencil_b200", "csrc"), "-I", cuda, str(src), "-o", str(out)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-4000:]
+    return C.CDLL(str(out)).at
+
+
+def test_every_new_page_has_one_place_and_no_place_another_page(page_at_place):
+    """Over the whole grid of an append, with rows of nobody ahead of the first sequence and behind the last: the pages that a sequence's new tokens touch
+    come up once each, and nothing else does (no entry in front of the sequence's row of the table, none of an earlier page)."""
+    rnd = random.Random(5)
+    for trial in range(300):
+        shift, n = rnd.choice([4, 5, 6]), rnd.randint(1, 6)
+        page = 1 << shift
+        lead = [0, 1, page - 1, page, 3 * page, 40 * page + 5][trial % 6]
+        new = [rnd.choice([0, 1, rnd.randint(0, 5 * page)]) for _ in range(n)]
+        cu = [lead + sum(new[:i]) for i in range(n + 1)]
+        first = [rnd.choice([0, 0, rnd.randint(0, 10 * page)]) for _ in range(n)]
+        rows = cu[n] + rnd.choice([0, 1, 2 * page])
+        seen = [[] for _ in range(n)]
+        for x in range(rows // page + 2 * n):
+            i = max([0] + [j for j in range(n) if cu[j] // page + 2 * j <= x])      # the kernel's search: sequence 0 where there is none
+            if new[i] == 0:
+                continue
+            pg = page_at_place(x, i, cu[i], first[i], first[i] + new[i], shift)
+            if pg != -1:
+                seen[i].append(pg)
+        for i in range(n):
+            assert seen[i] == (list(range(first[i] // page, (first[i] + new[i] - 1) // page + 1)) if new[i] else [])
+    assert page_at_place(0, 0, 48, 0, 1, 4) == -1 and page_at_place(3, 0, 48, 0, 1, 4) == 0
+    # offsets out of order, which a call may not have, lead nowhere else either
+    for _ in range(2000):
+        shift, first, n_new = rnd.choice([4, 5, 6]), rnd.randint(0, 1 << 29), rnd.randint(1, 1 << 20)
+        pg = page_at_place(rnd.randint(0, 1 << 23), rnd.randint(0, 1 << 22), rnd.randint(0, 1 << 26), first, first + n_new, shift)
+        assert pg == -1 or first >> shift <= pg <= (first + n_new - 1) >> shift

@@ -608,3 +608,32 @@ def test_long_prompts_are_cached_as_short_ones_are(be, page, hd, total, dt):
 def test_many_rows_over_a_long_cache(be, new, heads, kv, dt):
     """16 to 32 rows a kv head, joined from parts by two blocks."""
     test_attention_matches_the_formula(be, [5000, 700], new, heads, kv, 128, 64, dt, "s8")
+
+
+@pytest.mark.parametrize("fmt,dt", [("s8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("page,hd", [(16, 64), (16, 128), (32, 64), (64, 128)])
+@pytest.mark.parametrize("lead", [(0, 1), (1, 0), (2, 0), (7, 5)])
+def test_rows_of_nobody_around_an_append(be, lead, page, hd, fmt, dt):
+    """The batch's rows begin behind `lead` pages and tokens of somebody else's rows (NaN), and more of those follow: bytes, scales and tables of the
+    whole pool are the model's, whether the batch's first sequence is the table's first, new, continued, or next to a row that is full."""
+    kv, max_pages = 2, 4
+    rng = np.random.default_rng(page + hd + 8 * lead[0] + lead[1])
+    for order in ([0, 2], [2, 0], [2], [0], [3, 0, 2]):
+        c, m = both(be, n_pages=24, max_seqs=4, max_pages=max_pages, page=page, kv=kv, hd=hd, fmt=fmt)
+        c.extend(i32([1, 2]), i32([max_pages * page, page + 3])), m.extend([1, 2], [max_pages * page, page + 3])
+        append(c, m, [1, 2], [tuple(values(rng, n, kv, hd, dt) for _ in range(2)) for n in (max_pages * page, page + 3)])
+        new = {0: 1, 2: 2 * page, 3: page}
+        n = [new[s] for s in order]
+        c.extend(i32(order), i32(n)), m.extend(order, n)
+        xs = [tuple(values(rng, k, kv, hd, dt, 4.0) for _ in range(2)) for k in n]
+        front, behind = lead[0] * page + lead[1], page + 1
+        k, v = (torch.cat([torch.full((front, kv, hd), float("nan"), dtype=DT[dt]).cuda()] + [x[i] for x in xs]
+                          + [torch.full((behind, kv, hd), float("nan"), dtype=DT[dt]).cuda()]) for i in (0, 1))
+        c.append(0, k, v, i32(order), i32(front + np.cumsum([0] + n)))
+        for s, x in zip(order, xs):
+            for name, t in zip("kv", x):
+                m.append(0, name, s, t.double().cpu().numpy())
+        same_tables(c, m)
+        assert c.check() == m.result[1]
+        for name, q, scale in (("k", c.k, c.k_scale), ("v", c.v, c.v_scale)):
+            assert np.array_equal(q.float().cpu().numpy(), m.q[name]) and np.array_equal(scale.cpu().numpy(), m.scale[name])
