@@ -322,7 +322,7 @@ class Backend:
                                                    kv_heads, head_dim, float(scale) if scale is not None else head_dim ** -0.5)
         if rc != TPB_OK:
             self._check(rc)
-        self.launches += 1
+        self.launches += tokens > 0 and cu.shape[0] > 1
         return out
 
     def _packed_ld(self, name: str, t: torch.Tensor, tokens: int, heads: int, head_dim: int) -> int:

@@ -134,7 +134,7 @@ class KvCache:
         rc = self._calls.tpb_kv_append(be._hv, be._stream(), self._d, layer, k.data_ptr(), ld_k, v.data_ptr(), ld_v, dtype, ids, at, n, rows)
         if rc != TPB_OK:
             be._check(rc)
-        be.launches += 1
+        be.launches += n > 0 and rows > 0
 
     def read(self, layer: int, seqs: torch.Tensor, cu: torch.Tensor, rows: int, start: Optional[torch.Tensor] = None,
              dtype: torch.dtype = torch.float32, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -155,7 +155,7 @@ class KvCache:
                                      None if start is None else self._ints("start", start, n), at, n, rows)
         if rc != TPB_OK:
             be._check(rc)
-        be.launches += 1
+        be.launches += n > 0 and rows > 0
         return k, v
 
     def attention(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, cu: torch.Tensor, heads: int, scale: Optional[float] = None,
@@ -178,7 +178,8 @@ class KvCache:
                                           None if work is None else work.data_ptr(), 0 if work is None else self._workspace_bytes)
         if rc != TPB_OK:
             be._check(rc)
-        be.launches += 1
+        if n > 0 and rows > 0:
+            be.launches += 1 if work is None else 2
         return out
 
     # -- pages -----------------------------------------------------------------------

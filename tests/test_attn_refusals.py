@@ -254,3 +254,32 @@ def test_every_new_page_has_one_place_and_no_place_another_page(page_at_place):
         shift, first, n_new = rnd.choice([4, 5, 6]), rnd.randint(0, 1 << 29), rnd.randint(1, 1 << 20)
         pg = page_at_place(rnd.randint(0, 1 << 23), rnd.randint(0, 1 << 22), rnd.randint(0, 1 << 26), first, first + n_new, shift)
         assert pg == -1 or first >> shift <= pg <= (first + n_new - 1) >> shift
+
+
+def test_launches_are_counted_as_they_are_made():
+    """Backend.launches counts kernels: attention over the cache is two where a workspace joins parts, and a call with nothing to do is none."""
+    class Calls:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    be = cpu_backend()
+    be._hv, be._stream, be.launches, be._attn_calls = 0, lambda: 0, 0, Calls()
+    c = KvCache.__new__(KvCache)
+    c.be, c.kv_heads, c.head_dim, c._index, c._calls, c._d, c._like = be, 2, 64, -1, Calls(), 0, {}
+    c._scale, c._no_workspace, c._scratch, c._workspace_bytes = 0.125, _lib.KV_SHORT, torch.empty(8, dtype=torch.uint8), 64
+    ids, cu, none = torch.zeros(1, dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    zero = torch.zeros(1, dtype=torch.int32)
+    x, q = torch.zeros(5, 128), torch.zeros(5, 256)
+    b = q.bfloat16()
+    for call, want in ((lambda: c.append(0, x, x, ids, cu), 1), (lambda: c.append(0, x[:0], x[:0], ids, cu), 0),
+                       (lambda: c.append(0, x, x, none, zero), 0),
+                       (lambda: c.read(0, ids, cu, 5), 1), (lambda: c.read(0, ids, cu, 0), 0), (lambda: c.read(0, none, zero, 5), 0),
+                       (lambda: c.attention(0, q, ids, cu, 4), 2), (lambda: c.attention(0, q, ids, cu, 4, max_len=257), 2),
+                       (lambda: c.attention(0, q, ids, cu, 4, max_len=256), 1), (lambda: c.attention(0, q[:0], ids, cu, 4), 0),
+                       (lambda: c.attention(0, q, none, zero, 4), 0),
+                       (lambda: be.attentionPacked(b, b[:, :128], b[:, :128], cu, 4, 2, 64), 1),
+                       (lambda: be.attentionPacked(b, b[:, :128], b[:, :128], zero, 4, 2, 64), 0),
+                       (lambda: be.attentionPacked(b[:0], b[:0, :128], b[:0, :128], cu, 4, 2, 64), 0)):
+        before = be.launches
+        call()
+        assert be.launches - before == want

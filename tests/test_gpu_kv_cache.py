@@ -637,3 +637,19 @@ def test_rows_of_nobody_around_an_append(be, lead, page, hd, fmt, dt):
         assert c.check() == m.result[1]
         for name, q, scale in (("k", c.k, c.k_scale), ("v", c.v, c.v_scale)):
             assert np.array_equal(q.float().cpu().numpy(), m.q[name]) and np.array_equal(scale.cpu().numpy(), m.scale[name])
+
+
+def test_launches_are_the_kernels_of_a_captured_call(be):
+    from graph_nodes import kernels
+    c, m = filled(be, [300, 20], "s8", 16, 2, 64, 1)
+    ids, cu, src, free, one = i32([0, 1]), i32([0, 1, 2]), i32([0]), i32([2]), i32([1, 1])
+    x, q = torch.zeros((2, 128)).cuda(), torch.zeros((2, 256)).cuda()
+    b = q.bfloat16()
+    for call in (lambda: c.extend(ids, one), lambda: c.append(0, x, x, ids, cu), lambda: c.append(0, x[:0], x[:0], ids, cu),
+                 lambda: c.read(0, ids, cu, 2), lambda: c.attention(0, q, ids, cu, 4), lambda: c.attention(0, q, ids, cu, 4, max_len=256),
+                 lambda: c.attention(0, q, ids, cu, 4, max_len=400), lambda: c.attention(0, q[:0], ids, cu, 4), lambda: c.truncate(ids, one),
+                 lambda: c.fork(src, free), lambda: c.compact(), lambda: c.truncate(free),
+                 lambda: be.attentionPacked(b, b[:, :128], b[:, 128:], cu, 4, 2, 64)):
+        before = be.launches
+        made = kernels(call)
+        assert len(made) == be.launches - before, [k.name for k in made]
