@@ -61,10 +61,13 @@ const char *tpb_status_string(int status);
 
 /* Reads (and clears) the device status word that bounded waits inside the
  * kernels write when they give up.  Synchronises `stream` first.  Returns
- * TPB_OK, TPB_ERR_TIMEOUT or TPB_ERR_STATE; *detail (optional) receives the raw word:
- * (role << 24) | stage, role 1 = tile loader, 2 = MMA issuer, 3 = epilogue.  A role of 32 or
- * more is no wait that ran out but a key / value cache whose contents do not fit the call
- * (stage 1 = sequence id, 2 = page, 3 = length, 4 = rows that are not the last extension's): TPB_ERR_STATE. */
+ * TPB_OK, TPB_ERR_TIMEOUT or TPB_ERR_STATE; *detail (optional) receives the raw word,
+ * (role << 24) | stage:
+ *   role 32   no wait that ran out but a key / value cache whose contents do not fit the call: TPB_ERR_STATE.
+ *             Stage 1 = sequence id, 2 = page, 3 = length, 4 = rows that are not the last extension's
+ *   others    a wait that ran out: TPB_ERR_TIMEOUT.  0xBA: tpb_peer_barrier's.  Below 32: one inside a kernel, which numbers its
+ *             roles for itself (int8 GEMM: 1 = tile loader, 2 = MMA issuer, 3 = epilogue; packed attention: 12 = loads and
+ *             the next pair of tiles, 13 = MMA issuer, 14 = softmax and output, 15 = the look over V, 16 = waiting for a pair) */
 int tpb_status_poll(tpb_handle_t h, tpb_stream_t stream, uint32_t *detail);
 
 /* Device facts the host side sizes its work with. */

@@ -96,8 +96,8 @@ class Backend:
             raise TpbError(rc, self.lib.tpb_last_error(self.h).decode())
 
     def status_poll(self) -> int:
-        """Synchronises and raises TpbError(TPB_ERR_TIMEOUT) if a bounded
-        device-side wait gave up."""
+        """Synchronises and raises TpbError(TPB_ERR_TIMEOUT) if a bounded device-side wait gave up, or TpbError(TPB_ERR_STATE) if a kernel
+        met a key / value cache that does not fit its call; whichever kernel of this backend was the first since the last poll."""
         detail = C.c_uint32(0)
         rc = self.lib.tpb_status_poll(self.h, self._stream(), C.byref(detail))
         self._check(rc)

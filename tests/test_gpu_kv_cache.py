@@ -653,3 +653,33 @@ def test_launches_are_the_kernels_of_a_captured_call(be):
         before = be.launches
         made = kernels(call)
         assert len(made) == be.launches - before, [k.name for k in made]
+
+
+def test_status_words_of_a_cache_and_of_a_wait(be):
+    """Role 32 alone is a cache that does not fit (TPB_ERR_STATE); a wait that ran out is TPB_ERR_TIMEOUT, the peer barrier's with its 0xBA above 32."""
+    import ctypes as C
+
+    from tensorpencil_b200 import _lib
+
+    def poll():
+        word = C.c_uint32(0)
+        return be.lib.tpb_status_poll(be.h, be._stream(), C.byref(word)), word.value
+
+    c, m = filled(be, [40, 20], "s8", 16, 1, 64, 3)
+    q, x = torch.zeros((1, 128)).cuda(), torch.zeros((1, 64)).cuda()
+    assert poll() == (_lib.TPB_OK, 0)
+    c.attention(0, q, i32([9]), i32([0, 1]), 2)
+    assert poll() == (_lib.TPB_ERR_STATE, (32 << 24) | 1)
+    c.append(0, x, x, i32([0]), i32([0, 1]))
+    assert poll() == (_lib.TPB_ERR_STATE, (32 << 24) | 4)
+    c.table[0, 1], c.lens[1] = -1, -5
+    c.read(0, i32([0]), i32([0, 1]), 1, start=i32([17]))
+    assert poll() == (_lib.TPB_ERR_STATE, (32 << 24) | 2)
+    c.attention(0, q, i32([1]), i32([0, 1]), 2)
+    assert poll() == (_lib.TPB_ERR_STATE, (32 << 24) | 3)
+    flags = [torch.zeros(128, dtype=torch.int32, device="cuda") for _ in range(2)]
+    both = (C.c_void_p * 2)(*[f.data_ptr() for f in flags])
+    be._check(be.lib.tpb_peer_barrier(be.h, be._stream(), both, 2, 0, 1, 50))      # a rank that never comes: gives up after 50 ms
+    status, word = poll()
+    assert status == _lib.TPB_ERR_TIMEOUT and word >> 24 == 0xBA
+    assert poll() == (_lib.TPB_OK, 0)
