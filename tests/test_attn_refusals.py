@@ -283,3 +283,19 @@ def test_launches_are_counted_as_they_are_made():
         before = be.launches
         call()
         assert be.launches - before == want
+
+
+def test_workspaces_are_measured_before_anything_is_launched(lib):
+    """A stand-in handle with SMs: every word of it is written with its own place until the library's answer tells where the number of SMs lies."""
+    buf = (C.c_int32 * (1 << 18))(*range(1, (1 << 18) + 1))
+    handle = (C.addressof(buf) + 255) & ~255
+    word = lib.tpb_device_sm_count(handle)
+    C.memset(buf, 0, C.sizeof(buf))
+    buf[word - 1] = 148
+    assert lib.tpb_device_sm_count(handle) == 148
+    c = C.addressof(desc())
+    need = lib.tpb_kv_attention_workspace_bytes(handle, 64)
+    assert need >= 148 * 2 * 32 * (64 + 3) * 4
+    for max_len in (0, 257, 1 << 20):
+        for work, nbytes in ((4096, need - 1), (4096, need // 2), (4096, 0), (0, need)):
+            assert lib.tpb_kv_attention(handle, None, c, 0, 4096, 256, 4096, 256, 0, 4096, 4096, 1, 1, 4, 0.1, max_len, work, nbytes) == INVALID

@@ -683,3 +683,25 @@ def test_status_words_of_a_cache_and_of_a_wait(be):
     status, word = poll()
     assert status == _lib.TPB_ERR_TIMEOUT and word >> 24 == 0xBA
     assert poll() == (_lib.TPB_OK, 0)
+
+
+def test_a_workspace_that_is_too_small_is_refused(be):
+    from tensorpencil_b200 import _lib
+    c, m = filled(be, [200, 20], "s8", 16, 2, 64, 3)
+    q, out, ids, cu = torch.randn((2, 256)).cuda(), torch.full((2, 256), 7.0).cuda(), i32([0, 1]), i32([0, 1, 2])
+    need = be.lib.tpb_kv_attention_workspace_bytes(be.h, 64)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    call = lambda max_len, ws, n: be.lib.tpb_kv_attention(be.h, be._stream(), c._d, 0, out.data_ptr(), 256, q.data_ptr(), 256,      # noqa: E731
+                                                          _lib.TPB_F32, ids.data_ptr(), cu.data_ptr(), 2, 2, 4, 0.125, max_len, ws, n)
+    assert need > 0
+    for max_len in (0, 257):
+        for n in (0, need // 2, need - 1):
+            assert call(max_len, work.data_ptr(), n) == _lib.TPB_ERR_INVALID_ARG
+        assert call(max_len, None, need) == _lib.TPB_ERR_INVALID_ARG
+    be.status_poll()
+    assert (out == 7.0).all()
+    for max_len, ws, n in ((0, work.data_ptr(), need), (257, work.data_ptr(), need), (256, None, 0)):
+        out.fill_(7.0)
+        assert call(max_len, ws, n) == _lib.TPB_OK
+        be.status_poll()
+        check_attention(c, m, out, q, [0, 1], [1, 1], 4, "f32")
