@@ -479,8 +479,9 @@ int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t
  * one cache are ordered by the caller (one stream, or events), as for any memory; different caches are independent.
  * A page operation either happens as a whole or, with result[0] != TPB_OK, changes nothing (but sets the listed sequences' tail to 0
  * where it is an extension): TPB_ERR_OOM = not enough free pages, TPB_ERR_INVALID_ARG = a sequence id out of range or listed twice, a
- * length that does not fit, a fork onto a sequence in use.  A kernel that meets an id, a page or a length out of range skips it and sets the
- * status word: tpb_status_poll then returns TPB_ERR_STATE. */
+ * length that does not fit, a fork onto a sequence in use.  Such a refusal is in `result` alone, and the next page operation writes over it.  A
+ * kernel that meets an id, a page or a length out of range skips it and sets the status word of the handle (all its caches share it):
+ * tpb_status_poll then returns TPB_ERR_STATE. */
 typedef enum tpb_kv_format { TPB_KV_S8 = 0, TPB_KV_E4M3 = 1 } tpb_kv_format;
 typedef struct tpb_kv_cache {
     void *k, *v;

@@ -212,7 +212,8 @@ class KvCache:
 
     def check(self) -> int:
         """Waits for the device; the number of free pages after the last page operation.  Raises TpbError where that operation was
-        refused, or where a kernel met a sequence, page or length that does not fit."""
+        refused (a refusal of an earlier one is written over), or where a kernel of this cache's backend, another cache's call among
+        them, met a sequence, page or length that does not fit since the last poll."""
         self.be.status_poll()
         status, free, _, needed = self.result.tolist()
         if status != TPB_OK:

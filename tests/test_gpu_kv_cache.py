@@ -705,3 +705,32 @@ def test_a_workspace_that_is_too_small_is_refused(be):
         assert call(max_len, ws, n) == _lib.TPB_OK
         be.status_poll()
         check_attention(c, m, out, q, [0, 1], [1, 1], 4, "f32")
+
+
+def test_what_a_refused_operation_says_and_where(be):
+    """`result` alone tells of a refusal, until the next page operation; what a kernel skips is in the handle's status word, whatever comes after it, and
+    the operation that met it is done."""
+    from tensorpencil_b200 import _lib
+    c, m = both(be, n_pages=6, max_seqs=4, max_pages=4, kv=1)
+    other, _ = both(be, n_pages=2, kv=1)
+    c.extend(i32([0]), i32([40])), m.extend([0], [40])
+    for refused, status in (((c.extend, (i32([1]), i32([64]))), _lib.TPB_ERR_OOM), ((c.fork, (i32([0, 0]), i32([1, 2]), False)), _lib.TPB_ERR_OOM),
+                            ((c.fork, (i32([0]), i32([0]))), _lib.TPB_ERR_INVALID_ARG), ((c.truncate, (i32([0, 0]),)), _lib.TPB_ERR_INVALID_ARG)):
+        refused[0](*refused[1])
+        assert c.result.tolist()[0] == status
+        be.status_poll()
+        c.extend(i32([3]), i32([0]))
+        assert c.check() == 3
+    m.tail[1] = m.tail[3] = 0
+    m.result = c.result.tolist()
+    same_tables(c, m)
+    page = int(c.table[0, 1])
+    c.table[0, 1] = 99
+    c.fork(i32([0]), i32([1]))                             # skips that entry, and is done
+    c.extend(i32([3]), i32([0]))
+    assert c.result.tolist()[0] == _lib.TPB_OK and c.lens.tolist() == [40, 40, 0, 0] and int(c.table[1, 0]) == int(c.table[0, 0])
+    with pytest.raises(_lib.TpbError) as e:
+        other.check()                                      # the word is the handle's
+    assert e.value.status == _lib.TPB_ERR_STATE
+    assert c.check() == 2
+    c.table[0, 1] = page
