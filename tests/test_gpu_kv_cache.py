@@ -736,3 +736,28 @@ def test_what_a_refused_operation_says_and_where(be):
     assert e.value.status == _lib.TPB_ERR_STATE
     assert c.check() == 2
     c.table[0, 1] = page
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads", [1, 8, 16, 24, 32])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_f32_and_f16_rows_keep_both_terms(be, dt, heads, hd, fmt):
+    """Inputs and bounds that one f16 term of the queries or of the weights would not meet (attn_accuracy.py, test_attn_accuracy.py)."""
+    import attn_accuracy as acc
+    page = 64
+    for n in acc.TOKENS:
+        q, k, v, ks, vs = acc.case(fmt, dt, n, heads, hd, n + hd)
+        c, _ = both(be, n_pages=3, max_seqs=1, max_pages=2, page=page, kv=1, hd=hd, fmt=fmt)
+        for t, sc, x, f in ((c.k, c.k_scale, k, ks), (c.v, c.v_scale, v, vs)):
+            x = torch.from_numpy(x)
+            t[0, 2, 0, :n] = (x.to(torch.int8) if fmt == "s8" else x.float().to(torch.float8_e4m3fn)).cuda()
+            sc[0, 2, 0] = f
+        c.table[0, 0], c.lens[0], c.refs[2] = 2, n, 1
+        o, a, s = acc.formula(q, k, v, ks, vs)
+        tol = acc.tolerance(o, a, s, vs, dt)
+        for max_len in (0, n):
+            out = c.attention(0, torch.from_numpy(q.reshape(1, -1)).to(DT[dt]).cuda(), i32([0]), i32([0, 1]), heads, scale=acc.SCALE, max_len=max_len)
+            be.status_poll()
+            err = np.abs(out.double().cpu().numpy().reshape(heads, hd) - o)
+            assert (err <= tol).all(), (n, max_len, float((err / tol).max()))
