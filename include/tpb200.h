@@ -452,7 +452,8 @@ int tpb_attention(tpb_handle_t h, tpb_stream_t stream, void *out, int out_dtype,
  * NaN and infinities included.  A NaN or infinity at a visible place follows the formula.
  * head_dim 64 or 128; heads a multiple of kv_heads and at most 128 times as many; pointers 16-byte aligned, ld_* multiples of 8
  * elements, kv_heads below 65536, scale finite and not negative.  out must not overlap the inputs.  f32 scores and sums; probabilities are rounded to `dtype` for the
- * second product. */
+ * second product.  Scores, |scale * q . k|, stay below 2^22: f32 has no use of their fraction from there on, and finite ones
+ * of 2^26 and more may come out as NaN. */
 int tpb_attention_packed(tpb_handle_t h, tpb_stream_t stream, void *out, int64_t ld_out, const void *q, int64_t ld_q,
                          const void *k, int64_t ld_k, const void *v, int64_t ld_v, int dtype, const int32_t *cu, int n_seqs,
                          int64_t tokens, int heads, int kv_heads, int head_dim, float scale);
@@ -529,7 +530,8 @@ int tpb_kv_compact(tpb_handle_t h, tpb_stream_t stream, const tpb_kv_cache *c);
  * attention  rows are the queries of the sequence's last cu[i+1] - cu[i] tokens, causal among themselves:
  *          out[r] = sum_{j <= p(r)} softmax_j(scale * q[r] . k[j]) v[j],  p(r) = lens - (cu[i+1] - r); zero where p(r) < 0.
  *          heads a multiple of kv_heads, scale finite and not negative.  f32 accuracy for f32 and f16 rows:
- *          q and the probabilities are split in two f16 terms; bf16 rows: one f16 term each (q's is exact).  The cache's values are exact; an
+ *          q and the probabilities are split in two f16 terms; bf16 rows: one f16 term each (q's is exact).  Scores, |scale * q . k|, stay below
+ *          2^22: from there on f32 loses what tells one page's value scale from another's.  The cache's values are exact; an
  *          e4m3 byte that a row of the batch sees must not be NaN (append writes none).
  *          max_len: an upper bound of the lengths that the host knows (0 = none): a hint that saves a launch for short sequences.
  *          workspace: tpb_kv_attention_workspace_bytes(h, head_dim) bytes, 16-byte aligned, of this call alone while it runs; with

@@ -300,7 +300,7 @@ class Backend:
         """Causal attention of whole prompts, packed one behind another: sequence s is the rows cu[s] .. cu[s + 1] - 1 (cu: int32, on the
         device).  q [tokens][heads*hd], k / v [tokens][kv_heads*hd], all bf16 or all f16, contiguous within a row (parts of a fused
         projection's output may be passed as they are); head_dim 64 or 128.  The result has q's type; rows in no sequence are not
-        written."""
+        written.  Scores, |scale * q . k|, stay below 2^22."""
         dtype, tokens, index = q.dtype, q.shape[0], self._index
         if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
             raise TypeError("attentionPacked: q, k and v must all be bfloat16 or all float16")

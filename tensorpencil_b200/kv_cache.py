@@ -161,7 +161,7 @@ class KvCache:
     def attention(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, cu: torch.Tensor, heads: int, scale: Optional[float] = None,
                   max_len: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of each sequence's last cu[i + 1] - cu[i] tokens, whose queries are q's rows ([rows][heads * head_dim], f32, bf16 or
-        f16), over the sequence's cache; the result has q's type.  ``max_len``: an upper bound of the lengths, where the host knows one."""
+        f16), over the sequence's cache; the result has q's type.  Scores, |scale * q . k|, stay below 2^22.  ``max_len``: an upper bound of the lengths, where the host knows one."""
         be, dtype = self.be, self._dtype("q", q)
         rows, n = q.shape[0], seqs.shape[0]
         ld_q = self._rows("q", q, rows, heads, q.dtype)

@@ -239,3 +239,29 @@ def test_large_batches_give_the_bits_of_small_ones(be, lens, heads, kv, hd, dt):
         assert torch.equal(out[rows], be.attentionPacked(q[rows], k[rows], v[rows], offsets([n]), heads, kv, hd)), n
         at += n
     check(out, q, k, v, lens, heads, kv, hd, dt, rows_at_most=20)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_up_to_the_documented_limit(be, hd, dt):
+    """Single products up to 2^22, exact in f32 and 2^14 apart or equal: the row's largest has all the weight, or its equals share it.  What rounding the
+    reference point loses is the same factor for weights and sum."""
+    lens, heads, kv = [1, 5, 300], 2, 1
+    total = sum(lens)
+    g = torch.Generator().manual_seed(hd)
+    q, k = torch.zeros((total, heads, hd)), torch.zeros((total, hd))
+    q[:, 0, 0], q[:, 1, 3] = 2048.0, -2040.0
+    k[:, 0], k[:, 3] = (1024.0 * (1.0 + torch.randint(0, 128, (total,), generator=g) / 128.0) * s for s in (1.0, -1.0))
+    v = torch.randn((total, hd), generator=g)
+    q, k, v = (t.reshape(total, -1).to(DT[dt]).cuda() for t in (q, k, v))
+    out = be.attentionPacked(q, k, v, offsets(lens), heads, kv, hd, scale=1.0)
+    be.status_poll()
+    got, q, k, v = (t.double().cpu().numpy() for t in (out, q, k, v))
+    at = 0
+    for n in lens:
+        for h in range(heads):
+            mine = slice(h * hd, (h + 1) * hd)
+            o, a, _ = attend(q[at:at + n, mine], k[at:at + n], v[at:at + n], np.arange(n), 1.0)
+            tol = tolerance(o, a, np.zeros(n), hd, HALF_STEP[dt], HALF_STEP[dt])
+            assert (np.abs(got[at:at + n, mine] - o) <= tol).all()
+        at += n

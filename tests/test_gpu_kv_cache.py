@@ -761,3 +761,34 @@ def test_f32_and_f16_rows_keep_both_terms(be, dt, heads, hd, fmt):
             be.status_poll()
             err = np.abs(out.double().cpu().numpy().reshape(heads, hd) - o)
             assert (err <= tol).all(), (n, max_len, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("fmt", ["s8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_scores_up_to_the_documented_limit(be, dt, fmt):
+    """Single products up to 2^22, far apart or equal: a row's largest has all the weight, or its equals (of one scale) share it.  Scales are append's, powers
+    of two, whose logarithms the references of the weights hold exactly."""
+    kv, heads, hd = 1, 4, 64
+    lens = [1, 4, 30]
+    c, m = both(be, n_pages=8, max_seqs=3, max_pages=4, kv=kv, hd=hd, fmt=fmt)
+    rng = np.random.default_rng(3)
+    c.extend(i32(range(3)), i32(lens)), m.extend(range(3), lens)
+    xs = []
+    for n in lens:
+        k = np.zeros((n, kv, hd))
+        k[:, 0, 5] = 1024.0 + 1024.0 * rng.permutation(60)[:n] / 64.0       # 16 apart: s8 holds multiples of 16 here
+        if fmt == "e4m3":
+            k[:, 0, 5] = 1024.0 * 2.0 ** -np.arange(n) if n < 5 else 1024.0 * (1.0 + np.arange(n) % 2 / 8.0 * 7.0)
+        xs.append((torch.from_numpy(k).to(DT[dt]).cuda(), values(rng, n, kv, hd, dt)))
+    append(c, m, range(3), xs)
+    q = torch.zeros((3, heads, hd))
+    q[:, :, 5] = torch.tensor([2048.0, 2047.0 if dt != "bf16" else 2040.0, 2000.0, 1500.0])
+    q = q.reshape(3, -1).to(DT[dt]).cuda()
+    out = c.attention(0, q, i32(range(3)), offsets([1] * 3), heads, scale=1.0)
+    be.status_poll()
+    got, q = out.double().cpu().numpy(), q.double().cpu().numpy()
+    for s in range(3):
+        k, v = m.read(0, "k", s)[:, 0], m.read(0, "v", s)[:, 0]
+        o, a, _ = attend(q[s].reshape(heads, hd), k, v, [lens[s] - 1] * heads, 1.0)
+        tol = tolerance(o, a, np.zeros(heads), hd, HALF_STEP[dt], WEIGHTS[dt])
+        assert (np.abs(got[s].reshape(heads, hd) - o) <= tol).all()
