@@ -54,9 +54,14 @@ struct Cfg {
     static constexpr int kMergeLd = HD + 4;
     static constexpr int kMerge = 2 * kRows * kMergeLd * 4;              // where the warps' sums are added up, in pairs
     static constexpr int kSmem = kWarps * kRing + kMerge + kQf;
-    static constexpr int kCtas = NT == 1 ? 3 : 2;                        // per SM
+    // CTAs an SM that the registers are cut for and the grid is sized by.  They all fit its shared memory but for two terms of 32 rows of 128: one at a
+    // time there (20000 tokens, 32 rows a kv head, f32 60 us; with bf16's one term, where two fit, 39; 24 rows, f32 37).
+    static constexpr int kCtas = NT == 1 ? 3 : 2;
+    static constexpr bool kOneFits = HD == 128 && SPLIT && NT == 4;
+    static constexpr int kStatic = 2336 + kRows * 48 + (kQRegs ? 8 : kRows * 8);     // Chunk, the warps' references and sums, q's factors
+    static constexpr int kTaken = (kSmem + kStatic + 127) / 128 * 128 + 1024;        // by a CTA; 1024 of it the system's
     static_assert(kRows <= 32, "rows fit a slot");
-    static_assert(kCtas * (kSmem + 2816 + 1024) <= 228 * 1024 || NT > 1, "three CTAs fit an SM (2816: the static shared memory)");
+    static_assert((kOneFits ? 1 : kCtas) * kTaken <= 228 * 1024 && (!kOneFits || 2 * kTaken > 228 * 1024), "so many CTAs fit an SM");
 };
 constexpr int kMaxCtas = 3, kMaxRows = 32;
 
